@@ -305,6 +305,78 @@ int sh_attention_batched_prefetch(uint64_t q, uint64_t k, uint64_t v, uint64_t o
                                   uint64_t bsq, uint64_t bsk, uint64_t bsv, uint64_t bso, float scale, uint32_t sq,
                                   uint64_t pf0, uint64_t pf0_bytes, uint64_t pf1, uint64_t pf1_bytes);
 
+/* ---- 8-bit paged key / value cache (no counterpart in the reference) -----------------------------------------------
+ * Keys and values of many requests in pages of `bs` tokens, 8-bit codes with one fp32 scale for each page and head:
+ * value = code x scale. A request's tokens 0, 1, ... lie in the pages its row of the block table names, bs to a page.
+ * SH_INT8: two's complement, -127 .. 127. SH_FP8: OCP e4m3 (finite, largest 448). Values are stored with the tokens of a
+ * page consecutive, as the product with the probabilities reads them.
+ * A serving step: sh_kv_slots (where the new tokens go), the projections, sh_rope at the positions it gives,
+ * sh_kv_append, sh_attention_kv. The calls need no device memory of the library's own and no host synchronisation, so a
+ * step captures into a HIP graph whose replays read the lengths of that moment. */
+typedef struct {
+    uint64_t k;           /* codes: pages of [hkv][bs][dh], 16-byte aligned */
+    uint64_t v;           /* codes: pages of [hkv][dh][bs], 16-byte aligned */
+    uint64_t ks, vs;      /* fp32 scales: pages of [hkv] */
+    uint64_t pgk, pgv;    /* bytes from a page to the next, multiples of 16 and >= hkv bs dh; 0: hkv bs dh */
+    uint32_t pgs;         /* floats from a page's scales to the next page's, >= hkv; 0: hkv */
+    uint32_t pages;       /* pages of the cache, pages x bs < 2^31 */
+    uint32_t hkv;         /* key / value heads, 1 .. 1024 */
+    uint32_t dh;          /* head width: a multiple of 16, 16 .. 256 */
+    uint32_t bs;          /* tokens of a page: 16, 32 or 64 */
+    uint32_t fmt;         /* SH_INT8 | SH_FP8 */
+} sh_kv_cache;
+
+/* Block table, slots and lengths of a step, on the GPU. All arrays int32 in GPU memory, written in place:
+ *   table [B][ld]     page of each bs tokens of a request (in / out: the new pages' entries are written)
+ *   lens [B]          tokens each request holds; lens_out [B] (may be lens): with the new ones
+ *   add [B]           tokens each adds (0: none), or < 0: the request has ended, its pages go back
+ *   pool [pages]      ring of free page numbers; state {head, count, -}: its first entry and how many there are (to begin:
+ *                     pool[i] = i, state = {0, pages, 0}); state_out (may be state) {head, count, requests refused}
+ *   row_start [B + 1] first row of each request among the step's new rows, in order, and their total
+ *   slots, pos [rows] of each new row: page x bs + offset, and position in its request; -1 for the rows of a refused
+ *                     request and behind the last row
+ *   kv_len [B]        keys that a request's rows see with themselves (lens + add); 0 for an ended or refused request
+ * Requests take pages in order. One that needs more than are left, whose rows end behind `rows` or whose tokens exceed
+ * ld x bs is refused: its length and table stay, and those after it that need pages are served only if the pages that
+ * it and they ask for together are there. Pages of ended requests can be taken from the next call on. The sum of `add` stays
+ * below 2^31. B x ld and pages x bs below 2^31, B <= 65536. 0, -1 for bad arguments, SH_EHIP. */
+int sh_kv_slots(uint64_t table, uint32_t ld, uint64_t lens, uint64_t lens_out, uint64_t add, uint64_t pool, uint64_t state, uint64_t state_out,
+                uint64_t row_start, uint64_t slots, uint64_t pos, uint64_t kv_len, uint32_t B, uint32_t bs, uint32_t pages, uint32_t rows);
+
+/* New key and value rows (fp16, [rows][hkv dh], leading dims ldk / ldv) into the cache at slots[row] (int32; rows with a
+ * slot outside the cache are skipped). The scale of a page and head is the smallest power of two s >= 2^-32 with
+ * |x| <= 127 s (448 s for SH_FP8) for its tokens, and never smaller than the one its older tokens have; where it grows, they are
+ * rounded to it again. Codes round to nearest even. NaN is stored as 0, infinities as +-65504. A request's new tokens are
+ * consecutive rows with ascending slots within a page, and a page that is written belongs to one request: rows that
+ * put two requests, or one slot twice, into one page leave that page undefined. A first token at offset 0 starts a
+ * page anew; other codes of the page are left as they are. 0, -1, SH_EHIP. */
+int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uint32_t ldv, uint64_t slots, uint32_t rows);
+
+/* Causal attention of new rows over the cache: o = softmax(scale q k^T) v per head, fp32 sums. Request b's rows are
+ * row_start[b] .. row_start[b + 1] - 1 of q / o (fp16, [rows][H dh]; row_start = 0: row b), its keys the first kv_len[b]
+ * tokens of its table row, and its last row sees all of them, each earlier row one key less. window > 0: a row sees
+ * only its last `window` keys; pages wholly before every row's window are not read. Head h reads key / value head h / (H / hkv). Keys
+ * in pages outside the cache (table entries < 0 or >= pages) are left out. A row that sees no key gets zeros; rows of no
+ * request are left as they are, as are a request's rows beyond its first max_q. max_q: an upper bound of a request's rows. ws: scratch
+ * of at least sh_attention_kv_ws_bytes(c, B, rows, max_q, H, ld_table) bytes, 16-byte aligned, that no call running at the same
+ * time uses (another stream, or a graph replayed beside this one, needs its own); what it holds need not be kept.
+ * 0, -1 for bad arguments, -2 for too small a ws, SH_EHIP. Deterministic; how keys are shared out depends on the whole
+ * batch, so a request's low bits may differ with its neighbours. */
+int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table, uint32_t ld_table, uint64_t kv_len, uint64_t row_start,
+                    uint32_t B, uint32_t rows, uint32_t max_q, uint32_t H, uint32_t ldq, uint32_t ldo, float scale, uint32_t window,
+                    uint64_t ws, uint64_t ws_bytes);
+uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t rows, uint32_t max_q, uint32_t H, uint32_t ld_table);
+
+/* Few rows times a weight of 4-bit codes (no counterpart in the reference): z = act(x . W + bias) rounded to fp16, then
+ * [+ residual, rounded again], W[k][n] = (code[k][n] - zero[k / group][n]) scale[k / group][n]. w: words [K / 8][N]
+ * (uint32, leading dim ldw), bits 4 j .. 4 j + 3 of word (i, n) the code of k = 8 i + j. scale: fp16 [ceil(K / group)][N],
+ * zero: one byte (0 .. 15) each, same shape and leading dim lds; zero = 0: 8 throughout. K a multiple of 8, group a multiple of 32
+ * (the last group may be short). epi: bias, act, residual as sh_gemm_ex (splits 0 or 1, no LayerNorm fold, no row
+ * partials). fp32 sums, scales applied in fp32. Written for M up to 64; more rows read the weight again for every 64. A
+ * row's bits do not depend on M or on the other rows. 0, -1 for bad arguments, SH_EHIP. */
+int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero, uint64_t z, uint32_t M, uint32_t N, uint32_t K, uint32_t group,
+               uint32_t ldx, uint32_t ldw, uint32_t lds, uint32_t ldz, const sh_gemm_epi *epi);
+
 /* LayerNorm with separate input / output leading dims (fused residual stream layouts). */
 void sh_layernorm_ld(uint64_t y, uint64_t x, uint64_t gamma, uint64_t beta, uint32_t rows, uint32_t cols,
                      uint32_t ldy, uint32_t ldx, float eps);

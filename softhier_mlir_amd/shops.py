@@ -42,6 +42,12 @@ class sh_gemm_epi(C.Structure):
                 ("ln_eps", C.c_float)]
 
 
+class sh_kv_cache(C.Structure):
+    """The 8-bit paged key / value cache of sh_kv_append and sh_attention_kv (additive)."""
+    _fields_ = [("k", C.c_uint64), ("v", C.c_uint64), ("ks", C.c_uint64), ("vs", C.c_uint64), ("pgk", C.c_uint64), ("pgv", C.c_uint64),
+                ("pgs", C.c_uint32), ("pages", C.c_uint32), ("hkv", C.c_uint32), ("dh", C.c_uint32), ("bs", C.c_uint32), ("fmt", C.c_uint32)]
+
+
 u32, u64, i32, f32, i16 = C.c_uint32, C.c_uint64, C.c_int, C.c_float, C.c_uint16
 _P = C.c_char_p
 _SIGS: dict[str, tuple] = {
@@ -92,6 +98,12 @@ _SIGS: dict[str, tuple] = {
     "sh_attention_batched": (i32, [u64, u64, u64, u64, u32, u32, u32, u32, u32, u32, u32, u32, u64, u64, u64, u64, f32, u32]),
     "sh_attention_batched_prefetch": (i32, [u64, u64, u64, u64, u32, u32, u32, u32, u32, u32, u32, u32, u64, u64, u64, u64, f32,
                                             u32, u64, u64, u64, u64]),
+    # 8-bit key / value cache, 4-bit weights
+    "sh_kv_slots": (i32, [u64, u32, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u32, u32, u32, u32]),
+    "sh_kv_append": (i32, [C.POINTER(sh_kv_cache), u64, u64, u32, u32, u64, u32]),
+    "sh_attention_kv": (i32, [u64, u64, C.POINTER(sh_kv_cache), u64, u32, u64, u64, u32, u32, u32, u32, u32, u32, f32, u32, u64, u64]),
+    "sh_attention_kv_ws_bytes": (u64, [C.POINTER(sh_kv_cache), u32, u32, u32, u32, u32]),
+    "sh_gemm_w4": (i32, [u64, u64, u64, u64, u64, u32, u32, u32, u32, u32, u32, u32, u32, C.POINTER(sh_gemm_epi)]),
     # test helpers
     "sh_test_fill_int_fp16": (None, [u64, u32, u32, u32, u32, i32, i32]),
     "sh_test_fill_fp16": (None, [u64, u32, u32, u32, u32, i32, i32, f32]),
@@ -151,6 +163,11 @@ def epi(bias: int = 0, bias_fmt: int = SH_BIAS_FP16, act: int = SH_ACT_NONE, res
         splits: int = 1, ln_stats: int = 0, ln_c: int = 0, stats_out: int = 0, ln_parts: int = 0,
         ln_eps: float = 0.0) -> sh_gemm_epi:
     return sh_gemm_epi(bias, bias_fmt, act, residual, ldr, splits, ln_stats, ln_c, stats_out, ln_parts, ln_eps)
+
+
+def kv_cache(k: int, v: int, ks: int, vs: int, pages: int, hkv: int, dh: int, bs: int, fmt: int = SH_INT8, pgk: int = 0,
+             pgv: int = 0, pgs: int = 0) -> sh_kv_cache:
+    return sh_kv_cache(k, v, ks, vs, pgk, pgv, pgs, pages, hkv, dh, bs, fmt)
 
 
 def addr(t, elem_offset: int = 0) -> int:
