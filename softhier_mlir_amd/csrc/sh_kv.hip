@@ -174,7 +174,8 @@ struct AppendArgs {
     const uint16_t *k, *v;
     uint64_t ldk, ldv;
     const int32_t *slots;
-    uint32_t rows;
+    uint32_t rows, rg;
+    ShDiv dch;                             // by dh / 8
 };
 
 // |x| of a pair of halves as integers (monotone), NaN as 0, infinity as 65504.
@@ -182,10 +183,7 @@ __device__ __forceinline__ uint32_t abs_bits(uint32_t h) {
     const uint32_t a = h & 0x7FFFu;
     return a > 0x7C00u ? 0u : min(a, 0x7BFFu);
 }
-__device__ __forceinline__ float clean(uint16_t h) {
-    const float f = __uint_as_float((__float_as_uint(sh_dev_h2f((uint16_t)abs_bits(h)))) | ((uint32_t)(h & 0x8000u) << 16));
-    return f;
-}
+__device__ __forceinline__ float clean(uint16_t h) { return sh_dev_h2f((uint16_t)(abs_bits(h) | (h & 0x8000u))); }
 
 // The smallest power of two s >= 2^-32 with amax <= s Q, Q = 127 or 448: amax = f 2^e with f in [0.5, 1), Q = q 2^x likewise.
 template <bool FP8>
@@ -196,62 +194,150 @@ __device__ __forceinline__ float pow2_scale(float amax) {
     const int p = amax > 0.f ? max(f <= q ? e - x : e - x + 1, -32) : -32;
     return __uint_as_float((uint32_t)(p + 127) << 23);
 }
-// The code of x (already divided by its scale): nearest, ties to even.
+// The codes of four values already divided by their scale, in a word: nearest, ties to even.
 template <bool FP8>
-__device__ __forceinline__ uint8_t code_of(float x) {
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
     if constexpr (FP8) {
-        x = __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
-        return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false);
+        const auto lim = [](float x) { return __builtin_amdgcn_fmed3f(x, -448.f, 448.f); };
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lim(c), lim(d), __builtin_amdgcn_cvt_pk_fp8_f32(lim(a), lim(b), 0, false), true);
     } else {
-        return (uint8_t)(int8_t)__builtin_amdgcn_fmed3f(__builtin_rintf(x), -127.f, 127.f);
+        const auto q = [](float x) { return (uint32_t)(int)__builtin_amdgcn_fmed3f(__builtin_rintf(x), -127.f, 127.f); };
+        const uint32_t lo = __builtin_amdgcn_perm(q(b), q(a), 0x0C0C0400u), hi = __builtin_amdgcn_perm(q(d), q(c), 0x04000C0Cu);
+        return lo | hi;
     }
 }
 template <bool FP8>
-__device__ __forceinline__ float value_of(uint8_t c) {
-    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8(c, 0);
-    else return (float)(int8_t)c;
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+    if constexpr (FP8)
+        return codes4<FP8>(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * ratio,
+                           __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * ratio, __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * ratio);
+    else
+        return codes4<FP8>((float)(int8_t)w * ratio, (float)(int8_t)(w >> 8) * ratio, (float)(int8_t)(w >> 16) * ratio, (float)(int8_t)(w >> 24) * ratio);
 }
 
-// One wave per (row, head, k or v); the wave of a page's first new row does that page, the others end.
-template <bool FP8>
-__global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
-    const uint32_t lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y, isv = blockIdx.z;
-    if (r >= a.rows) return;
+// A workgroup takes RG rows, one head and keys or values, and does the pages whose first new row is among its rows, one after
+// the other. A thread holds four tokens by eight columns of the page (one such item), the tokens at the page's own multiples of
+// four: four 16-byte loads; after the page's largest value is known, the codes of a key's eight columns are one 8-byte store a
+// token, those of a value's four tokens one 4-byte store a column (a page of values has its tokens consecutive). At most 64 x 256
+// values a page: 512 items. Bound by HBM: 2 bytes read and 1 written a value; written pages are whole lines in L2.
+template <bool FP8, int NT>
+__global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
+    __shared__ uint32_t s_top[NT / 64];
     const KvCache &c = a.c;
-    const uint32_t cap = c.pages << c.lbs;
-    const uint32_t s0 = (uint32_t)a.slots[r];
-    if (s0 >= cap) return;
-    const uint32_t off = s0 & (c.bs - 1), page = s0 >> c.lbs;
-    if (off && r && (uint32_t)a.slots[r - 1] == s0 - 1) return;
-    // rows of this page: lane i holds row r + i's slot (bs <= 64)
-    const bool mine = r + lane < a.rows && lane < c.bs - off && (uint32_t)a.slots[min(r + lane, a.rows - 1)] == s0 + lane;
-    const uint64_t has = __ballot(mine);
-    const uint32_t n = ~has ? __builtin_ctzll(~has) : 64u;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, r0 = blockIdx.x * a.rg, h = blockIdx.y, isv = blockIdx.z;
+    const uint32_t cap = c.pages << c.lbs, dh = c.dh, nch = dh / 8;
+    // the first row of a page's run: it begins a page, or the row before does not precede it. Lane i: row r0 + i
+    const uint32_t rl = r0 + lane;
+    const uint32_t sl = rl < a.rows ? (uint32_t)a.slots[rl] : ~0u;
+    const uint32_t sb = rl < a.rows && rl ? (uint32_t)a.slots[rl - 1] : ~0u;
+    uint64_t lead = __ballot(lane < a.rg && sl < cap && (!(sl & (c.bs - 1)) || !rl || sb != sl - 1));
     const uint64_t ld = isv ? a.ldv : a.ldk;
-    const uint16_t *src = (isv ? a.v : a.k) + (uint64_t)r * ld + (uint64_t)h * c.dh;
-    uint8_t *dst = isv ? c.v + page * c.pgv : c.k + page * c.pgk;
-    dst += (uint64_t)h * c.bs * c.dh;
-    float *sp = (isv ? c.vs : c.ks) + (uint64_t)page * c.pgs + h;
-    const uint32_t items = n * c.dh;
-    uint32_t top = 0;
-    for (uint32_t i = lane; i < items; i += 64) top = max(top, abs_bits(src[(i / c.dh) * ld + i % c.dh]));
+    while (lead) {
+        const uint32_t f = __builtin_ctzll(lead), r = r0 + f;
+        lead &= lead - 1;
+        const uint32_t s0 = (uint32_t)__builtin_amdgcn_readlane((int)sl, (int)f), off = s0 & (c.bs - 1), page = s0 >> c.lbs;
+        // the run's rows, a page's rest of at most 64: among the rows read, or read again
+        uint64_t has;
+        if (f + c.bs - off <= 64) has = __ballot(lane >= f && lane - f < c.bs - off && sl == s0 + lane - f) >> f;
+        else has = __ballot(lane < c.bs - off && r + lane < a.rows && (uint32_t)a.slots[min(r + lane, a.rows - 1)] == s0 + lane);
+        const uint32_t n = ~has ? (uint32_t)__builtin_ctzll(~has) : 64u, end = off + n;
+        const uint16_t *src = (isv ? a.v : a.k) + (uint64_t)r * ld + (uint64_t)h * dh;
+        uint8_t *dst = (isv ? c.v + page * c.pgv : c.k + page * c.pgk) + (uint64_t)h * c.bs * dh;
+        float *sp = (isv ? c.vs : c.ks) + (uint64_t)page * c.pgs + h;
+        const float was = off ? *sp : 0.f;
+        const uint32_t blk0 = off / 4, items = ((end + 3) / 4 - blk0) * nch;
+        uint4 x[4];
+        uint32_t top = 0;
+        const uint32_t bl = sh_div(tid, a.dch), ch = tid - bl * nch, t0 = 4 * (blk0 + bl);
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    const float was = off ? *sp : 0.f, need = pow2_scale<FP8>(sh_dev_h2f((uint16_t)top)), s = fmaxf(was, need);
-    if (off && s != was) {
-        const float ratio = was / s;
-        for (uint32_t i = lane; i < off * c.dh; i += 64) {
-            const uint32_t t = i / c.dh, d = i % c.dh;
-            uint8_t *p = isv ? dst + d * c.bs + t : dst + t * c.dh + d;
-            *p = code_of<FP8>(value_of<FP8>(*p) * ratio);
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t t = t0 + j;
+            x[j] = make_uint4(0, 0, 0, 0);
+            if (tid < items && t >= off && t < end) x[j] = sh_ld16_any(src + (uint64_t)(t - off) * ld + 8 * ch);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, max(abs_bits(w[e] & 0xFFFFu), abs_bits(w[e] >> 16)));
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        if constexpr (NT > 64) {
+            __syncthreads();                                        // the last page's maxima are read
+            if (lane == 0) s_top[tid / 64] = top;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NT / 64; ++i) top = max(top, s_top[i]);
+        }
+        const float s = fmaxf(was, pow2_scale<FP8>(sh_dev_h2f((uint16_t)top)));
+        if (off && s != was) {                                      // the page's older tokens: whole words, and the bytes beside the new ones
+            const float ratio = was / s;
+            uint32_t *d32 = (uint32_t *)dst;
+            if (!isv) {
+                for (uint32_t i = tid; i < off * dh / 4; i += NT) d32[i] = rescale4<FP8>(d32[i], ratio);
+            } else {
+                for (uint32_t i = tid; i < blk0 * dh; i += NT) {
+                    uint32_t *p = d32 + (i / blk0) * (c.bs / 4) + i % blk0;
+                    *p = rescale4<FP8>(*p, ratio);
+                }
+                for (uint32_t i = tid; i < (off & 3) * dh; i += NT) {
+                    uint8_t *p = dst + (i % dh) * c.bs + 4 * blk0 + i / dh;
+                    *p = (uint8_t)rescale4<FP8>(*p, ratio);
+                }
+            }
+        }
+        // x / s: the reciprocal of a power of two is exact (only a caller's own scales are not one)
+        const bool p2 = (__float_as_uint(s) & 0x7FFFFFu) == 0;
+        const float inv = 1.f / s;
+        if (tid < items) {
+            float v[4][8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = clean((uint16_t)(w[e / 2] >> (16 * (e & 1))));
+            }
+            if (p2) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j / 8][j % 8] *= inv;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j / 8][j % 8] /= s;
+            }
+            if (!isv) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t t = t0 + j;
+                    if (t >= off && t < end)
+                        *(uint2 *)(dst + t * dh + 8 * ch) = make_uint2(codes4<FP8>(v[j][0], v[j][1], v[j][2], v[j][3]), codes4<FP8>(v[j][4], v[j][5], v[j][6], v[j][7]));
+                }
+            } else {
+                const bool whole = t0 >= off && t0 + 4 <= end;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    uint8_t *p = dst + (8 * ch + e) * c.bs + t0;
+                    const uint32_t w = codes4<FP8>(v[0][e], v[1][e], v[2][e], v[3][e]);
+                    if (whole) *(uint32_t *)p = w;
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (t0 + j >= off && t0 + j < end) p[j] = (uint8_t)(w >> (8 * j));
+                }
+            }
+        }
+        if (tid == 0) *sp = s;
     }
-    for (uint32_t i = lane; i < items; i += 64) {
-        const uint32_t t = i / c.dh, d = i % c.dh;
-        uint8_t *p = isv ? dst + d * c.bs + off + t : dst + (off + t) * c.dh + d;
-        *p = code_of<FP8>(clean(src[t * ld + d]) / s);
-    }
-    if (lane == 0) *sp = s;
+}
+
+template <bool FP8>
+void launch_append(AppendArgs &a, hipStream_t st) {
+    const dim3 grid(sh_cdiv(a.rows, a.rg), a.c.hkv, 2);
+    const uint32_t items = a.c.bs * a.c.dh / 32;
+    if (items <= 64) hipLaunchKernelGGL((k_kv_append<FP8, 64>), grid, dim3(64), 0, st, a);
+    else if (items <= 128) hipLaunchKernelGGL((k_kv_append<FP8, 128>), grid, dim3(128), 0, st, a);
+    else if (items <= 256) hipLaunchKernelGGL((k_kv_append<FP8, 256>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_kv_append<FP8, 512>), grid, dim3(512), 0, st, a);
 }
 
 }  // namespace
@@ -305,9 +391,11 @@ int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uin
     a.ldk = ldk; a.ldv = ldv;
     a.slots = (const int32_t *)slots;
     a.rows = rows;
-    const dim3 grid(sh_cdiv(rows, 4), c->hkv, 2);
-    if (c->fmt == SH_FP8) hipLaunchKernelGGL(k_kv_append<true>, grid, dim3(256), 0, sh_stream(), a);
-    else hipLaunchKernelGGL(k_kv_append<false>, grid, dim3(256), 0, sh_stream(), a);
+    a.dch = sh_make_div(c->dh / 8);
+    // rows of a workgroup: one while all pages run at once, then few enough that most have a page to do in a prompt
+    a.rg = rows <= 512 ? 1 : rows <= 4096 ? 4 : c->bs;
+    if (c->fmt == SH_FP8) launch_append<true>(a, sh_stream());
+    else launch_append<false>(a, sh_stream());
     return sh_launch_ok("sh_kv_append") ? 0 : SH_EHIP;
 }
 

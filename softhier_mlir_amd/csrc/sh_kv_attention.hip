@@ -20,7 +20,10 @@ namespace {
 
 constexpr uint32_t KT = 64;                // keys of a tile
 constexpr uint32_t QT = 16;                // rows of a tile
-constexpr uint32_t GROUPS = 512;           // workgroups: two for each CU
+constexpr uint32_t GROUPS = 512;           // workgroups at most: two for each CU
+constexpr uint32_t WHOLE_TILES = 4;        // key tiles of an item for each wave up to which it is not cut between workgroups
+
+struct ChunkUnit { uint32_t parts, r0, nrow, qt, h, step, pad[2]; };      // a cut unit: of an item's first part; parts 0: another part
 
 struct AttnArgs {
     KvCache c;
@@ -28,9 +31,10 @@ struct AttnArgs {
     uint16_t *o;
     const int32_t *table, *kv_len, *row_start;
     uint64_t ldq, ldo;
-    uint32_t ld, B, rows, max_q, grp, prow, window, groups;
+    uint32_t ld, B, rows, max_q, grp, prow, window, groups, fast, whole;
     float sc;                              // scale x log2 e
     float *part, *ml;                      // partials [groups][2][prow][dh], their (max, sum) [groups][2][prow][2]
+    ChunkUnit *unit;                       // [2 CUT]
     int4 *meta;                            // [groups]: request, item, last workgroup of the item begun here (-1: none)
 };
 
@@ -39,6 +43,7 @@ struct Seq {
     int32_t L;
 };
 
+template <uint32_t QTILE>
 __device__ __forceinline__ Seq seq_of(const AttnArgs &a, uint32_t b) {
     Seq s;
     int32_t r0 = (int32_t)b, r1 = (int32_t)b + 1;
@@ -48,7 +53,7 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, uint32_t b) {
     s.nf = r1 > r0 ? (uint32_t)(r1 - r0) : 0u;
     s.n = min(min(s.nf, a.max_q), s.r0 < a.rows ? a.rows - s.r0 : 0u);
     s.L = min(max(a.kv_len[b], 0), (int32_t)(a.ld << a.c.lbs));
-    s.nqt = (s.n * a.grp + QT - 1) / QT;
+    s.nqt = (s.n * a.grp + QTILE - 1) / QTILE;
     const int64_t lo = a.window ? max((int64_t)s.L - s.nf + 1 - a.window, (int64_t)0) : 0;
     s.ft = (uint32_t)lo / KT;
     s.nt = s.n ? max((uint32_t)(s.L + KT - 1) / KT, s.ft + 1) - s.ft : 0u;
@@ -91,44 +96,95 @@ __device__ __forceinline__ void store4(uint16_t *p, float a, float b, float c, f
     *(sh_u2v_a2 *)p = (sh_u2v_a2){__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
 }
 
+// Sum of the lanes up to this one (v_add with DPP moves: shifts within rows of 16, then the rows' last lanes broadcast).
+__device__ __forceinline__ uint32_t wave_scan32(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+__device__ __forceinline__ uint64_t div64(uint64_t a, uint32_t d) { return a >> 32 ? a / d : (uint64_t)((uint32_t)a / d); }
+__device__ __forceinline__ Seq lane_seq(const Seq &s, uint32_t b) {
+    const auto rl = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)b); };
+    return Seq{rl(s.r0), rl(s.n), rl(s.nf), rl(s.nqt), rl(s.ft), rl(s.nt), (int32_t)rl((uint32_t)s.L)};
+}
+
 // All tiles of all (request, head, row tile) items, one behind the other, are dealt out evenly: workgroup i of N takes
-// tiles i T / N .. (i + 1) T / N, its four waves a quarter each. A wave that has an item from its first tile to its last stores the
+// tiles i T / N .. (i + 1) T / N, its NW waves a share each. A wave that has an item from its first tile to its last stores the
 // result; parts of items are joined through LDS, and what crosses workgroups through `part` by k_kv_join. The lengths are
 // on the GPU only, so the host cannot choose a split; this one keeps every CU busy whether one request is long or many are short.
-template <int DP, bool FP8>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) {
+// `whole`: where the table bounds an item to a few tiles for each wave, items are not cut between workgroups (each belongs to the
+// one its first tile falls to) and the joining launch is not made.
+// Up to 64 requests: a lane holds a request, every wave finds its tiles by itself; otherwise through LDS.
+template <int DP, bool FP8, bool FULL, int NW>
+__global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     constexpr int NP = DP / 64, MT = DP / 16;
-    extern __shared__ float s_o[];                                  // [8][prow][DP]
-    __shared__ float s_ml[8][QT][2];
-    __shared__ uint32_t s_seg[8][5];                                // request, item, first tile, end tile, tiles; request -1: none
-    __shared__ uint64_t s_sum[4], s_base[4];
-    __shared__ uint32_t s_b[4];
+    extern __shared__ float s_o[];                                  // [2 NW][prow][DP]
+    __shared__ float s_ml[2 * NW][QT][2];
+    __shared__ uint32_t s_seg[2 * NW][5];                           // request, item, first tile, end tile, tiles; request -1: none
+    __shared__ uint64_t s_sum[NW], s_base[NW];
+    __shared__ uint32_t s_b[NW];
     const KvCache &c = a.c;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
-    const uint32_t dh = c.dh;
+    const uint32_t dh = FULL ? DP : c.dh, wg = blockIdx.x;
 
     // ---- this wave's tiles
-    uint64_t mine = 0;
-    for (uint32_t b = tid; b < a.B; b += 256) { const Seq s = seq_of(a, b); mine += (uint64_t)s.nt * s.nqt * c.hkv; }
-    const uint64_t wsum = wave_sum64(mine);
-    if (lane == 0) s_sum[wave] = wsum;
-    if (tid < 8) s_seg[tid][0] = ~0u;
-    __syncthreads();
-    const uint64_t T = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-    const uint32_t N = (uint32_t)min((uint64_t)a.groups, max(T / 4, (uint64_t)1)), wg = blockIdx.x;
-    if (wg >= N || T == 0) {
-        if (tid == 0) a.meta[wg] = make_int4(-1, 0, 0, 0);
-        return;
-    }
-    const uint64_t g0 = wg * T / N, g1 = (wg + 1) * T / N;
-    uint64_t t = g0 + wave * (g1 - g0) / 4;
-    const uint64_t t1 = g0 + (wave + 1) * (g1 - g0) / 4;
-    {
+    Seq mine{};
+    uint64_t T, g0, g1, t, t1, base = 0;
+    uint32_t N, b = 0;
+    if (lane < 2) s_seg[2 * wave + lane][0] = ~0u;                  // (only this wave writes these two until the barrier)
+    if (a.fast) {
+        if (lane < a.B) mine = seq_of<QT>(a, lane);
+        const uint32_t w = mine.nt * mine.nqt * c.hkv, up = wave_scan32(w);
+        T = (uint32_t)__builtin_amdgcn_readlane((int)up, 63);
+        N = (uint32_t)min((uint64_t)a.groups, max(T / NW, (uint64_t)1));
+        if (wg >= N || T == 0) {
+            if (tid == 0 && !a.whole) a.meta[wg] = make_int4(-1, 0, 0, 0);
+            return;
+        }
+        g0 = wg * T / N;
+        g1 = (wg + 1) * T / N;
+        const auto owner = [&](uint64_t x) { return (uint32_t)__builtin_ctzll(__ballot(up > (uint32_t)x)); };    // x < T
+        const auto before = [&](uint32_t i) { return i ? (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)up, (int)i - 1) : 0ull; };
+        if (a.whole) {
+            const auto snap = [&](uint64_t x) {                     // the first item that begins at or behind x
+                if (x >= T) return T;
+                const uint32_t i = owner(x);
+                const uint64_t z = before(i);
+                const uint32_t nt = (uint32_t)__builtin_amdgcn_readlane((int)mine.nt, (int)i);
+                return z + ((uint32_t)(x - z) + nt - 1) / nt * nt;
+            };
+            g0 = snap(g0);
+            g1 = snap(g1);
+        }
+        t = g0 + wave * (g1 - g0) / NW;
+        t1 = g0 + (wave + 1) * (g1 - g0) / NW;
+        if (t < t1) { b = owner(t); base = before(b); }
+    } else {
+        uint64_t sum = 0;
+        for (uint32_t i = tid; i < a.B; i += 64 * NW) { const Seq s = seq_of<QT>(a, i); sum += (uint64_t)s.nt * s.nqt * c.hkv; }
+        sum = wave_sum64(sum);
+        if (lane == 0) s_sum[wave] = sum;
+        __syncthreads();
+        T = 0;
+        for (uint32_t i = 0; i < NW; ++i) T += s_sum[i];
+        N = (uint32_t)min((uint64_t)a.groups, max(T / NW, (uint64_t)1));
+        if (wg >= N || T == 0) {
+            if (tid == 0) a.meta[wg] = make_int4(-1, 0, 0, 0);
+            return;
+        }
+        g0 = wg * T / N;
+        g1 = (wg + 1) * T / N;
+        t = g0 + wave * (g1 - g0) / NW;
+        t1 = g0 + (wave + 1) * (g1 - g0) / NW;
         uint64_t carry = 0;
-        for (uint32_t b0 = 0; b0 < a.B; b0 += 256) {
-            const uint32_t b = b0 + tid;
+        for (uint32_t b0 = 0; b0 < a.B; b0 += 64 * NW) {
+            const uint32_t i = b0 + tid;
             uint64_t w = 0;
-            if (b < a.B) { const Seq s = seq_of(a, b); w = (uint64_t)s.nt * s.nqt * c.hkv; }
+            if (i < a.B) { const Seq s = seq_of<QT>(a, i); w = (uint64_t)s.nt * s.nqt * c.hkv; }
             uint64_t v = w;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
@@ -138,26 +194,30 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
             __syncthreads();
             if (lane == 63) s_sum[wave] = v;
             __syncthreads();
-            uint64_t base = carry;
-            for (uint32_t i = 0; i < 4; ++i) { if (i < wave) base += s_sum[i]; carry += s_sum[i]; }
-            v += base;
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint64_t x = g0 + i * (g1 - g0) / 4;
-                if (w && v - w <= x && x < v) { s_b[i] = b; s_base[i] = v - w; }
+            uint64_t z = carry;
+            for (uint32_t k = 0; k < NW; ++k) { if (k < wave) z += s_sum[k]; carry += s_sum[k]; }
+            v += z;
+            for (uint32_t k = 0; k < NW; ++k) {
+                const uint64_t x = g0 + k * (g1 - g0) / NW;
+                if (w && v - w <= x && x < v) { s_b[k] = i; s_base[k] = v - w; }
             }
         }
         __syncthreads();
+        if (t < t1) { b = __builtin_amdgcn_readfirstlane(s_b[wave]); base = s_base[wave]; }
     }
-    uint32_t b = 0, item = 0, j0 = 0;
+    const auto get = [&](uint32_t i) { return a.fast ? lane_seq(mine, i) : seq_of<QT>(a, i); };
     Seq s{};
+    uint32_t item = 0, j0 = 0;
     if (t < t1) {
-        b = __builtin_amdgcn_readfirstlane(s_b[wave]);
-        s = seq_of(a, b);
-        const uint64_t in = t - s_base[wave];
-        item = __builtin_amdgcn_readfirstlane((uint32_t)(in / s.nt));
+        s = get(b);
+        const uint64_t in = t - base;
+        item = __builtin_amdgcn_readfirstlane((uint32_t)div64(in, s.nt));
         j0 = __builtin_amdgcn_readfirstlane((uint32_t)(in - (uint64_t)item * s.nt));
     }
     const uint32_t kg = m >> 2, kr0 = m & 3;
+    uint32_t kcol[NP];                                              // columns past the head's width: read as its first ones, against zeros of Q
+#pragma unroll
+    for (int p = 0; p < NP; ++p) kcol[p] = FULL || 64 * p + 16 * g < dh ? 64 * p + 16 * g : 0;
     while (t < t1) {
         const uint32_t h = item / s.nqt, qt = item - h * s.nqt;
         const uint32_t j1 = (uint32_t)min((uint64_t)s.nt, j0 + (t1 - t));
@@ -168,13 +228,41 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
         const int32_t pos = r < nrow ? first + (int32_t)qi : -1;
         const int32_t pmin = first + (int32_t)(qt * QT / a.grp), pmax = first + (int32_t)((min(qt * QT + QT, nrow) - 1) / a.grp);
         const int32_t slo = a.window ? max(max(pmin, 0) - (int32_t)a.window + 1, 0) : 0;        // keys that any row sees: slo .. pmax
+        // ---- key tiles that any row sees
+        const uint32_t ja = max(j0, (uint32_t)slo / KT - s.ft), jb = pmax < 0 ? 0u : min(j1, (uint32_t)pmax / KT + 1 - s.ft);
+        const int32_t *tb = a.table + (uint64_t)b * a.ld;
+        const uint32_t npg = max((uint32_t)(s.L + c.bs - 1) >> c.lbs, 1u), hoff = h * c.bs * dh;
+        const auto page_at = [&](uint32_t j, uint32_t sub) { return (uint32_t)tb[min(((s.ft + j) * KT + sub) >> c.lbs, npg - 1)]; };
+        uint4 kr[4][NP], vr[MT];
+        float ksc = 0.f, vsc = 0.f;
+        uint32_t kp = 0, vp = 0;
+        bool bad = false;
+        const auto load_k = [&](uint32_t j) {
+            const uint32_t kt = (s.ft + j) * KT + 16 * kg, pk = kp < c.pages ? kp : 0, pv = vp < c.pages ? vp : 0;
+            const uint8_t *kb = c.k + pk * c.pgk + hoff + ((kt & (c.bs - 1)) + kr0) * dh;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int p = 0; p < NP; ++p) kr[q][p] = *(const uint4 *)(kb + 4 * q * dh + kcol[p]);
+            ksc = c.ks[(uint64_t)pv * c.pgs + h];
+            vsc = c.vs[(uint64_t)pv * c.pgs + h];
+        };
+        const auto load_v = [&](uint32_t j, uint32_t page) {
+            const uint32_t vt = (s.ft + j) * KT + 16 * g, pv = page < c.pages ? page : 0;
+            const uint8_t *vb = c.v + pv * c.pgv + hoff + m * c.bs + (vt & (c.bs - 1));
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                if (FULL || 16u * i < dh) vr[i] = *(const uint4 *)(vb + 16 * i * c.bs);
+        };
+        uint32_t vpc = 0;
+        if (ja < jb) { kp = page_at(ja, 16 * kg); vp = page_at(ja, 16 * g); }
         const uint16_t *qp = a.q + (uint64_t)(s.r0 + qi) * a.ldq + (uint64_t)qh * dh;
         uint16_t *op = a.o + (uint64_t)(s.r0 + qi) * a.ldo + (uint64_t)qh * dh;
         sh_h8 qf[2 * NP];
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             uint4 x = make_uint4(0, 0, 0, 0), y = x;
-            if (r < nrow && 64 * p + 16 * g < dh) { x = sh_ld16_any(qp + 64 * p + 16 * g); y = sh_ld16_any(qp + 64 * p + 16 * g + 8); }
+            if (r < nrow && (FULL || 64 * p + 16 * g < dh)) { x = sh_ld16_any(qp + 64 * p + 16 * g); y = sh_ld16_any(qp + 64 * p + 16 * g + 8); }
             qf[2 * p] = __builtin_bit_cast(sh_h8, x);
             qf[2 * p + 1] = __builtin_bit_cast(sh_h8, y);
         }
@@ -182,31 +270,17 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
 #pragma unroll
         for (int i = 0; i < MT; ++i) oa[i] = sh_f4v{0.f, 0.f, 0.f, 0.f};
         float mx = -1e30f, l = 0.f, cn = 0.f;
-
-        const int32_t *tb = a.table + (uint64_t)b * a.ld;
-        const uint32_t npg = max((uint32_t)(s.L + c.bs - 1) >> c.lbs, 1u), hoff = h * c.bs * dh;
-        auto page_at = [&](uint32_t tok) { return (uint32_t)tb[min(tok >> c.lbs, npg - 1)]; };
-        for (uint32_t j = j0; j < j1; ++j) {
-            const uint32_t k0 = (s.ft + j) * KT;
-            if ((int32_t)k0 > pmax || (int32_t)(k0 + KT) <= slo) continue;                  // no row of the item sees these keys
-            const uint32_t kt = k0 + 16 * kg, vt = k0 + 16 * g;
-            uint32_t kp = page_at(kt), vp = page_at(vt);
-            const bool bad = vp >= c.pages;
-            kp = kp < c.pages ? kp : 0;
-            vp = bad ? 0 : vp;
-            const uint8_t *kb = c.k + kp * c.pgk + hoff + ((kt & (c.bs - 1)) + kr0) * dh + 16 * g;
-            const uint8_t *vb = c.v + vp * c.pgv + hoff + m * c.bs + (vt & (c.bs - 1));
-            uint4 kr[4][NP], vr[MT];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    kr[q][p] = 64 * p + 16 * g < dh ? *(const uint4 *)(kb + (uint64_t)(4 * q) * dh + 64 * p) : make_uint4(0, 0, 0, 0);
-            const float ksc = c.ks[(uint64_t)vp * c.pgs + h] * a.sc;
-            float vsc = c.vs[(uint64_t)vp * c.pgs + h];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) vr[i] = 16u * i < dh ? *(const uint4 *)(vb + (uint64_t)(16 * i) * c.bs) : make_uint4(0, 0, 0, 0);
-
+        if (ja < jb) {
+            const uint32_t kn = page_at(ja + 1, 16 * kg), vn = page_at(ja + 1, 16 * g);
+            vpc = vp;
+            load_k(ja);
+            load_v(ja, vpc);
+            kp = kn;
+            vp = vn;
+        }
+        for (uint32_t j = ja; j < jb; ++j) {
+            const uint32_t k0 = (s.ft + j) * KT, vt = k0 + 16 * g;
+            bad = vpc >= c.pages;
             sh_f4v sa[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -217,9 +291,18 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
                     sa[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(kr[q][p].z, kr[q][p].w), qf[2 * p + 1], sa[q], 0, 0, 0);
                 }
             }
-            float x[16];
+            float x[16], vs = vsc;
+            const float ks = ksc * a.sc;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = sa[i >> 2][i & 3] * ksc;
+            for (int i = 0; i < 16; ++i) x[i] = sa[i >> 2][i & 3] * ks;
+            // the pages after the next tile's first (loads end in order), then its keys
+            const uint32_t vcur = vp;
+            if (j + 1 < jb) {
+                const uint32_t kn = page_at(j + 2, 16 * kg), vn = page_at(j + 2, 16 * g);
+                load_k(j + 1);
+                kp = kn;
+                vp = vn;
+            }
             const bool edge = (int32_t)(k0 + KT - 1) > pmin || (a.window && (int32_t)k0 < pmax - (int32_t)a.window + 1) || __any(bad);
             if (edge) {
                 const int32_t at = (int32_t)vt, from = a.window ? max(pos, 0) - (int32_t)a.window + 1 : 0;
@@ -227,7 +310,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
                 for (int i = 0; i < 16; ++i) x[i] = !bad && at + i <= pos && at + i >= from ? x[i] : -INFINITY;
                 // what no row sees may hold anything: its codes and scale must not meet a probability of 0
                 const int lo = bad ? 16 : max(slo - at, 0), hi = max(pmax + 1 - at, 0);
-                if (lo >= min(hi, 16)) vsc = 0.f;
+                if (lo >= min(hi, 16)) vs = 0.f;
 #pragma unroll
                 for (int i = 0; i < MT; ++i) vr[i] = keep_bytes(vr[i], lo, hi);
             }
@@ -235,7 +318,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
 #pragma unroll
             for (int i = 1; i < 16; ++i) tm = fmaxf(tm, x[i]);
             tm = max_xor16_32(tm);
-            const float mn = fmaxf(mx, tm), vm = max_xor16_32(vsc);
+            const float mn = fmaxf(mx, tm), vm = max_xor16_32(vs);
             float cs = cn;
             if (!(vm * cn <= 16384.f) || cn == 0.f) cs = __builtin_amdgcn_ldexpf(1.f, 14 - (vm > 1e-30f ? __builtin_amdgcn_frexp_expf(vm) : -99));
             if (__any(mn > mx) || cs != cn) {
@@ -246,7 +329,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
                 mx = mn;
                 cn = cs;
             }
-            const float w = vsc * cn;
+            const float w = vs * cn;
             sh_h8 pf[2];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -256,10 +339,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
-                if (16u * i < dh) {
+                if (FULL || 16u * i < dh) {
                     oa[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(vr[i].x, vr[i].y), pf[0], oa[i], 0, 0, 0);
                     oa[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(vr[i].z, vr[i].w), pf[1], oa[i], 0, 0, 0);
                 }
+            vpc = vcur;
+            if (j + 1 < jb) load_v(j + 1, vpc);
         }
         l = sum_xor16_32(l);
         const float ic = cn > 0.f ? 1.f / cn : 0.f;
@@ -268,13 +353,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
             if (r < nrow)
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    if (16u * i < dh) store4(op + 16 * i + 4 * g, oa[i][0] * f, oa[i][1] * f, oa[i][2] * f, oa[i][3] * f);
+                    if (FULL || 16u * i < dh) store4(op + 16 * i + 4 * g, oa[i][0] * f, oa[i][1] * f, oa[i][2] * f, oa[i][3] * f);
         } else {
             const uint32_t sg = 2 * wave + (j0 ? 0 : 1);
             if (m < a.prow) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    if (16u * i < dh) *(sh_f4v *)&s_o[(sg * a.prow + m) * DP + 16 * i + 4 * g] = oa[i] * ic;
+                    if (FULL || 16u * i < dh) *(sh_f4v *)&s_o[(sg * a.prow + m) * DP + 16 * i + 4 * g] = oa[i] * ic;
                 if (g == 0) { s_ml[sg][m][0] = mx; s_ml[sg][m][1] = l; }
             }
             if (lane == 0) { s_seg[sg][0] = b; s_seg[sg][1] = item; s_seg[sg][2] = j0; s_seg[sg][3] = j1; s_seg[sg][4] = s.nt; }
@@ -284,38 +369,49 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
         if (j1 == s.nt && t < t1) {
             if (++item == s.nqt * c.hkv) {
                 item = 0;
-                do { s = seq_of(a, ++b); } while (s.nt == 0 && b + 1 < a.B);
+                do { s = get(++b); } while (s.nt == 0 && b + 1 < a.B);
             }
         }
     }
     __syncthreads();
 
     // ---- parts that belong together: consecutive, the first and the last may reach beyond this workgroup
-    if (tid == 0) a.meta[wg] = make_int4(-1, 0, 0, 0);
-    uint32_t i0 = 0;
-    while (i0 < 8) {
-        if (s_seg[i0][0] == ~0u) { ++i0; continue; }
-        const uint32_t bb = s_seg[i0][0], it = s_seg[i0][1], ja = s_seg[i0][2], nt = s_seg[i0][4];
-        uint32_t i1 = i0, je = s_seg[i0][3];
-        for (uint32_t i = i0 + 1; i < 8; ++i)
-            if (s_seg[i][0] == bb && s_seg[i][1] == it) { i1 = i; je = s_seg[i][3]; }
-        const Seq q = seq_of(a, bb);
+    if (tid == 0 && !a.whole) a.meta[wg] = make_int4(-1, 0, 0, 0);
+    const uint32_t gs = min(lane, 2u * NW - 1);                     // lane i holds part i
+    const uint32_t gb = lane < 2 * NW ? s_seg[gs][0] : ~0u, gi = s_seg[gs][1], ga = s_seg[gs][2], ge = s_seg[gs][3], gn = s_seg[gs][4];
+    uint64_t left = __ballot(gb != ~0u);
+    while (left) {
+        const auto rl = [](uint32_t v, uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
+        const uint32_t i0 = __builtin_ctzll(left), bb = rl(gb, i0), it = rl(gi, i0);
+        const uint64_t in = __ballot(gb == bb && gi == it);
+        left &= ~in;
+        const uint32_t ja = rl(ga, i0), nt = rl(gn, i0), je = rl(ge, 63 - __builtin_clzll(in));
+        const Seq q = get(bb);
         const uint32_t h = it / q.nqt, qt = it - h * q.nqt, nrow = q.n * a.grp, qn = dh / 4;
-        const bool whole = ja == 0 && je == nt;
+        const bool all = ja == 0 && je == nt;
         const uint32_t slot = ja ? 0 : 1;
-        for (uint32_t e = tid; e < a.prow * qn; e += 256) {
+        for (uint32_t e = tid; e < a.prow * qn; e += 64 * NW) {
             const uint32_t row = e / qn, d = 4 * (e - row * qn), r = qt * QT + row;
             if (r >= nrow) continue;
-            float M = -1e30f, l = 0.f;
-            sh_f4v o = {0.f, 0.f, 0.f, 0.f};
-            for (uint32_t i = i0; i <= i1; ++i) if (s_seg[i][0] == bb && s_seg[i][1] == it) M = fmaxf(M, s_ml[i][row][0]);
-            for (uint32_t i = i0; i <= i1; ++i)
-                if (s_seg[i][0] == bb && s_seg[i][1] == it) {
-                    const float f = sh_fast_exp2(s_ml[i][row][0] - M);
-                    l += f * s_ml[i][row][1];
-                    o += f * *(const sh_f4v *)&s_o[(i * a.prow + row) * DP + d];
-                }
-            if (whole) {
+            // every read is made, a part of another item's from the first part's place and without weight: none waits for another
+            float pm[2 * NW], pl[2 * NW], M = -1e30f, l = 0.f;
+            sh_f4v o = {0.f, 0.f, 0.f, 0.f}, po[2 * NW];
+#pragma unroll
+            for (uint32_t i = 0; i < 2 * NW; ++i) {
+                const uint32_t at = in >> i & 1 ? i : i0;
+                pm[i] = s_ml[at][row][0];
+                pl[i] = s_ml[at][row][1];
+                po[i] = *(const sh_f4v *)&s_o[(at * a.prow + row) * DP + d];
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 2 * NW; ++i) M = fmaxf(M, pm[i]);
+#pragma unroll
+            for (uint32_t i = 0; i < 2 * NW; ++i) {
+                const float f = in >> i & 1 ? sh_fast_exp2(pm[i] - M) : 0.f;
+                l += f * pl[i];
+                o += f * po[i];
+            }
+            if (all) {
                 const float f = l > 0.f || l != l ? 1.f / l : 0.f;
                 const uint32_t qi = r / a.grp, qh = h * a.grp + (r - qi * a.grp);
                 store4(a.o + (uint64_t)(q.r0 + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
@@ -325,11 +421,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_attn(AttnArgs a) 
                 if (d == 0) { a.ml[at * 2] = M; a.ml[at * 2 + 1] = l; }
             }
         }
-        if (!whole && slot && tid == 0) {
+        if (!all && slot && tid == 0) {
             const uint64_t te = g1 + (nt - je);                                          // the item's end: it leaves here at je
             a.meta[wg] = make_int4((int)bb, (int)it, (int)((te * N - 1) / T), 0);
         }
-        i0 = i1 + 1;
     }
 }
 
@@ -342,7 +437,7 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
     const int4 me = a.meta[blockIdx.x];
     if (me.x < 0) return;
     const uint32_t wg = blockIdx.x, dh = a.c.dh, row = blockIdx.y, y = threadIdx.x / L, d = 4 * (threadIdx.x % L);
-    const Seq q = seq_of(a, (uint32_t)me.x);
+    const Seq q = seq_of<QT>(a, (uint32_t)me.x);
     const uint32_t h = (uint32_t)me.y / q.nqt, qt = (uint32_t)me.y - h * q.nqt, r = qt * QT + row;
     if (r >= q.n * a.grp) return;
     float M = -1e30f, l = 0.f;
@@ -374,21 +469,330 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
     store4(a.o + (uint64_t)(q.r0 + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
 }
 
+// ---- many rows: chunks of prompts ------------------------------------------------------------------------------------
+// A workgroup of four waves takes 128 rows of an item, 32 a wave, through the keys the rows see, 64 at a time: the codes are converted
+// once for all four waves into LDS (K rows and V^T rows of fp16, padded by 16 bytes: the operand reads then meet every bank once), two
+// buffers, the codes after the next in flight. S^T and O^T on v_mfma_f32_32x32x16_f16. As above no operand moves between
+// lanes: row m of a score tile's A operand is key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that the lane (n, hi) gets
+// the scores of keys 16 q + 8 hi + 0 .. 7 of row n, which is the second product's operand.
+// Bound by the vector pipe: for 64 keys by 32 rows a wave issues 32 matrix instructions (1024 cycles of their pipe) beside the
+// scores' multiply-add, maximum, exponential (four issues each), sum, weight and conversion (~1100 cycles) and 80 to convert codes.
+// The keys of an item are cut into parts of C tiles, C a 512th of all tiles (and at least 8): one long request among short ones, or a
+// few rows over a long context, then keep every CU busy. Units are dealt out by the hardware, the request's last row tiles first
+// (they see most). A request that is cut has more than C tiles, so cut units number at most 2 T / C <= 1024: their parts go to as many places
+// of `part`, which k_kv_chunk_join adds up.
+constexpr uint32_t CT = 128;               // rows of a unit
+constexpr uint32_t CUT = 512;              // units that share the whole evenly: two workgroups a CU
+constexpr uint32_t CUT_MIN = 8;            // tiles of a part at least
+template <int DP, bool FP8>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a) {
+    constexpr int KS = DP / 16, DT = DP / 32, NC = DP / 64;          // k-steps, column tiles, 16-byte chunks of K (of V) a thread stages
+    constexpr uint32_t KLD = DP + 8, VLD = KT + 8;
+    __shared__ __align__(16) uint16_t s_k[2][KT * KLD];
+    __shared__ __align__(16) uint16_t s_v[2][DP * VLD];
+    __shared__ float s_sc[2][4][2];
+    __shared__ uint32_t s_bad[2][4];
+    const KvCache &c = a.c;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hi = lane >> 5, dh = c.dh;
+
+    // ---- the unit: heads first, then parts, then row tiles from the last one on, then requests
+    uint64_t all = 0;
+    Seq q{};
+    for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+        q = Seq{};
+        if (b0 + lane < a.B) q = seq_of<CT>(a, b0 + lane);
+        all += (uint64_t)q.nt * q.nqt * c.hkv;
+    }
+    all = wave_sum64(all);
+    const uint32_t C = (uint32_t)max((all + CUT - 1) / CUT, (uint64_t)CUT_MIN);
+    uint32_t idx = blockIdx.x, b = 0, parts = 1, cut0 = 0;           // cut0: cut units before this request
+    Seq s{};
+    bool found = false;
+    for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
+        if (a.B > 64) {
+            q = Seq{};
+            if (b0 + lane < a.B) q = seq_of<CT>(a, b0 + lane);
+        }
+        const uint32_t p = (q.nt + C - 1) / C, w = q.nqt * c.hkv * p, up = wave_scan32(w), cu = wave_scan32(p > 1 ? w : 0u);
+        const auto last = [](uint32_t v, uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
+        const uint64_t hit = found ? 0 : __ballot(up > idx);
+        if (hit) {
+            const uint32_t i = __builtin_ctzll(hit);
+            b = b0 + i;
+            s = lane_seq(q, i);
+            parts = last(p, i);
+            idx -= i ? last(up, i - 1) : 0u;
+            cut0 += i ? last(cu, i - 1) : 0u;
+            found = true;
+            if (blockIdx.x) break;
+            if (tid == 0) a.meta[0].x = (int)(cut0 - (i ? last(cu, i - 1) : 0u) + last(cu, 63));        // (block 0 finds the first request with rows)
+        } else if (!found) {
+            idx -= last(up, 63);
+            cut0 += last(cu, 63);
+        } else if (tid == 0) {
+            a.meta[0].x += (int)last(cu, 63);
+        }
+    }
+    if (!found) {
+        if (blockIdx.x == 0 && tid == 0) a.meta[0].x = 0;
+        return;
+    }
+    const uint32_t h = idx % c.hkv, sp = idx / c.hkv % parts, qt = s.nqt - 1 - idx / c.hkv / parts, cut = cut0 + idx;
+    if (parts > 1 && cut >= 2 * CUT) return;                        // (row ranges that overlap beyond measure: nothing outside ws)
+
+    // ---- rows
+    const uint32_t nrow = s.n * a.grp, w0 = qt * CT + 32 * wave, r = w0 + n;
+    const uint32_t qi = r / a.grp, qh = h * a.grp + (r - qi * a.grp);
+    const int32_t first = s.L - (int32_t)s.nf;
+    const int32_t pos = r < nrow ? first + (int32_t)qi : -1;
+    const auto row_pos = [&](uint32_t x) { return first + (int32_t)(min(x, nrow - 1) / a.grp); };
+    const int32_t pmin = row_pos(qt * CT), pmax = row_pos(qt * CT + CT - 1);                // of the workgroup, and of this wave
+    const int32_t wmin = row_pos(w0), wmax = w0 < nrow ? row_pos(w0 + 31) : -1;
+    const int32_t win = (int32_t)a.window;
+    const int32_t slo = win ? max(max(pmin, 0) - win + 1, 0) : 0;
+    uint32_t ja = (uint32_t)slo / KT, jb = pmax < 0 ? ja : (uint32_t)pmax / KT + 1;
+    if (parts > 1) {
+        const uint32_t t = jb - ja, z = ja;
+        ja = z + (uint32_t)((uint64_t)sp * t / parts);
+        jb = z + (uint32_t)((uint64_t)(sp + 1) * t / parts);
+    }
+    const uint16_t *qp = a.q + (uint64_t)(s.r0 + qi) * a.ldq + (uint64_t)qh * dh;
+    sh_h8 qf[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < nrow && 16u * k < dh) x = sh_ld16_any(qp + 16 * k + 8 * hi);
+        qf[k] = __builtin_bit_cast(sh_h8, x);
+    }
+
+    // ---- staging: K chunk i is key (tid + 256 i) / (DP / 16), column 16 (tid % (DP / 16)); V chunk i is column d (tid + 256 i) / 4,
+    // keys 16 (tid % 4)
+    const int32_t *tb = a.table + (uint64_t)b * a.ld;
+    const uint32_t npg = max((uint32_t)(s.L + c.bs - 1) >> c.lbs, 1u), hoff = h * c.bs * dh;
+    const uint32_t kcol = 16 * (tid % (DP / 16)), vg = tid & 3;
+    uint32_t kpg[NC], vpg = 0, vpc = 0;
+    uint4 kr[NC], vr[NC];
+    float ksc = 0.f, vsc = 0.f;
+    const auto key_of = [&](int i) { return (tid + 256u * i) / (DP / 16); };
+    const auto pages = [&](uint32_t j) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) kpg[i] = (uint32_t)tb[min((j * KT + key_of(i)) >> c.lbs, npg - 1)];
+        vpg = (uint32_t)tb[min((j * KT + 16 * vg) >> c.lbs, npg - 1)];
+    };
+    const auto load = [&](uint32_t j) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const uint32_t p = kpg[i] < c.pages ? kpg[i] : 0, key = (j * KT + key_of(i)) & (c.bs - 1);
+            kr[i] = kcol < dh ? *(const uint4 *)(c.k + p * c.pgk + hoff + key * dh + kcol) : make_uint4(0, 0, 0, 0);
+        }
+        vpc = vpg;
+        const uint32_t p = vpg < c.pages ? vpg : 0, key = (j * KT + 16 * vg) & (c.bs - 1);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const uint32_t d = (tid + 256 * i) / 4;
+            vr[i] = d < dh ? *(const uint4 *)(c.v + p * c.pgv + hoff + d * c.bs + key) : make_uint4(0, 0, 0, 0);
+        }
+        if (tid < 4) {
+            ksc = c.ks[(uint64_t)p * c.pgs + h] * a.sc;
+            vsc = c.vs[(uint64_t)p * c.pgs + h];
+        }
+    };
+    const auto store16 = [](uint16_t *p, uint4 v) {
+        *(sh_h8 *)p = kv_half8<FP8>(v.x, v.y);
+        *(sh_h8 *)(p + 8) = kv_half8<FP8>(v.z, v.w);
+    };
+    const auto stage = [&](uint32_t j) {
+        const uint32_t u = j & 1;
+        const int32_t at = (int32_t)(j * KT + 16 * vg);
+        const bool bad = vpc >= c.pages;
+        const int lo = bad ? 16 : max(slo - at, 0), hic = max(pmax + 1 - at, 0);            // what no row sees may hold anything
+        if (lo > 0 || hic < 16)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) vr[i] = keep_bytes(vr[i], lo, hic);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            store16(&s_k[u][key_of(i) * KLD + kcol], kr[i]);
+            store16(&s_v[u][(tid + 256 * i) / 4 * VLD + 16 * vg], vr[i]);
+        }
+        if (tid < 4) {
+            s_sc[u][tid][0] = ksc;
+            s_sc[u][tid][1] = lo >= min(hic, 16) ? 0.f : vsc;
+            s_bad[u][tid] = bad;
+        }
+    };
+
+    sh_f16v oa[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) oa[i] = sh_f16v{};
+    float mx = -1e30f, l = 0.f, cn = 0.f;
+    if (ja < jb) {
+        pages(ja);
+        load(ja);
+        pages(ja + 1);
+        stage(ja);
+        if (ja + 1 < jb) { load(ja + 1); pages(ja + 2); }
+    }
+    const uint32_t krow = 16 * (n >> 4) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
+    for (uint32_t j = ja; j < jb; ++j) {
+        __syncthreads();                                            // tile j is staged, tile j - 1 is read
+        if (j + 1 < jb) {
+            stage(j + 1);
+            if (j + 2 < jb) { load(j + 2); pages(j + 3); }
+        }
+        const uint32_t u = j & 1;
+        const int32_t k0 = (int32_t)(j * KT);
+        if (k0 > wmax || (win && k0 + (int32_t)KT <= max(wmin, 0) - win + 1)) continue;     // this wave's rows see none of these keys
+        sh_f16v sa[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            sa[t] = sh_f16v{};
+            const uint16_t *kp = &s_k[u][(32 * t + krow) * KLD + 8 * hi];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) sa[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const sh_h8 *)(kp + 16 * k), qf[k], sa[t], 0, 0, 0);
+        }
+        float ks[4], vs[4];
+        uint32_t bad = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { ks[q] = s_sc[u][q][0]; vs[q] = s_sc[u][q][1]; bad |= s_bad[u][q] << q; }
+        bad = __builtin_amdgcn_readfirstlane(bad);
+        float x[4][8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[q][e] = sa[q >> 1][8 * (q & 1) + e] * ks[q];
+        if (k0 + (int32_t)KT - 1 > wmin || (win && k0 < wmax - win + 1) || bad) {
+            const int32_t at = k0 + 8 * (int32_t)hi, from = win ? max(pos, 0) - win + 1 : 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int32_t key = at + 16 * q + e;
+                    x[q][e] = key <= pos && key >= from && !(bad >> q & 1) ? x[q][e] : -INFINITY;
+                }
+        }
+        float tm = x[0][0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) tm = fmaxf(tm, x[i >> 3][i & 7]);
+        const float mn = fmaxf(mx, sh_max_xor32(tm)), vm = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+        float cs = cn;
+        if (!(vm * cn <= 16384.f) || cn == 0.f) cs = __builtin_amdgcn_ldexpf(1.f, 14 - (vm > 1e-30f ? __builtin_amdgcn_frexp_expf(vm) : -99));
+        if (__any(mn > mx) || cs != cn) {
+            const float al = sh_fast_exp2(mx - mn), be = al * (cn == 0.f ? 0.f : cs / cn);
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) oa[i] *= be;
+            mx = mn;
+            cn = cs;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float w = vs[q] * cn;
+            sh_h8 pf;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = sh_fast_exp2(x[q][e] - mx);
+                l += p;
+                pf[e] = (_Float16)(p * w);
+            }
+            const uint16_t *vp = &s_v[u][n * VLD + 16 * q + 8 * hi];
+#pragma unroll
+            for (int i = 0; i < DT; ++i) oa[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const sh_h8 *)(vp + 32 * i * VLD), pf, oa[i], 0, 0, 0);
+        }
+    }
+    const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
+    const float ic = cn > 0.f ? 1.f / cn : 0.f;
+    if (parts == 1) {
+        if (r >= nrow) return;
+        uint16_t *op = a.o + (uint64_t)(s.r0 + qi) * a.ldo + (uint64_t)qh * dh;
+        const float f = l > 0.f || l != l ? ic / l : 0.f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t d = 32 * i + 8 * k + 4 * hi;
+                if (d < dh) store4(op + d, oa[i][4 * k] * f, oa[i][4 * k + 1] * f, oa[i][4 * k + 2] * f, oa[i][4 * k + 3] * f);
+            }
+    } else {
+        if (tid == 0) a.unit[cut] = ChunkUnit{sp ? 0u : parts, s.r0, nrow, qt, h, c.hkv, {0, 0}};
+        if (r >= nrow) return;
+        const uint64_t at = (uint64_t)cut * CT + 32 * wave + n;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t d = 32 * i + 8 * k + 4 * hi;
+                if (d < dh) *(sh_f4v *)&a.part[at * dh + d] = sh_f4v{oa[i][4 * k], oa[i][4 * k + 1], oa[i][4 * k + 2], oa[i][4 * k + 3]} * ic;
+            }
+        if (hi == 0) { a.ml[at * 2] = mx; a.ml[at * 2 + 1] = l; }
+    }
+}
+
+// The parts of a cut item, in order: this block's unit is its first, the others follow `step` places apart.
+__global__ __launch_bounds__(256) void k_kv_chunk_join(AttnArgs a) {
+    const uint32_t cut = blockIdx.x;
+    if (cut >= (uint32_t)a.meta[0].x) return;
+    const ChunkUnit u = a.unit[cut];
+    const uint32_t dh = a.c.dh, qn = dh / 4, half = CT / gridDim.y;
+    if (!u.parts) return;
+    for (uint32_t e = threadIdx.x; e < half * qn; e += 256) {
+        const uint32_t row = blockIdx.y * half + e / qn, d = 4 * (e % qn), r = u.qt * CT + row;
+        if (r >= u.nrow) break;
+        float M = -1e30f, l = 0.f;
+        sh_f4v o = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t i = 0; i < u.parts; ++i) {
+            const uint64_t at = (uint64_t)(cut + i * u.step) * CT + row;
+            const float m = a.ml[at * 2], s = a.ml[at * 2 + 1];
+            const sh_f4v v = *(const sh_f4v *)&a.part[at * dh + d];
+            const float mn = fmaxf(M, m), f = sh_fast_exp2(M - mn), g = sh_fast_exp2(m - mn);
+            o = o * f + v * g;
+            l = l * f + s * g;
+            M = mn;
+        }
+        const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+        const uint32_t qi = r / a.grp, qh = u.h * a.grp + (r - qi * a.grp);
+        store4(a.o + (uint64_t)(u.r0 + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+    }
+}
+
 uint32_t part_rows(uint32_t max_q, uint32_t grp) { return (uint32_t)min((uint64_t)QT, (uint64_t)max_q * grp); }
 
-template <int DP, bool FP8>
-bool launch_attn(const AttnArgs &a, hipStream_t st) {
+template <int DP, bool FP8, bool FULL, int NW>
+bool launch_attn(AttnArgs a, uint32_t tiles, hipStream_t st) {
     static bool set = false;
-    const uint32_t lds = 8 * a.prow * DP * 4;
+    const uint32_t lds = 2 * NW * a.prow * DP * 4;
     if (!set) {
-        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_kv_attn<DP, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * QT * DP * 4),
+        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_kv_attn<DP, FP8, FULL, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * NW * QT * DP * 4),
                        "sh_attention_kv hipFuncSetAttribute")) return false;
         set = true;
     }
-    hipLaunchKernelGGL((k_kv_attn<DP, FP8>), dim3(a.groups), dim3(256), lds, st, a);
-    hipLaunchKernelGGL(k_kv_join<DP>, dim3(a.groups, a.prow), dim3(256), 0, st, a);
+    a.groups = DP == 128 ? GROUPS / 2 : GROUPS;
+    a.whole = a.fast && tiles <= WHOLE_TILES * NW;
+    hipLaunchKernelGGL((k_kv_attn<DP, FP8, FULL, NW>), dim3(a.groups), dim3(64 * NW), lds, st, a);
+    if (!a.whole) hipLaunchKernelGGL(k_kv_join<DP>, dim3(a.groups, a.prow), dim3(256), 0, st, a);
     return sh_launch_ok("sh_attention_kv");
 }
+template <bool FP8>
+bool launch_attn_width(const AttnArgs &a, uint32_t tiles, hipStream_t st) {
+    if (a.c.dh == 64) return launch_attn<64, FP8, true, 8>(a, tiles, st);
+    if (a.c.dh == 128) return launch_attn<128, FP8, true, 8>(a, tiles, st);
+    if (a.c.dh < 64) return launch_attn<64, FP8, false, 8>(a, tiles, st);
+    if (a.c.dh < 128) return launch_attn<128, FP8, false, 8>(a, tiles, st);
+    return launch_attn<256, FP8, false, 4>(a, tiles, st);
+}
+
+template <bool FP8>
+bool launch_chunk(const AttnArgs &a, uint32_t units, hipStream_t st) {
+    if (a.c.dh <= 64) hipLaunchKernelGGL((k_kv_chunk<64, FP8>), dim3(units), dim3(256), 0, st, a);
+    else if (a.c.dh <= 128) hipLaunchKernelGGL((k_kv_chunk<128, FP8>), dim3(units), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_kv_chunk<256, FP8>), dim3(units), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_kv_chunk_join, dim3(2 * CUT, 4), dim3(256), 0, st, a);
+    return sh_launch_ok("sh_attention_kv");
+}
+
+// More rows a request than CHUNK_ROWS: the kernel that shares converted keys between the rows of a workgroup.
+constexpr uint32_t CHUNK_ROWS = 32;
+bool chunked(uint32_t max_q, uint32_t grp) { return (uint64_t)max_q * grp > CHUNK_ROWS; }
 
 }  // namespace
 
@@ -396,6 +800,8 @@ extern "C" {
 
 uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t rows, uint32_t max_q, uint32_t H, uint32_t ld_table) {
     if (!c || !B || !rows || !max_q || !c->hkv || !H || !ld_table || !c->dh) return 0;
+    max_q = min(max_q, rows);
+    if (chunked(max_q, H / c->hkv)) return 2 * CUT * ((uint64_t)CT * (c->dh + 2) * 4 + sizeof(ChunkUnit)) + 16;
     const uint64_t prow = part_rows(max_q, H / c->hkv);
     return (uint64_t)GROUPS * (2 * prow * (c->dh + 2) * 4 + 16);
 }
@@ -432,19 +838,29 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     a.q = (const uint16_t *)q; a.o = (uint16_t *)o;
     a.table = (const int32_t *)table; a.kv_len = (const int32_t *)kv_len; a.row_start = (const int32_t *)row_start;
     a.ldq = ldq; a.ldo = ldo; a.ld = ld_table;
-    a.B = B; a.rows = rows; a.max_q = min(max_q, rows); a.grp = grp; a.prow = part_rows(max_q, grp);
+    a.B = B; a.rows = rows; a.max_q = min(max_q, rows); a.grp = grp; a.prow = part_rows(a.max_q, grp);
     a.window = window < ld_table * c->bs ? window : 0;               // (one that no key falls out of is none)
     a.groups = GROUPS;
     a.sc = scale * 1.4426950408889634f;
     a.meta = (int4 *)ws;
+    const hipStream_t st = sh_stream();
+    if (chunked(a.max_q, grp)) {
+        // units: the row tiles, each request's last one short, and at most CUT parts more
+        const uint64_t tiles = min((uint64_t)B * (((uint64_t)a.max_q * grp + CT - 1) / CT), ((uint64_t)rows * grp + CT - 1) / CT + B);
+        if (tiles * c->hkv + CUT >= (1ull << 31)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", rows, H); return -1; }
+        const uint32_t units = (uint32_t)(tiles * c->hkv) + CUT;
+        a.unit = (ChunkUnit *)(ws + 16);
+        a.part = (float *)(ws + 16 + 2 * CUT * sizeof(ChunkUnit));
+        a.ml = a.part + (uint64_t)2 * CUT * CT * c->dh;
+        return (c->fmt == SH_FP8 ? launch_chunk<true>(a, units, st) : launch_chunk<false>(a, units, st)) ? 0 : SH_EHIP;
+    }
     a.part = (float *)(ws + GROUPS * 16);
     a.ml = a.part + (uint64_t)GROUPS * 2 * a.prow * c->dh;
-    const hipStream_t st = sh_stream();
-    const bool f8 = c->fmt == SH_FP8;
-    bool ok;
-    if (c->dh <= 64) ok = f8 ? launch_attn<64, true>(a, st) : launch_attn<64, false>(a, st);
-    else if (c->dh <= 128) ok = f8 ? launch_attn<128, true>(a, st) : launch_attn<128, false>(a, st);
-    else ok = f8 ? launch_attn<256, true>(a, st) : launch_attn<256, false>(a, st);
+    uint64_t tiles = ((uint64_t)ld_table * c->bs + KT - 1) / KT + 1;                     // an item's, at most
+    if (a.window) tiles = min(tiles, ((uint64_t)a.window + a.max_q) / KT + 2);
+    const uint64_t items = (uint64_t)c->hkv * (((uint64_t)a.max_q * grp + QT - 1) / QT);
+    a.fast = B <= 64 && tiles * items < (1ull << 31) / B;
+    const bool ok = c->fmt == SH_FP8 ? launch_attn_width<true>(a, (uint32_t)tiles, st) : launch_attn_width<false>(a, (uint32_t)tiles, st);
     return ok ? 0 : SH_EHIP;
 }
 

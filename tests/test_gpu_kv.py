@@ -288,6 +288,11 @@ ATTNS = [   # H, hkv, dh, bs, lengths, new rows
     (2, 1, 256, 32, [150], [33]),
     (3, 3, 48, 16, [40, 10], [3, 12]),                        # more rows than keys: the first two see none
     (16, 2, 128, 16, [150, 600, 20], [150, 1, 3]),
+    (4, 1, 64, 16, [6000, 3], [20, 1]),                       # few rows over a long context: its keys in parts
+    (8, 1, 128, 64, [2600, 900], [9, 17]),
+    (4, 2, 112, 32, [1500], [40]),
+    (12, 1, 256, 16, [900, 1], [30, 1]),
+    (1, 1, 16, 16, [700], [700]),
 ]
 
 
@@ -305,7 +310,7 @@ def test_attention(lib, gpu, case, fmt):
 
 
 @pytest.mark.parametrize("window", [1, 15, 64, 100, 5000])
-@pytest.mark.parametrize("new", [None, [1, 40, 3]])
+@pytest.mark.parametrize("new", [None, [1, 4, 3], [1, 40, 3]])
 def test_attention_window(lib, gpu, window, new):
     """Pages before every window hold NaN codes and scales and have table entries outside the cache: nothing of them is seen."""
     rng = np.random.default_rng(window)
@@ -325,7 +330,7 @@ def test_attention_window(lib, gpu, window, new):
     c.dks.copy_(dev(host[2])); c.dvs.copy_(dev(host[3]))                                       # noqa: E702
     clean = [np.where((h & 127) == 127, 0, h).astype(np.uint8) if h.dtype == np.uint8 else np.nan_to_num(h) for h in host]
     start = None if new is None else np.concatenate([[0], np.cumsum(new)])
-    q = rng.standard_normal((3 if new is None else 44, H * dh)).astype(np.float16)
+    q = rng.standard_normal((3 if new is None else sum(new), H * dh)).astype(np.float16)
     _attend(lib, c, q, table, L, start, H, 0.125, window=window, host=clean)
 
 
@@ -407,6 +412,22 @@ def test_attention_many_requests(lib, gpu):
     start = np.concatenate([[0], np.cumsum(new)])
     pages = int(sum(-(-n // bs) for n in L)) + 1
     c = Cache(rng, pages, 1, dh, bs, INT8)
+    q = rng.standard_normal((int(start[-1]), 2 * dh)).astype(np.float16)
+    _attend(lib, c, q, _table(rng, L.tolist(), bs, pages), L.tolist(), start, 2, 0.2)
+
+
+@pytest.mark.parametrize("B", [65, 200])
+def test_attention_many_chunks(lib, gpu, B):
+    """Chunks of more requests than a wave has lanes, one of them long enough to be cut."""
+    rng = np.random.default_rng(B)
+    bs, dh = 16, 32
+    new = np.where(rng.random(B) < 0.3, 0, rng.integers(1, 12, B))
+    new[3], new[B - 1] = 40, 50
+    L = new + np.where(rng.random(B) < 0.5, 0, rng.integers(0, 200, B))
+    L[B - 1] = 4000
+    start = np.concatenate([[0], np.cumsum(new)])
+    pages = int(sum(-(-n // bs) for n in L)) + 1
+    c = Cache(rng, pages, 1, dh, bs, FP8, values=True)
     q = rng.standard_normal((int(start[-1]), 2 * dh)).astype(np.float16)
     _attend(lib, c, q, _table(rng, L.tolist(), bs, pages), L.tolist(), start, 2, 0.2)
 
