@@ -1,10 +1,13 @@
 // Few rows times a weight of 4-bit codes (sh_gemm_w4).
 //
-// z[m][n] = sum_g s[g][n] sum_{k in g} x[m][k] (c[k][n] - z[g][n]): the inner sum on MFMA (v_mfma_f32_16x16x32_f16, 16 rows
-// by 16 columns) with the integer c - z, which fp16 holds exactly; the scale multiplies the fp32 sum of its group. A word holds
-// eight k of one column, which is one lane's operand of a step: lane (n, g) reads the word of column n and octet 4 step + g, so
-// no operand is moved. In fp16 the number 1024 + c is 0x6400 | c: two codes of a word four apart are masked into a pair of
-// halves at once, so the lane's k order is 0 4 1 5 2 6 3 7, and X's operand is put into the same order.
+// z[m][n] = sum_g s[g][n] (sum_{k in g} x[m][k] c[k][n] - z[g][n] sum_{k in g} x[m][k]): both inner sums on MFMA
+// (v_mfma_f32_16x16x32_f16, 16 rows by 16 columns, the second against ones), the scale and the zero applied to the fp32 sums.
+// A word holds eight k of one column, which is one lane's operand of a step: lane (n, g) reads the word of column n and octet
+// 4 step + g, so no operand is moved. A code in the low four bits of a half is the subnormal c 2^-24, which the matrix pipe multiplies
+// exactly, and 16 times that four bits higher: two codes, eight k apart in the word's halves, are masked out at once, and
+// only every second pair needs a shift: 5 vector instructions for 8 codes, 11 where they are made numbers 1024 + c and the zero is taken off
+// each (one row of 4096 x 14336: 10.7 us). The pairs are the k (0, 4) and (2, 6), and (1, 5) and (3, 7) 16 times as large: of
+// two steps' words the former make one operand, the latter another with a sum of its own, and x's are put into the same order.
 #include "sh_common.h"
 
 namespace {
@@ -14,7 +17,7 @@ struct W4Args {
     const uint32_t *w;
     const uint8_t *zero;
     uint16_t *z;
-    uint32_t M, N, K, ugroup;          // ugroup: units of a group
+    uint32_t M, N, K, groups, per;     // per: (GS steps) of a group
     uint64_t ldx, ldw, lds, ldz, ldr;
     const void *bias;
     const uint16_t *res;
@@ -55,32 +58,39 @@ __device__ __forceinline__ uint32_t ld_zeros(const uint8_t *p) {
     else return *p;
 }
 
-// The eight codes of a word minus the zero: pairs (0, 4), (1, 5), (2, 6), (3, 7).
-__device__ __forceinline__ sh_h8 w4_half8(uint32_t w, sh_h2 z1024) {
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const sh_h2 v = __builtin_bit_cast(sh_h2, ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u) - z1024;
-        r[i] = __builtin_bit_cast(uint32_t, v);
-    }
-    return __builtin_bit_cast(sh_h8, make_uint4(r[0], r[1], r[2], r[3]));
+// Two words' codes of k 0, 4, 2, 6 as c 2^-24, and of k 1, 5, 3, 7 as c 2^-20.
+__device__ __forceinline__ sh_h8 codes_lo(uint32_t a, uint32_t b) {
+    constexpr uint32_t m = 0x000F000Fu;
+    return __builtin_bit_cast(sh_h8, make_uint4(a & m, (a >> 8) & m, b & m, (b >> 8) & m));
 }
-// Eight consecutive halves in that order.
-__device__ __forceinline__ sh_h8 x_order(uint4 v) {
-    return __builtin_bit_cast(sh_h8, make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                                                __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)));
+__device__ __forceinline__ sh_h8 codes_hi(uint32_t a, uint32_t b) {
+    constexpr uint32_t m = 0x00F000F0u;
+    return __builtin_bit_cast(sh_h8, make_uint4(a & m, (a >> 8) & m, b & m, (b >> 8) & m));
+}
+// One word's codes of k 0, 4, 1, 5, 2, 6, 3, 7 as c 2^-20.
+__device__ __forceinline__ sh_h8 codes_one(uint32_t a) {
+    constexpr uint32_t m = 0x00F000F0u;
+    return __builtin_bit_cast(sh_h8, make_uint4((a << 4) & m, a & m, (a >> 4) & m, (a >> 8) & m));
+}
+// Eight consecutive halves: k 0, 4 / 1, 5 / 2, 6 / 3, 7.
+struct XPairs { uint32_t p04, p15, p26, p37; };
+__device__ __forceinline__ XPairs x_pairs(uint4 v) {
+    return XPairs{__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
+                  __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
 }
 
 __device__ __forceinline__ float gelu(float x) {          // x / (1 + 2^{x (k0 + k1 x^2)}), fp32
     return x * sh_fast_rcp(1.f + sh_fast_exp2(x * fmaf(SH_GELU_K1 * x, x, SH_GELU_K0)));
 }
 
-// A workgroup of NW waves: 16 CW columns (lane n has CW consecutive ones), 16 MT rows; wave i takes the units (32 SU values
-// of k, all of one group) i, i + NW, ..., the next one's words in flight while it multiplies; the waves' sums are added in LDS in wave
-// order. Columns and octets past the end are read from the last ones: their products are dropped or meet zeros of x.
-template <int MT, int CW, int NW, int SU>
+// A workgroup of NW waves: 16 CW columns (lane n has CW consecutive ones), 16 MT rows; wave i takes the units (SU
+// steps of 32 k) i, i + NW, ..., the next one's words in flight while it multiplies; the waves' sums are added in LDS in wave order. Every
+// GS steps of a unit the sums are scaled: GS = 4, 2, 1 for groups that are multiples of 128, 64, 32. Columns and octets past the end
+// are read from the last ones: their products are dropped or meet zeros of x.
+template <int MT, int CW, int NW, int GS, int SU>
 __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
     constexpr uint32_t LC = 16 * CW + 1;
+    constexpr int NG = SU / GS;
     constexpr bool PX = MT == 1;                                    // x's next operands too
     extern __shared__ float s_z[];                                  // [NW][rows][LC]
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -97,7 +107,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < CW; ++j) acc[i][j] = sh_f4v{0.f, 0.f, 0.f, 0.f};
-    struct Ops { Run<CW> w[SU]; uint4 x[PX ? SU : 1][MT]; float sc[CW]; uint32_t zr; };
+    struct Ops { Run<CW> w[SU]; uint4 x[PX ? SU : 1][MT]; float sc[NG][CW]; uint32_t zr[NG]; };
     // octets past K: the last one again
     const auto back = [&](uint32_t u, int s) { const uint32_t o = (u * SU + s) * 4 + g; return o < oct ? 0u : o - (oct - 1); };
     const auto load_x = [&](uint32_t u, int s, uint4 (&x)[MT]) {
@@ -116,43 +126,76 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
         if constexpr (PX)
 #pragma unroll
             for (int s = 0; s < SU; ++s) load_x(u, s, o.x[s]);
-        const uint64_t gi = (uint64_t)(u / a.ugroup) * a.lds + col;
-        ld_scales<CW>(a.scale + gi, o.sc);
-        o.zr = a.zero ? ld_zeros<CW>(a.zero + gi) : 0x08080808u;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            const uint64_t gi = (uint64_t)min((u * NG + k) / a.per, a.groups - 1) * a.lds + col;
+            ld_scales<CW>(a.scale + gi, o.sc[k]);
+            o.zr[k] = a.zero ? ld_zeros<CW>(a.zero + gi) : 0x08080808u;
+        }
     };
     const auto multiply = [&](uint32_t u, Ops &o) {
         uint4 x[SU][MT];
 #pragma unroll
         for (int s = 0; s < SU; ++s)
             if constexpr (PX) x[s][0] = o.x[s][0]; else load_x(u, s, x[s]);
-        sh_h2 z[CW];
-#pragma unroll
-        for (int j = 0; j < CW; ++j) {
-            const uint32_t zz = 0x6400u | ((o.zr >> (8 * j)) & 15u);                     // the half 1024 + zero
-            z[j] = __builtin_bit_cast(sh_h2, zz | zz << 16);
-        }
-        sh_f4v p[MT][CW];
         const bool tail = (u + 1) * 4 * SU > oct;
+        if (tail)
 #pragma unroll
-        for (int s = 0; s < SU; ++s) {
-            sh_h8 wf[CW];
+            for (int s = 0; s < SU; ++s)
+                if (back(u, s))
 #pragma unroll
-            for (int j = 0; j < CW; ++j) wf[j] = w4_half8(o.w[s].w[j], z[j]);
+                    for (int i = 0; i < MT; ++i) x[s][i] = make_uint4(0, 0, 0, 0);
+        const sh_f4v zero = {0.f, 0.f, 0.f, 0.f};
+        const sh_h8 ones = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if (tail && back(u, s)) x[s][i] = make_uint4(0, 0, 0, 0);
-                const sh_h8 xf = x_order(x[s][i]);
+        for (int k = 0; k < NG; ++k) {
+            sh_f4v lo[MT][CW], hi[MT][CW], xs[MT];                  // sums of x c 2^-24, of x c 2^-20, of x
 #pragma unroll
-                for (int j = 0; j < CW; ++j)
-                    p[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf, wf[j], s ? p[i][j] : sh_f4v{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            for (int i = 0; i < MT; ++i) xs[i] = zero;
+            if constexpr (GS == 1) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const XPairs q = x_pairs(x[k][i]);
+                    const sh_h8 xf = __builtin_bit_cast(sh_h8, make_uint4(q.p04, q.p15, q.p26, q.p37));
+                    xs[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf, ones, zero, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < CW; ++j) hi[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf, codes_one(o.w[k].w[j]), zero, 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int s = k * GS; s < (k + 1) * GS; s += 2) {
+                    sh_h8 cl[CW], ch[CW];
+#pragma unroll
+                    for (int j = 0; j < CW; ++j) { cl[j] = codes_lo(o.w[s].w[j], o.w[s + 1].w[j]); ch[j] = codes_hi(o.w[s].w[j], o.w[s + 1].w[j]); }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const XPairs p = x_pairs(x[s][i]), q = x_pairs(x[s + 1][i]);
+                        const sh_h8 xl = __builtin_bit_cast(sh_h8, make_uint4(p.p04, p.p26, q.p04, q.p26)),
+                                    xh = __builtin_bit_cast(sh_h8, make_uint4(p.p15, p.p37, q.p15, q.p37));
+                        xs[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, ones, xs[i], 0, 0, 0);
+                        xs[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, ones, xs[i], 0, 0, 0);
+#pragma unroll
+                        for (int j = 0; j < CW; ++j) {
+                            lo[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, cl[j], s > k * GS ? lo[i][j] : zero, 0, 0, 0);
+                            hi[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, ch[j], s > k * GS ? hi[i][j] : zero, 0, 0, 0);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < CW; ++j) {
+                const float sc = o.sc[k][j], sz = -sc * (float)((o.zr[k] >> (8 * j)) & 15u), s24 = sc * 0x1p24f, s20 = sc * 0x1p20f;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // (the products are of like size and may cancel: first against each other, then into the sum)
+                        float t = hi[i][j][e] * s20;
+                        if constexpr (GS > 1) t = fmaf(lo[i][j][e], s24, t);
+                        acc[i][j][e] += fmaf(xs[i][e], sz, t);
+                    }
             }
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < CW; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(o.sc[j], p[i][j][e], acc[i][j][e]);
     };
     Ops o0, o1;
     uint32_t u = wave;
@@ -192,27 +235,37 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
     }
 }
 
-template <int MT, int CW, int SU>
+template <int MT, int CW, int GS, int SU>
 bool launch_w4(const W4Args &a, hipStream_t st) {
     constexpr uint32_t NW = 8, most = NW * 16 * MT * (16 * CW + 1) * 4;
     static bool set = false;
     if (!set && most > 65536) {
-        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_w4<MT, CW, NW, SU>, hipFuncAttributeMaxDynamicSharedMemorySize, most),
+        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_w4<MT, CW, NW, GS, SU>, hipFuncAttributeMaxDynamicSharedMemorySize, most),
                        "sh_gemm_w4 hipFuncSetAttribute")) return false;
         set = true;
     }
     const uint32_t lds = NW * (a.M < 16 * MT ? a.M : 16 * MT) * (16 * CW + 1) * 4;
-    hipLaunchKernelGGL((k_w4<MT, CW, NW, SU>), dim3(sh_cdiv(a.N, 16 * CW), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL((k_w4<MT, CW, NW, GS, SU>), dim3(sh_cdiv(a.N, 16 * CW), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), lds, st, a);
     return sh_launch_ok("sh_gemm_w4");
 }
-template <int SU>
+// The widest tile that still makes 192 workgroups of the 256 CUs: columns first (a word is converted once for every 16 rows of a
+// workgroup, x is read once for every 16 CW columns), then 32 rows.
+template <int GS, int SU>
 bool launch_w4_tile(const W4Args &a, hipStream_t st) {
     const uint32_t mt = sh_cdiv(a.M, 16);
-    const auto fills = [&](uint32_t m, uint32_t c) { return sh_cdiv(a.N, 16 * c) * sh_cdiv(mt, m) >= 192; };
-    if (a.N < 4) return launch_w4<1, 1, SU>(a, st);
-    if (fills(1, 4)) return launch_w4<1, 4, SU>(a, st);
-    if (fills(1, 2)) return launch_w4<1, 2, SU>(a, st);
-    return launch_w4<1, 1, SU>(a, st);
+    const auto fills = [&](uint32_t m, uint32_t c) { return (uint64_t)sh_cdiv(a.N, 16 * c) * sh_cdiv(mt, m) >= 192; };
+    if (a.N >= 4 && mt > 1 && fills(2, 4)) return launch_w4<2, 4, GS, SU>(a, st);
+    if (a.N >= 4 && fills(1, 4)) return launch_w4<1, 4, GS, SU>(a, st);
+    if (a.N >= 2 && fills(1, 2)) return launch_w4<1, 2, GS, SU>(a, st);
+    return launch_w4<1, 1, GS, SU>(a, st);
+}
+
+// Units of 128 k keep the most words in flight (one row of 4096 x 14336, groups of 64: 10.9 us against 12.1 in units of 64); with
+// fewer than eight of them (K < 1024) units of a group's own steps use every wave (one row of 720 x 2048, groups of 32: 3.6 against 4.1).
+template <int GS>
+bool launch_w4_unit(W4Args a, uint32_t group, hipStream_t st) {
+    a.per = group / (32 * GS);
+    return a.K < 1024 ? launch_w4_tile<GS, GS>(a, st) : launch_w4_tile<GS, 4>(a, st);
 }
 
 }  // namespace
@@ -240,7 +293,7 @@ extern "C" int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero,
             return -1;
         }
     }
-    W4Args a{(const uint16_t *)x, (const uint16_t *)scale, (const uint32_t *)w, (const uint8_t *)zero, (uint16_t *)z, M, N, K, 0,
+    W4Args a{(const uint16_t *)x, (const uint16_t *)scale, (const uint32_t *)w, (const uint8_t *)zero, (uint16_t *)z, M, N, K, (K + group - 1) / group, 0,
              ldx, ldw, lds, ldz, 0, nullptr, nullptr, 0, 0};
     if (epi) {
         a.bias = (const void *)epi->bias; a.bias_fp32 = epi->bias_fmt == SH_BIAS_FP32;
@@ -249,8 +302,8 @@ extern "C" int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero,
     }
     const hipStream_t st = sh_stream();
     bool ok;
-    if (group % 128 == 0) { a.ugroup = group / 128; ok = launch_w4_tile<4>(a, st); }
-    else if (group % 64 == 0) { a.ugroup = group / 64; ok = launch_w4_tile<2>(a, st); }
-    else { a.ugroup = group / 32; ok = launch_w4_tile<1>(a, st); }
+    if (group % 128 == 0) ok = launch_w4_unit<4>(a, group, st);
+    else if (group % 64 == 0) ok = launch_w4_unit<2>(a, group, st);
+    else ok = launch_w4_unit<1>(a, group, st);
     return ok ? 0 : SH_EHIP;
 }

@@ -53,10 +53,13 @@ def _run(lib, x, codes, scale, zero, group, bias=None, bias32=False, act=0, resi
 
 
 def _check(got, x, codes, scale, zero, group, bias=None, gelu=False, residual=None):
-    """Rounding to fp16 (half a step, 2^-11, twice with a residual); exact products summed in fp32: a chain of at most 128
-    within a group, one term for each group of the chain's wave, then the waves, and up to eight more operations, each 2^-23 of
-    sum |x||w| at most; GELU's slope is below 1.13, and its hardware exp2 and reciprocal add 2^-20 of the result."""
-    z, s = R.gemm_w4(x, codes, scale, zero, group, bias, gelu)
+    """Rounding to fp16 (half a step, 2^-11, twice with a residual); sums of x code and of x zero, exact products in fp32: a chain
+    of at most 128 within a group, one term for each group of the chain's wave, then the waves, and up to eight more operations,
+    each 2^-23 of sum |x| (code + zero) scale at most; GELU's slope is below 1.13, and its hardware exp2 and reciprocal add
+    2^-20 of the result."""
+    z, _ = R.gemm_w4(x, codes, scale, zero, group, bias, gelu)
+    of = np.arange(codes.shape[0]) // group
+    s = np.abs(x.astype(np.float64)) @ ((codes + (8.0 if zero is None else zero.astype(np.float64)[of])) * np.abs(scale.astype(np.float64))[of])
     d = (128 + 8 + 8 + codes.shape[0] / 256) * 2.0 ** -23 * (s + (0 if bias is None else np.abs(bias)))
     tol = 2.0 ** -11 * np.abs(z) + (1.13 if gelu else 1.0) * d + 2.0 ** -25 + (2.0 ** -19 * np.abs(z) + 2.0 ** -22 if gelu else 0)
     if residual is not None:
@@ -98,6 +101,16 @@ def test_w4_epilogue(lib, gpu, M, N, K, gelu, bias32):
     x, b, r = rng.standard_normal((M, K)).astype(np.float16), rng.standard_normal(N).astype(np.float16), rng.standard_normal((M, N)).astype(np.float16)
     got = _run(lib, x, *w, 32, bias=b, bias32=bias32, act=int(gelu), residual=r)
     _check(got, x, *w, 32, bias=b.astype(np.float64), gelu=gelu, residual=r)
+
+
+def test_w4_subnormal_and_large_rows(lib, gpu):
+    """Rows of the smallest halves and of large ones: the code's own subnormals are exact beside them."""
+    rng = np.random.default_rng(4)
+    w = _weights(rng, 512, 64, 128, True)
+    x = (rng.standard_normal((4, 512)) * np.array([[6e-8], [1e-4], [1.0], [3000.0]])).astype(np.float16)
+    w = (w[0], (w[1].astype(np.float32) * 16).astype(np.float16), w[2])
+    x[3] = np.clip(x[3], -60, 60)
+    _check(_run(lib, x, *w, 128), x, *w, 128)
 
 
 def test_w4_exact_on_integers(lib, gpu):
