@@ -316,7 +316,7 @@ int sh_attention_batched_prefetch(uint64_t q, uint64_t k, uint64_t v, uint64_t o
 typedef struct {
     uint64_t k;           /* codes: pages of [hkv][bs][dh], 16-byte aligned */
     uint64_t v;           /* codes: pages of [hkv][dh][bs], 16-byte aligned */
-    uint64_t ks, vs;      /* fp32 scales: pages of [hkv] */
+    uint64_t ks, vs;      /* fp32 scales, finite and >= 0: pages of [hkv] */
     uint64_t pgk, pgv;    /* bytes from a page to the next, multiples of 16 and >= hkv bs dh; 0: hkv bs dh */
     uint32_t pgs;         /* floats from a page's scales to the next page's, >= hkv; 0: hkv */
     uint32_t pages;       /* pages of the cache, pages x bs < 2^31 */
@@ -352,7 +352,7 @@ int sh_kv_slots(uint64_t table, uint32_t ld, uint64_t lens, uint64_t lens_out, u
  * page anew; other codes of the page are left as they are. 0, -1, SH_EHIP. */
 int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uint32_t ldv, uint64_t slots, uint32_t rows);
 
-/* Causal attention of new rows over the cache: o = softmax(scale q k^T) v per head, fp32 sums. Request b's rows are
+/* Causal attention of new rows over the cache: o = softmax(scale q k^T) v per head, scale > 0, fp32 sums. Request b's rows are
  * row_start[b] .. row_start[b + 1] - 1 of q / o (fp16, [rows][H dh]; row_start = 0: row b), its keys the first kv_len[b]
  * tokens of its table row, and its last row sees all of them, each earlier row one key less. window > 0: a row sees
  * only its last `window` keys; pages wholly before every row's window are not read. Head h reads key / value head h / (H / hkv). Keys

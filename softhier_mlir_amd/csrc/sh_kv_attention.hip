@@ -537,6 +537,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
         if (blockIdx.x == 0 && tid == 0) a.meta[0].x = 0;
         return;
     }
+    // (all of it is uniform: kept in scalar registers)
+    const auto uni = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+    s = Seq{uni(s.r0), uni(s.n), uni(s.nf), uni(s.nqt), uni(s.ft), uni(s.nt), (int32_t)uni((uint32_t)s.L)};
+    b = uni(b); parts = uni(parts); idx = uni(idx); cut0 = uni(cut0);
     const uint32_t h = idx % c.hkv, sp = idx / c.hkv % parts, qt = s.nqt - 1 - idx / c.hkv / parts, cut = cut0 + idx;
     if (parts > 1 && cut >= 2 * CUT) return;                        // (row ranges that overlap beyond measure: nothing outside ws)
 
@@ -565,37 +569,36 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
         qf[k] = __builtin_bit_cast(sh_h8, x);
     }
 
-    // ---- staging: K chunk i is key (tid + 256 i) / (DP / 16), column 16 (tid % (DP / 16)); V chunk i is column d (tid + 256 i) / 4,
-    // keys 16 (tid % 4)
-    const int32_t *tb = a.table + (uint64_t)b * a.ld;
+    // ---- staging: K chunk i of the wave is keys (64 wave + 256 i) / (DP / 16) on (16 at most, of one page), a lane 16 columns of one;
+    // V chunk i is keys 16 wave .. 16 wave + 15 of column 64 i + lane. So a wave's pages are scalars, a lane's offsets constants.
+    typedef const __attribute__((address_space(4))) int32_t *Table;
+    const Table tb = (Table)(uintptr_t)(a.table + (uint64_t)b * a.ld);
     const uint32_t npg = max((uint32_t)(s.L + c.bs - 1) >> c.lbs, 1u), hoff = h * c.bs * dh;
-    const uint32_t kcol = 16 * (tid % (DP / 16)), vg = tid & 3;
+    const uint32_t kcol = 16 * (lane % (DP / 16)), kofs = lane / (DP / 16) * dh + (kcol < dh ? kcol : 0);
+    uint32_t vofs[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) vofs[i] = min(64u * i + lane, dh - 1) * c.bs;
     uint32_t kpg[NC], vpg = 0, vpc = 0;
     uint4 kr[NC], vr[NC];
     float ksc = 0.f, vsc = 0.f;
-    const auto key_of = [&](int i) { return (tid + 256u * i) / (DP / 16); };
+    const auto key_of = [&](int i) { return (64u * wave + 256u * i) / (DP / 16); };
     const auto pages = [&](uint32_t j) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) kpg[i] = (uint32_t)tb[min((j * KT + key_of(i)) >> c.lbs, npg - 1)];
-        vpg = (uint32_t)tb[min((j * KT + 16 * vg) >> c.lbs, npg - 1)];
+        vpg = (uint32_t)tb[min((j * KT + 16 * wave) >> c.lbs, npg - 1)];
     };
     const auto load = [&](uint32_t j) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             const uint32_t p = kpg[i] < c.pages ? kpg[i] : 0, key = (j * KT + key_of(i)) & (c.bs - 1);
-            kr[i] = kcol < dh ? *(const uint4 *)(c.k + p * c.pgk + hoff + key * dh + kcol) : make_uint4(0, 0, 0, 0);
+            kr[i] = *(const uint4 *)(c.k + (uint64_t)p * c.pgk + (hoff + key * dh) + kofs);
         }
         vpc = vpg;
-        const uint32_t p = vpg < c.pages ? vpg : 0, key = (j * KT + 16 * vg) & (c.bs - 1);
+        const uint32_t p = vpg < c.pages ? vpg : 0, key = (j * KT + 16 * wave) & (c.bs - 1);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const uint32_t d = (tid + 256 * i) / 4;
-            vr[i] = d < dh ? *(const uint4 *)(c.v + p * c.pgv + hoff + d * c.bs + key) : make_uint4(0, 0, 0, 0);
-        }
-        if (tid < 4) {
-            ksc = c.ks[(uint64_t)p * c.pgs + h] * a.sc;
-            vsc = c.vs[(uint64_t)p * c.pgs + h];
-        }
+        for (int i = 0; i < NC; ++i) vr[i] = *(const uint4 *)(c.v + (uint64_t)p * c.pgv + (hoff + key) + vofs[i]);
+        ksc = c.ks[(uint64_t)p * c.pgs + h];
+        vsc = c.vs[(uint64_t)p * c.pgs + h];
     };
     const auto store16 = [](uint16_t *p, uint4 v) {
         *(sh_h8 *)p = kv_half8<FP8>(v.x, v.y);
@@ -603,7 +606,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
     };
     const auto stage = [&](uint32_t j) {
         const uint32_t u = j & 1;
-        const int32_t at = (int32_t)(j * KT + 16 * vg);
+        const int32_t at = (int32_t)(j * KT + 16 * wave);
         const bool bad = vpc >= c.pages;
         const int lo = bad ? 16 : max(slo - at, 0), hic = max(pmax + 1 - at, 0);            // what no row sees may hold anything
         if (lo > 0 || hic < 16)
@@ -611,13 +614,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
             for (int i = 0; i < NC; ++i) vr[i] = keep_bytes(vr[i], lo, hic);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            store16(&s_k[u][key_of(i) * KLD + kcol], kr[i]);
-            store16(&s_v[u][(tid + 256 * i) / 4 * VLD + 16 * vg], vr[i]);
+            // (columns past the head's width: zeros, for whatever bytes were read)
+            store16(&s_k[u][(key_of(i) + lane / (DP / 16)) * KLD + kcol], kcol < dh ? kr[i] : make_uint4(0, 0, 0, 0));
+            store16(&s_v[u][(64 * i + lane) * VLD + 16 * wave], vr[i]);
         }
-        if (tid < 4) {
-            s_sc[u][tid][0] = ksc;
-            s_sc[u][tid][1] = lo >= min(hic, 16) ? 0.f : vsc;
-            s_bad[u][tid] = bad;
+        if (lane == 0) {
+            s_sc[u][wave][0] = fmaxf(ksc * a.sc, 1e-37f);
+            s_sc[u][wave][1] = lo >= min(hic, 16) ? 0.f : vsc;
+            s_bad[u][wave] = bad;
         }
     };
 
@@ -642,24 +646,18 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
         const uint32_t u = j & 1;
         const int32_t k0 = (int32_t)(j * KT);
         if (k0 > wmax || (win && k0 + (int32_t)KT <= max(wmin, 0) - win + 1)) continue;     // this wave's rows see none of these keys
-        sh_f16v sa[2];
+        sh_f16v sa[2] = {};
+        const uint16_t *kp = &s_k[u][krow * KLD + 8 * hi];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            sa[t] = sh_f16v{};
-            const uint16_t *kp = &s_k[u][(32 * t + krow) * KLD + 8 * hi];
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) sa[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const sh_h8 *)(kp + 16 * k), qf[k], sa[t], 0, 0, 0);
-        }
+            for (int t = 0; t < 2; ++t)
+                sa[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const sh_h8 *)(kp + 32 * t * KLD + 16 * k), qf[k], sa[t], 0, 0, 0);
         float ks[4], vs[4];
         uint32_t bad = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) { ks[q] = s_sc[u][q][0]; vs[q] = s_sc[u][q][1]; bad |= s_bad[u][q] << q; }
         bad = __builtin_amdgcn_readfirstlane(bad);
-        float x[4][8];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[q][e] = sa[q >> 1][8 * (q & 1) + e] * ks[q];
         if (k0 + (int32_t)KT - 1 > wmin || (win && k0 < wmax - win + 1) || bad) {
             const int32_t at = k0 + 8 * (int32_t)hi, from = win ? max(pos, 0) - win + 1 : 0;
 #pragma unroll
@@ -667,12 +665,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int32_t key = at + 16 * q + e;
-                    x[q][e] = key <= pos && key >= from && !(bad >> q & 1) ? x[q][e] : -INFINITY;
+                    float &x = ((float *)&sa[q >> 1])[8 * (q & 1) + e];
+                    x = key <= pos && key >= from && !(bad >> q & 1) ? x : -INFINITY;
                 }
         }
-        float tm = x[0][0];
+        // a page's scores have one scale: its largest is the largest product's
+        float tm = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < 32; ++i) tm = fmaxf(tm, x[i >> 3][i & 7]);
+        for (int q = 0; q < 4; ++q) {
+            float m8 = sa[q >> 1][8 * (q & 1)];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) m8 = fmaxf(m8, sa[q >> 1][8 * (q & 1) + e]);
+            tm = fmaxf(tm, m8 * ks[q]);
+        }
         const float mn = fmaxf(mx, sh_max_xor32(tm)), vm = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
         float cs = cn;
         if (!(vm * cn <= 16384.f) || cn == 0.f) cs = __builtin_amdgcn_ldexpf(1.f, 14 - (vm > 1e-30f ? __builtin_amdgcn_frexp_expf(vm) : -99));
@@ -684,16 +689,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
             mx = mn;
             cn = cs;
         }
+        // probability and weight in one exponential: 2^(score - maximum + log2 w), the sum taken back from it
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float w = vs[q] * cn;
+            const float w = fmaxf(vs[q] * cn, 1e-30f), z = __builtin_amdgcn_logf(w) - mx;
+            float sum = 0.f;
             sh_h8 pf;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float p = sh_fast_exp2(x[q][e] - mx);
-                l += p;
-                pf[e] = (_Float16)(p * w);
+                const float p = sh_fast_exp2(fmaf(sa[q >> 1][8 * (q & 1) + e], ks[q], z));
+                sum += p;
+                pf[e] = (_Float16)p;
             }
+            l = fmaf(sum, sh_fast_rcp(w), l);
             const uint16_t *vp = &s_v[u][n * VLD + 16 * q + 8 * hi];
 #pragma unroll
             for (int i = 0; i < DT; ++i) oa[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const sh_h8 *)(vp + 32 * i * VLD), pf, oa[i], 0, 0, 0);
@@ -828,7 +836,7 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     }
     const uint32_t grp = H / c->hkv;
     if ((uint64_t)min(max_q, rows) * grp >= (1ull << 31)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", max_q, H); return -1; }
-    if (!(fabsf(scale) <= 3.4e38f)) { sh_set_error(-1, "[sh_attention_kv] scale is not finite"); return -1; }
+    if (!(scale > 0.f && scale <= 3.4e38f)) { sh_set_error(-1, "[sh_attention_kv] scale %g must be positive and finite", (double)scale); return -1; }
     const uint64_t need = sh_attention_kv_ws_bytes(c, B, rows, max_q, H, ld_table);
     if (!ws || ws % 16) { sh_set_error(-1, "[sh_attention_kv] ws must be a 16-byte aligned address"); return -1; }
     if (ws_bytes < need) {

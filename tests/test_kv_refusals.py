@@ -48,7 +48,7 @@ def test_attention_refusals(lib):
     assert need > 0
     good = [ONE, ONE, c, ONE, 4, ONE, 0, 2, 2, 1, 4, 256, 256, 0.125, 0, ONE, need]
     for i, v in ((0, 0), (1, 0), (2, None), (3, 0), (5, 0), (4, 0), (4, 1 << 27), (7, 65537), (8, 1 << 31), (10, 0), (10, 3), (11, 255), (12, 255),
-                 (13, float("nan")), (13, float("inf")), (15, 0), (15, ONE + 8), (0, ONE + 1), (6, ONE + 2)):
+                 (13, float("nan")), (13, float("inf")), (13, 0.0), (13, -0.125), (15, 0), (15, ONE + 8), (0, ONE + 1), (6, ONE + 2)):
         a = list(good)
         a[i] = v
         assert lib.sh_attention_kv(*a) == -1, (i, v)
