@@ -31,11 +31,12 @@ struct AttnArgs {
     uint16_t *o;
     const int32_t *table, *kv_len, *row_start;
     uint64_t ldq, ldo;
-    uint32_t ld, B, rows, max_q, grp, prow, window, groups, fast, whole;
+    uint32_t ld, B, rows, max_q, grp, prow, window, groups, wide, whole;
     float sc;                              // scale x log2 e
     float *part, *ml;                      // partials [groups][2][prow][dh], their (max, sum) [groups][2][prow][2]
     ChunkUnit *unit;                       // [2 CUT]
-    int4 *meta;                            // [groups]: request, item, last workgroup of the item begun here (-1: none)
+    int4 *meta;                            // [groups][2]: of the item begun here and not ended: its last tile (-1: none), first row, rows, head;
+                                           // the request's first row, tiles of a workgroup, workgroups with one more
 };
 
 struct Seq {
@@ -106,113 +107,128 @@ __device__ __forceinline__ uint32_t wave_scan32(uint32_t v) {
     v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
     return v;
 }
-__device__ __forceinline__ uint64_t div64(uint64_t a, uint32_t d) { return a >> 32 ? a / d : (uint64_t)((uint32_t)a / d); }
 __device__ __forceinline__ Seq lane_seq(const Seq &s, uint32_t b) {
     const auto rl = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)b); };
     return Seq{rl(s.r0), rl(s.n), rl(s.nf), rl(s.nqt), rl(s.ft), rl(s.nt), (int32_t)rl((uint32_t)s.L)};
 }
 
-// All tiles of all (request, head, row tile) items, one behind the other, are dealt out evenly: workgroup i of N takes
-// tiles i T / N .. (i + 1) T / N, its NW waves a share each. A wave that has an item from its first tile to its last stores the
+// All tiles of all (request, head, row tile) items, one behind the other, are dealt out evenly: T tiles to N workgroups, T / N
+// or one more each, and those to its NW waves. A wave that has an item from its first tile to its last stores the
 // result; parts of items are joined through LDS, and what crosses workgroups through `part` by k_kv_join. The lengths are
 // on the GPU only, so the host cannot choose a split; this one keeps every CU busy whether one request is long or many are short.
 // `whole`: where the table bounds an item to a few tiles for each wave, items are not cut between workgroups (each belongs to the
 // one its first tile falls to) and the joining launch is not made.
-// Up to 64 requests: a lane holds a request, every wave finds its tiles by itself; otherwise through LDS.
-template <int DP, bool FP8, bool FULL, int NW>
+// Up to 64 requests a lane holds a request and every wave finds its tiles by itself, up to a workgroup's threads they are in LDS
+// (`wide`); MANY: more, the lengths are read in rounds. What runs once is kept short: its instructions come from memory, not the
+// instruction cache, and cost more than the work (64-bit divisions and unrolled joins: one request of 937 keys 12.4 us against 9.4).
+template <int DP, bool FP8, bool FULL, int NW, bool MANY>
 __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     constexpr int NP = DP / 64, MT = DP / 16;
     extern __shared__ float s_o[];                                  // [2 NW][prow][DP]
     __shared__ float s_ml[2 * NW][QT][2];
-    __shared__ uint32_t s_seg[2 * NW][5];                           // request, item, first tile, end tile, tiles; request -1: none
-    __shared__ uint64_t s_sum[NW], s_base[NW];
-    __shared__ uint32_t s_b[NW];
+    __shared__ uint32_t s_seg[2 * NW][9];                           // request (-1: none), item, first tile, end tile, tiles; first row tile row, rows, head, first row
+    __shared__ uint32_t s_sum[NW], s_b[NW], s_base[NW], s_up[MANY ? 1 : 64 * NW];
+    __shared__ Seq s_seq[MANY ? 1 : 64 * NW];
     const KvCache &c = a.c;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
     const uint32_t dh = FULL ? DP : c.dh, wg = blockIdx.x;
+    const auto uni = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+    const auto at_lane = [](uint32_t v, uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
 
     // ---- this wave's tiles
     Seq mine{};
-    uint64_t T, g0, g1, t, t1, base = 0;
-    uint32_t N, b = 0;
+    uint32_t T = 0, up = 0;
     if (lane < 2) s_seg[2 * wave + lane][0] = ~0u;                  // (only this wave writes these two until the barrier)
-    if (a.fast) {
-        if (lane < a.B) mine = seq_of<QT>(a, lane);
-        const uint32_t w = mine.nt * mine.nqt * c.hkv, up = wave_scan32(w);
-        T = (uint32_t)__builtin_amdgcn_readlane((int)up, 63);
-        N = (uint32_t)min((uint64_t)a.groups, max(T / NW, (uint64_t)1));
-        if (wg >= N || T == 0) {
-            if (tid == 0 && !a.whole) a.meta[wg] = make_int4(-1, 0, 0, 0);
-            return;
-        }
-        g0 = wg * T / N;
-        g1 = (wg + 1) * T / N;
-        const auto owner = [&](uint64_t x) { return (uint32_t)__builtin_ctzll(__ballot(up > (uint32_t)x)); };    // x < T
-        const auto before = [&](uint32_t i) { return i ? (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)up, (int)i - 1) : 0ull; };
-        if (a.whole) {
-            const auto snap = [&](uint64_t x) {                     // the first item that begins at or behind x
-                if (x >= T) return T;
-                const uint32_t i = owner(x);
-                const uint64_t z = before(i);
-                const uint32_t nt = (uint32_t)__builtin_amdgcn_readlane((int)mine.nt, (int)i);
-                return z + ((uint32_t)(x - z) + nt - 1) / nt * nt;
-            };
-            g0 = snap(g0);
-            g1 = snap(g1);
-        }
-        t = g0 + wave * (g1 - g0) / NW;
-        t1 = g0 + (wave + 1) * (g1 - g0) / NW;
-        if (t < t1) { b = owner(t); base = before(b); }
-    } else {
-        uint64_t sum = 0;
-        for (uint32_t i = tid; i < a.B; i += 64 * NW) { const Seq s = seq_of<QT>(a, i); sum += (uint64_t)s.nt * s.nqt * c.hkv; }
-        sum = wave_sum64(sum);
-        if (lane == 0) s_sum[wave] = sum;
+    if constexpr (MANY) {
+        uint32_t sum = 0;
+        for (uint32_t i = tid; i < a.B; i += 64 * NW) { const Seq q = seq_of<QT>(a, i); sum += q.nt * q.nqt * c.hkv; }
+        sum = wave_scan32(sum);
+        if (lane == 63) s_sum[wave] = sum;
         __syncthreads();
-        T = 0;
         for (uint32_t i = 0; i < NW; ++i) T += s_sum[i];
-        N = (uint32_t)min((uint64_t)a.groups, max(T / NW, (uint64_t)1));
-        if (wg >= N || T == 0) {
-            if (tid == 0) a.meta[wg] = make_int4(-1, 0, 0, 0);
-            return;
+        __syncthreads();
+    } else {
+        const uint32_t ix = a.wide ? tid : lane;
+        if (ix < a.B) mine = seq_of<QT>(a, ix);
+        up = wave_scan32(mine.nt * mine.nqt * c.hkv);
+        T = at_lane(up, 63);
+        if (a.wide) {
+            if (lane == 63) s_sum[wave] = up;
+            s_seq[tid] = mine;
+            __syncthreads();
+            uint32_t z = 0;
+            T = 0;
+            for (uint32_t i = 0; i < NW; ++i) { const uint32_t v = s_sum[i]; z += i < wave ? v : 0u; T += v; }
+            s_up[tid] = up + z;
+            __syncthreads();
         }
-        g0 = wg * T / N;
-        g1 = (wg + 1) * T / N;
-        t = g0 + wave * (g1 - g0) / NW;
-        t1 = g0 + (wave + 1) * (g1 - g0) / NW;
-        uint64_t carry = 0;
+    }
+    T = uni(T);
+    const uint32_t N = min(a.groups, max(T / NW, 1u));
+    if (wg >= N || T == 0) {
+        if (tid == 0 && !a.whole) a.meta[2 * wg] = make_int4(-1, 0, 0, 0);
+        return;
+    }
+    const uint32_t share = T / N, more = T - share * N;
+    uint32_t g0 = wg * share + min(wg, more), g1 = g0 + share + (wg < more ? 1 : 0), b = 0, base = 0;
+    // the request that tile x < T belongs to
+    const auto owner = [&](uint32_t x) {
+        if (!a.wide) return (uint32_t)__builtin_ctzll(__ballot(up > x));
+        uint32_t lo = 0, hi = a.B - 1;
+        while (lo < hi) {
+            const uint32_t i = (lo + hi) / 2;
+            if (uni(s_up[i]) > x) hi = i; else lo = i + 1;
+        }
+        return lo;
+    };
+    const auto before = [&](uint32_t i) { return !i ? 0u : a.wide ? uni(s_up[i - 1]) : at_lane(up, i - 1); };
+    if (!MANY && a.whole) {
+        for (int k = 0; k < 2; ++k) {                               // to the first item that begins there or behind
+            uint32_t &x = k ? g1 : g0;
+            if (x >= T) continue;
+            const uint32_t i = owner(x), z = before(i), nt = a.wide ? uni(s_seq[i].nt) : at_lane(mine.nt, i);
+            x = z + (x - z + nt - 1) / nt * nt;
+        }
+    }
+    const uint32_t t0 = g0 + wave * (g1 - g0) / NW, t1 = g0 + (wave + 1) * (g1 - g0) / NW;
+    uint32_t t = t0;
+    if constexpr (MANY) {
+        uint32_t carry = 0;
         for (uint32_t b0 = 0; b0 < a.B; b0 += 64 * NW) {
             const uint32_t i = b0 + tid;
-            uint64_t w = 0;
-            if (i < a.B) { const Seq s = seq_of<QT>(a, i); w = (uint64_t)s.nt * s.nqt * c.hkv; }
-            uint64_t v = w;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint64_t x = (uint64_t)__shfl_up((long long)v, d);
-                if ((int)lane >= d) v += x;
-            }
+            uint32_t w = 0;
+            if (i < a.B) { const Seq q = seq_of<QT>(a, i); w = q.nt * q.nqt * c.hkv; }
+            uint32_t v = wave_scan32(w);
             __syncthreads();
             if (lane == 63) s_sum[wave] = v;
             __syncthreads();
-            uint64_t z = carry;
-            for (uint32_t k = 0; k < NW; ++k) { if (k < wave) z += s_sum[k]; carry += s_sum[k]; }
+            uint32_t z = carry;
+            for (uint32_t k = 0; k < NW; ++k) { const uint32_t x = s_sum[k]; z += k < wave ? x : 0u; carry += x; }
             v += z;
             for (uint32_t k = 0; k < NW; ++k) {
-                const uint64_t x = g0 + k * (g1 - g0) / NW;
+                const uint32_t x = g0 + k * (g1 - g0) / NW;
                 if (w && v - w <= x && x < v) { s_b[k] = i; s_base[k] = v - w; }
             }
         }
         __syncthreads();
-        if (t < t1) { b = __builtin_amdgcn_readfirstlane(s_b[wave]); base = s_base[wave]; }
+        if (t < t1) { b = uni(s_b[wave]); base = uni(s_base[wave]); }
+    } else if (t < t1) {
+        b = owner(t);
+        base = before(b);
     }
-    const auto get = [&](uint32_t i) { return a.fast ? lane_seq(mine, i) : seq_of<QT>(a, i); };
+    const auto get = [&](uint32_t i) {
+        if constexpr (!MANY)
+            if (!a.wide) return lane_seq(mine, i);
+        Seq q;
+        if constexpr (MANY) q = seq_of<QT>(a, i); else q = s_seq[i];
+        return Seq{uni(q.r0), uni(q.n), uni(q.nf), uni(q.nqt), uni(q.ft), uni(q.nt), (int32_t)uni((uint32_t)q.L)};
+    };
     Seq s{};
     uint32_t item = 0, j0 = 0;
     if (t < t1) {
         s = get(b);
-        const uint64_t in = t - base;
-        item = __builtin_amdgcn_readfirstlane((uint32_t)div64(in, s.nt));
-        j0 = __builtin_amdgcn_readfirstlane((uint32_t)(in - (uint64_t)item * s.nt));
+        item = uni((t - base) / s.nt);
+        j0 = uni(t - base - item * s.nt);
     }
     const uint32_t kg = m >> 2, kr0 = m & 3;
     uint32_t kcol[NP];                                              // columns past the head's width: read as its first ones, against zeros of Q
@@ -220,7 +236,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     for (int p = 0; p < NP; ++p) kcol[p] = FULL || 64 * p + 16 * g < dh ? 64 * p + 16 * g : 0;
     while (t < t1) {
         const uint32_t h = item / s.nqt, qt = item - h * s.nqt;
-        const uint32_t j1 = (uint32_t)min((uint64_t)s.nt, j0 + (t1 - t));
+        const uint32_t j1 = min(s.nt, j0 + (t1 - t));
         // ---- rows
         const uint32_t r = qt * QT + m, nrow = s.n * a.grp;
         const uint32_t qi = r / a.grp, qh = h * a.grp + (r - qi * a.grp);
@@ -292,9 +308,9 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
                 }
             }
             float x[16], vs = vsc;
-            const float ks = ksc * a.sc;
+            const float ks = fmaxf(ksc * a.sc, 1e-37f);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = sa[i >> 2][i & 3] * ks;
+            for (int i = 0; i < 16; ++i) x[i] = sa[i >> 2][i & 3];
             // the pages after the next tile's first (loads end in order), then its keys
             const uint32_t vcur = vp;
             if (j + 1 < jb) {
@@ -317,7 +333,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
             float tm = x[0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) tm = fmaxf(tm, x[i]);
-            tm = max_xor16_32(tm);
+            tm = max_xor16_32(tm * ks);                             // (a lane's scores have one scale)
             const float mn = fmaxf(mx, tm), vm = max_xor16_32(vs);
             float cs = cn;
             if (!(vm * cn <= 16384.f) || cn == 0.f) cs = __builtin_amdgcn_ldexpf(1.f, 14 - (vm > 1e-30f ? __builtin_amdgcn_frexp_expf(vm) : -99));
@@ -329,14 +345,17 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
                 mx = mn;
                 cn = cs;
             }
-            const float w = vs * cn;
+            // probability and weight in one exponential: 2^(score - maximum + log2 w), the sum taken back from it
+            const float w = fmaxf(vs * cn, 1e-30f), z = __builtin_amdgcn_logf(w) - mx;
+            float sum = 0.f;
             sh_h8 pf[2];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float e = sh_fast_exp2(x[i] - mx);
-                l += e;
-                pf[i >> 3][i & 7] = (_Float16)(e * w);
+                const float e = sh_fast_exp2(fmaf(x[i], ks, z));
+                sum += e;
+                pf[i >> 3][i & 7] = (_Float16)e;
             }
+            l = fmaf(sum, sh_fast_rcp(w), l);
 #pragma unroll
             for (int i = 0; i < MT; ++i)
                 if (FULL || 16u * i < dh) {
@@ -362,7 +381,10 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
                     if (FULL || 16u * i < dh) *(sh_f4v *)&s_o[(sg * a.prow + m) * DP + 16 * i + 4 * g] = oa[i] * ic;
                 if (g == 0) { s_ml[sg][m][0] = mx; s_ml[sg][m][1] = l; }
             }
-            if (lane == 0) { s_seg[sg][0] = b; s_seg[sg][1] = item; s_seg[sg][2] = j0; s_seg[sg][3] = j1; s_seg[sg][4] = s.nt; }
+            if (lane == 0) {
+                s_seg[sg][0] = b; s_seg[sg][1] = item; s_seg[sg][2] = j0; s_seg[sg][3] = j1; s_seg[sg][4] = s.nt;
+                s_seg[sg][5] = qt * QT; s_seg[sg][6] = nrow; s_seg[sg][7] = h; s_seg[sg][8] = s.r0;
+            }
         }
         t += j1 - j0;
         j0 = 0;
@@ -375,55 +397,48 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     }
     __syncthreads();
 
-    // ---- parts that belong together: consecutive, the first and the last may reach beyond this workgroup
-    if (tid == 0 && !a.whole) a.meta[wg] = make_int4(-1, 0, 0, 0);
+    // ---- parts that belong together: consecutive, the first and the last may reach beyond this workgroup. A wave takes every NW-th
+    // 64 elements (four columns of a row each) of all of them.
+    if (tid == 0 && !a.whole) a.meta[2 * wg] = make_int4(-1, 0, 0, 0);
     const uint32_t gs = min(lane, 2u * NW - 1);                     // lane i holds part i
-    const uint32_t gb = lane < 2 * NW ? s_seg[gs][0] : ~0u, gi = s_seg[gs][1], ga = s_seg[gs][2], ge = s_seg[gs][3], gn = s_seg[gs][4];
-    uint64_t left = __ballot(gb != ~0u);
-    while (left) {
-        const auto rl = [](uint32_t v, uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
-        const uint32_t i0 = __builtin_ctzll(left), bb = rl(gb, i0), it = rl(gi, i0);
-        const uint64_t in = __ballot(gb == bb && gi == it);
+    const uint32_t gb = lane < 2 * NW ? s_seg[gs][0] : ~0u, gi = s_seg[gs][1];
+    const uint32_t qn = dh / 4, blocks = (a.prow * qn + 63) / 64;
+    uint32_t turn = wave;
+    for (uint64_t left = __ballot(gb != ~0u); left;) {
+        const uint32_t i0 = __builtin_ctzll(left);
+        const uint64_t in = __ballot(gb == at_lane(gb, i0) && gi == at_lane(gi, i0));
         left &= ~in;
-        const uint32_t ja = rl(ga, i0), nt = rl(gn, i0), je = rl(ge, 63 - __builtin_clzll(in));
-        const Seq q = get(bb);
-        const uint32_t h = it / q.nqt, qt = it - h * q.nqt, nrow = q.n * a.grp, qn = dh / 4;
+        const uint32_t iz = 63 - __builtin_clzll(in);
+        const uint32_t ja = uni(s_seg[i0][2]), je = uni(s_seg[iz][3]), nt = uni(s_seg[i0][4]), q0 = uni(s_seg[i0][5]), nrow = uni(s_seg[i0][6]),
+                       h = uni(s_seg[i0][7]), r0 = uni(s_seg[i0][8]);
         const bool all = ja == 0 && je == nt;
-        const uint32_t slot = ja ? 0 : 1;
-        for (uint32_t e = tid; e < a.prow * qn; e += 64 * NW) {
-            const uint32_t row = e / qn, d = 4 * (e - row * qn), r = qt * QT + row;
-            if (r >= nrow) continue;
-            // every read is made, a part of another item's from the first part's place and without weight: none waits for another
-            float pm[2 * NW], pl[2 * NW], M = -1e30f, l = 0.f;
-            sh_f4v o = {0.f, 0.f, 0.f, 0.f}, po[2 * NW];
-#pragma unroll
-            for (uint32_t i = 0; i < 2 * NW; ++i) {
-                const uint32_t at = in >> i & 1 ? i : i0;
-                pm[i] = s_ml[at][row][0];
-                pl[i] = s_ml[at][row][1];
-                po[i] = *(const sh_f4v *)&s_o[(at * a.prow + row) * DP + d];
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 2 * NW; ++i) M = fmaxf(M, pm[i]);
-#pragma unroll
-            for (uint32_t i = 0; i < 2 * NW; ++i) {
-                const float f = in >> i & 1 ? sh_fast_exp2(pm[i] - M) : 0.f;
-                l += f * pl[i];
-                o += f * po[i];
+        for (; turn < blocks; turn += NW) {
+            const uint32_t e = turn * 64 + lane, row = e / qn, d = 4 * (e - row * qn), r = q0 + row;
+            if (row >= a.prow || r >= nrow) continue;
+            float M = -1e30f, l = 0.f;
+            sh_f4v o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (uint64_t k = in; k; k &= k - 1) {
+                const uint32_t i = __builtin_ctzll(k);
+                const float pm = s_ml[i][row][0], mn = fmaxf(M, pm), f = sh_fast_exp2(M - mn), x = sh_fast_exp2(pm - mn);
+                l = l * f + s_ml[i][row][1] * x;
+                o = o * f + *(const sh_f4v *)&s_o[(i * a.prow + row) * DP + d] * x;
+                M = mn;
             }
             if (all) {
                 const float f = l > 0.f || l != l ? 1.f / l : 0.f;
                 const uint32_t qi = r / a.grp, qh = h * a.grp + (r - qi * a.grp);
-                store4(a.o + (uint64_t)(q.r0 + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+                store4(a.o + (uint64_t)(r0 + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
             } else {
-                const uint64_t at = ((uint64_t)wg * 2 + slot) * a.prow + row;
+                const uint64_t at = ((uint64_t)wg * 2 + (ja ? 0 : 1)) * a.prow + row;
                 *(sh_f4v *)&a.part[at * dh + d] = o;
                 if (d == 0) { a.ml[at * 2] = M; a.ml[at * 2 + 1] = l; }
             }
         }
-        if (!all && slot && tid == 0) {
-            const uint64_t te = g1 + (nt - je);                                          // the item's end: it leaves here at je
-            a.meta[wg] = make_int4((int)bb, (int)it, (int)((te * N - 1) / T), 0);
+        turn -= blocks;
+        if (!all && !ja && tid == 0) {                              // it begins here and leaves at je: where it ends, and how tiles are shared
+            a.meta[2 * wg] = make_int4((int)(g1 + (nt - je) - 1), (int)q0, (int)nrow, (int)h);
+            a.meta[2 * wg + 1] = make_int4((int)r0, (int)share, (int)more, 0);
         }
     }
 }
@@ -434,15 +449,16 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
     constexpr uint32_t L = DP / 4, P = 256 / L;                     // lanes of a row, parts in flight
     __shared__ sh_f4v s_o[256];
     __shared__ float s_m[P], s_l[P];
-    const int4 me = a.meta[blockIdx.x];
-    if (me.x < 0) return;
-    const uint32_t wg = blockIdx.x, dh = a.c.dh, row = blockIdx.y, y = threadIdx.x / L, d = 4 * (threadIdx.x % L);
-    const Seq q = seq_of<QT>(a, (uint32_t)me.x);
-    const uint32_t h = (uint32_t)me.y / q.nqt, qt = (uint32_t)me.y - h * q.nqt, r = qt * QT + row;
-    if (r >= q.n * a.grp) return;
+    const int4 me = a.meta[2 * blockIdx.x], at_ = a.meta[2 * blockIdx.x + 1];
+    if (me.x == -1) return;
+    const uint32_t wg = blockIdx.x, dh = a.c.dh, row = blockIdx.y, y = threadIdx.x / L, d = 4 * (threadIdx.x % L), r = (uint32_t)me.y + row;
+    if (r >= (uint32_t)me.z) return;
+    // the workgroup of the item's last tile
+    const uint32_t x = (uint32_t)me.x, share = (uint32_t)at_.y, more = (uint32_t)at_.z, big = more * (share + 1);
+    const uint32_t end = x < big ? x / (share + 1) : more + (x - big) / share;
     float M = -1e30f, l = 0.f;
     sh_f4v o = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t i = wg + y; i <= (uint32_t)me.z; i += P) {
+    for (uint32_t i = wg + y; i <= end; i += P) {
         const uint64_t at = ((uint64_t)i * 2 + (i == wg ? 1 : 0)) * a.prow + row;
         const float m = a.ml[at * 2], s = a.ml[at * 2 + 1];
         const sh_f4v v = d < dh ? *(const sh_f4v *)&a.part[at * dh + d] : sh_f4v{0.f, 0.f, 0.f, 0.f};
@@ -465,8 +481,8 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
     }
     if (d >= dh) return;
     const float f = t > 0.f || t != t ? 1.f / t : 0.f;
-    const uint32_t qi = r / a.grp, qh = h * a.grp + (r - qi * a.grp);
-    store4(a.o + (uint64_t)(q.r0 + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+    const uint32_t qi = r / a.grp, qh = (uint32_t)me.w * a.grp + (r - qi * a.grp);
+    store4(a.o + (uint64_t)((uint32_t)at_.x + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
 }
 
 // ---- many rows: chunks of prompts ------------------------------------------------------------------------------------
@@ -765,20 +781,26 @@ __global__ __launch_bounds__(256) void k_kv_chunk_join(AttnArgs a) {
 
 uint32_t part_rows(uint32_t max_q, uint32_t grp) { return (uint32_t)min((uint64_t)QT, (uint64_t)max_q * grp); }
 
-template <int DP, bool FP8, bool FULL, int NW>
-bool launch_attn(AttnArgs a, uint32_t tiles, hipStream_t st) {
+template <int DP, bool FP8, bool FULL, int NW, bool MANY>
+bool launch_attn_many(const AttnArgs &a, hipStream_t st) {
     static bool set = false;
     const uint32_t lds = 2 * NW * a.prow * DP * 4;
     if (!set) {
-        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_kv_attn<DP, FP8, FULL, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * NW * QT * DP * 4),
+        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_kv_attn<DP, FP8, FULL, NW, MANY>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * NW * QT * DP * 4),
                        "sh_attention_kv hipFuncSetAttribute")) return false;
         set = true;
     }
-    a.groups = DP == 128 ? GROUPS / 2 : GROUPS;
-    a.whole = a.fast && tiles <= WHOLE_TILES * NW;
-    hipLaunchKernelGGL((k_kv_attn<DP, FP8, FULL, NW>), dim3(a.groups), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL((k_kv_attn<DP, FP8, FULL, NW, MANY>), dim3(a.groups), dim3(64 * NW), lds, st, a);
     if (!a.whole) hipLaunchKernelGGL(k_kv_join<DP>, dim3(a.groups, a.prow), dim3(256), 0, st, a);
     return sh_launch_ok("sh_attention_kv");
+}
+template <int DP, bool FP8, bool FULL, int NW>
+bool launch_attn(AttnArgs a, uint32_t tiles, hipStream_t st) {
+    a.groups = DP == 128 ? GROUPS / 2 : GROUPS;
+    if (a.B > 64 * NW) return launch_attn_many<DP, FP8, false, NW, true>(a, st);
+    a.wide = a.B > 64;
+    a.whole = tiles <= WHOLE_TILES * NW;
+    return launch_attn_many<DP, FP8, FULL, NW, false>(a, st);
 }
 template <bool FP8>
 bool launch_attn_width(const AttnArgs &a, uint32_t tiles, hipStream_t st) {
@@ -811,7 +833,7 @@ uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t row
     max_q = min(max_q, rows);
     if (chunked(max_q, H / c->hkv)) return 2 * CUT * ((uint64_t)CT * (c->dh + 2) * 4 + sizeof(ChunkUnit)) + 16;
     const uint64_t prow = part_rows(max_q, H / c->hkv);
-    return (uint64_t)GROUPS * (2 * prow * (c->dh + 2) * 4 + 16);
+    return (uint64_t)GROUPS * (2 * prow * (c->dh + 2) * 4 + 32);
 }
 
 int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table, uint32_t ld_table, uint64_t kv_len, uint64_t row_start,
@@ -862,12 +884,15 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
         a.ml = a.part + (uint64_t)2 * CUT * CT * c->dh;
         return (c->fmt == SH_FP8 ? launch_chunk<true>(a, units, st) : launch_chunk<false>(a, units, st)) ? 0 : SH_EHIP;
     }
-    a.part = (float *)(ws + GROUPS * 16);
+    a.part = (float *)(ws + GROUPS * 32);
     a.ml = a.part + (uint64_t)GROUPS * 2 * a.prow * c->dh;
     uint64_t tiles = ((uint64_t)ld_table * c->bs + KT - 1) / KT + 1;                     // an item's, at most
     if (a.window) tiles = min(tiles, ((uint64_t)a.window + a.max_q) / KT + 2);
     const uint64_t items = (uint64_t)c->hkv * (((uint64_t)a.max_q * grp + QT - 1) / QT);
-    a.fast = B <= 64 && tiles * items < (1ull << 31) / B;
+    if (tiles * items >= (1ull << 32) / B) {                        // (tile counts of 32 bits)
+        sh_set_error(-1, "[sh_attention_kv] %u requests of up to %llu tokens and %u heads", B, (unsigned long long)ld_table * c->bs, H);
+        return -1;
+    }
     const bool ok = c->fmt == SH_FP8 ? launch_attn_width<true>(a, (uint32_t)tiles, st) : launch_attn_width<false>(a, (uint32_t)tiles, st);
     return ok ? 0 : SH_EHIP;
 }
