@@ -28,9 +28,10 @@ namespace {
 
 // ---- sh_kv_slots --------------------------------------------------------------------------------------------------
 // Three prefix sums over the requests (rows, pages taken, pages given back) decide everything; the work behind them is
-// one write for each new row, new page and returned page. Requests are scanned in chunks of the workgroup's threads; within a
-// chunk the rows and pages are spread evenly over threads (a binary search in the chunk's sums finds a row's request), so
-// one long prompt costs as much as many short requests.
+// one write for each new row, new page and returned page. Requests are scanned in chunks of the workgroup's threads. Where a chunk's
+// requests add a few rows each, a thread writes its own; else rows and pages are spread evenly over the threads of all
+// workgroups (a binary search in the chunk's sums finds a row's request), so one long prompt costs as much as many short requests.
+// Bound by latency: a launch, the lengths, then a page, then the writes.
 struct SlotArgs {
     int32_t *table; uint32_t ld;
     const int32_t *lens, *add, *state;
@@ -39,132 +40,133 @@ struct SlotArgs {
     uint32_t commit;     // this launch writes the new lengths and the ring's state
     uint32_t fill;       // this launch writes everything else
 };
+constexpr uint32_t OWN = 4;                // rows of a request up to which its thread writes them
 
-// Inclusive sum over the wave's lanes of a value split in 64 bits.
-__device__ __forceinline__ int64_t wave_scan64(int64_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
     return v;
 }
 
 // Inclusive sum over the workgroup, and its total; `part` holds one value a wave.
 template <int T>
-__device__ __forceinline__ int64_t group_scan64(int64_t v, int64_t *part, int64_t &total) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    v = wave_scan64(v);
+__device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t *part, uint32_t &total) {
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    v = wave_scan(v);
     if (lane == 63) part[wave] = v;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < T / 64; ++w) {
-        const int64_t p = part[w];
-        before += w < wave ? p : 0;
-        total += p;
-    }
-    __syncthreads();
-    return v + before;
+    const uint32_t p = wave_scan(lane < T / 64 ? part[lane] : 0u);
+    total = (uint32_t)__builtin_amdgcn_readlane((int)p, 63);
+    return v + (wave ? (uint32_t)__builtin_amdgcn_readlane((int)p, (int)__builtin_amdgcn_readfirstlane(wave) - 1) : 0u);
 }
 
 template <int T>
 __global__ __launch_bounds__(T) void k_kv_slots(SlotArgs a) {
-    __shared__ int64_t part[T / 64];
-    __shared__ int32_t s_end[T], s_need[T], s_back[T], s_len[T], s_flag[T];     // sums within the chunk; flag: request is served
-    __shared__ int32_t s_used, s_refused;
-    const uint32_t tid = threadIdx.x, bs = 1u << a.lbs;
-    const int64_t cap = (int64_t)a.ld << a.lbs;
-    const int32_t head = a.state[0], count0 = a.state[1];
-    const int64_t count = min(max(count0, 0), (int32_t)a.pages);
-    const uint32_t h0 = (uint32_t)max(head, 0) % a.pages;
+    __shared__ uint32_t part[3][T / 64];
+    __shared__ uint32_t s_end[T], s_need[T], s_back[T];              // sums within the chunk
+    __shared__ int32_t s_len[T], s_flag[T];                          // flag: the request is served
+    __shared__ uint32_t s_used, s_refused;
+    const uint32_t tid = threadIdx.x, bs = 1u << a.lbs, cap = a.ld << a.lbs;
+    const uint32_t count = (uint32_t)min(max(a.state[1], 0), (int32_t)a.pages), h0 = (uint32_t)max(a.state[0], 0) % a.pages;
+    const auto ring = [&](uint32_t i) {                              // i < 2^31 places behind the ring's first entry
+        const uint32_t x = h0 + i;
+        return x < a.pages ? x : x - a.pages < a.pages ? x - a.pages : x % a.pages;
+    };
     if (tid == 0) s_used = s_refused = 0;
-    int64_t rows0 = 0, need0 = 0, back0 = 0;                                    // the earlier chunks' sums
+    uint32_t rows0 = 0, need0 = 0, back0 = 0;                        // the earlier chunks' sums
     for (uint32_t b0 = 0; b0 < a.B; b0 += T) {
         const uint32_t b = b0 + tid;
-        const int32_t ad = b < a.B ? a.add[b] : 0;
-        const int64_t raw = b < a.B ? a.lens[b] : 0, len = min(max(raw, (int64_t)0), cap), n = max(ad, 0);
-        int64_t total_n, total_np;
-        const int64_t end = rows0 + group_scan64<T>(n, part, total_n);
-        bool ok = b < a.B && ad >= 0 && len + n <= cap && end <= (int64_t)a.rows;
-        const int32_t have = (int32_t)((len + bs - 1) >> a.lbs);
-        const int32_t need = ok ? (int32_t)((len + n + bs - 1) >> a.lbs) - have : 0, back = ad < 0 ? have : 0;
-        // both page sums stay below B ld < 2^31: one scan of the pair
-        const int64_t np = group_scan64<T>((int64_t)need << 32 | back, part, total_np);
-        const int64_t upto = need0 + (np >> 32);
+        const int32_t ad = b < a.B ? a.add[b] : 0, raw = b < a.B ? a.lens[b] : 0;
+        const uint32_t len = min((uint32_t)max(raw, 0), cap), n = (uint32_t)max(ad, 0);
+        uint32_t total_n, total_need, total_back;
+        const uint32_t in_n = group_scan<T>(n, part[0], total_n), end = rows0 + in_n;
+        bool ok = b < a.B && ad >= 0 && n <= cap - len && end <= a.rows;
+        const uint32_t have = (len + bs - 1) >> a.lbs, need = ok ? ((len + n + bs - 1) >> a.lbs) - have : 0, back = ad < 0 ? have : 0;
+        const uint32_t in_need = group_scan<T>(need, part[1], total_need), in_back = group_scan<T>(back, part[2], total_back);
+        const uint32_t upto = need0 + in_need, need_b = upto - need;
         ok = ok && (need == 0 || upto <= count);
-        if (need && ok) atomicMax(&s_used, (int32_t)upto);
+        if (need && ok) atomicMax(&s_used, upto);
         if (b < a.B && ad >= 0 && !ok) atomicAdd(&s_refused, 1);
-        if (b < a.B && a.commit) a.lens_out[b] = ok ? (int32_t)(len + n) : ad < 0 ? 0 : (int32_t)raw;
+        const int32_t *row = a.table + (uint64_t)b * a.ld;
+        // the ring's ranges taken from and given back to do not meet: together they are at most `pages` long
         if (a.fill) {
-            if (b < a.B && blockIdx.x == 0) {
+            const bool few = !__syncthreads_or(n > OWN || back);
+            if (blockIdx.x == 0 && b < a.B) {
                 a.row_start[b] = (int32_t)(end - n);
                 a.kv_len[b] = ok ? (int32_t)(len + n) : 0;
                 if (b == a.B - 1) a.row_start[a.B] = (int32_t)end;
             }
-            s_end[tid] = (int32_t)min(end - rows0, (int64_t)a.rows);            // (only rows below a.rows are looked up)
-            s_need[tid] = (int32_t)(np >> 32);
-            s_back[tid] = (int32_t)(uint32_t)np;
-            s_len[tid] = (int32_t)len;
-            s_flag[tid] = ok;
-            __syncthreads();
-            const uint32_t stride = T * gridDim.x, first = blockIdx.x * T + tid;
-            auto find = [&](const int32_t *s, int32_t i) {                      // first request whose sum exceeds i
-                uint32_t lo = 0, hi = T - 1;
-                while (lo < hi) {
-                    const uint32_t m = (lo + hi) / 2;
-                    if (s[m] > i) hi = m; else lo = m + 1;
+            if (few) {
+                if (blockIdx.x == 0 && b < a.B && n) {
+                    // n <= 4 rows lie in at most one page held and one page taken
+                    const int32_t held = (len & (bs - 1)) && ok ? row[len >> a.lbs] : 0, taken = need && ok ? a.pool[ring(need_b)] : 0;
+                    if (need && ok) a.table[(uint64_t)b * a.ld + have] = taken;
+                    for (uint32_t i = 0; i < n; ++i) {
+                        const uint32_t r = end - n + i, at = len + i;
+                        const int32_t page = (at >> a.lbs) < have ? held : taken;
+                        if (r >= a.rows) break;
+                        a.slots[r] = ok && (uint32_t)page < a.pages ? (int32_t)(((uint32_t)page << a.lbs) + (at & (bs - 1))) : -1;
+                        a.pos[r] = ok ? (int32_t)at : -1;
+                    }
                 }
-                return lo;
-            };
-            // the ring's ranges taken from and given back to do not meet: together they are at most `pages` long
-            const uint32_t pages_new = (uint32_t)(total_np >> 32), pages_back = (uint32_t)total_np;
-            for (uint32_t i = first; i < pages_new; i += stride) {
-                const uint32_t f = find(s_need, (int32_t)i);
-                if (!s_flag[f]) continue;
-                const uint32_t j = i - (f ? (uint32_t)s_need[f - 1] : 0u), hv = ((uint32_t)s_len[f] + bs - 1) >> a.lbs;
-                a.table[(uint64_t)(b0 + f) * a.ld + hv + j] = a.pool[(uint32_t)((h0 + (uint64_t)need0 + i) % a.pages)];
-            }
-            for (uint32_t i = first; i < pages_back; i += stride) {
-                const uint32_t f = find(s_back, (int32_t)i);
-                const uint32_t j = i - (f ? (uint32_t)s_back[f - 1] : 0u);
-                a.pool[(uint32_t)((h0 + (uint64_t)count + back0 + i) % a.pages)] = a.table[(uint64_t)(b0 + f) * a.ld + j];
-            }
-            const int64_t rows_here = min(total_n, (int64_t)a.rows - min(rows0, (int64_t)a.rows));
-            for (int64_t i = first; i < rows_here; i += stride) {
-                const uint32_t f = find(s_end, (int32_t)i);
-                const uint32_t at = (uint32_t)s_len[f] + (uint32_t)(i - (f ? s_end[f - 1] : 0)), j = at >> a.lbs;
-                int32_t slot = -1, p = -1;
-                if (s_flag[f]) {
-                    // a page of this step is read from the ring: its table entry is being written
-                    const uint32_t hv = ((uint32_t)s_len[f] + bs - 1) >> a.lbs, nb = f ? (uint32_t)s_need[f - 1] : 0u;
-                    const int32_t page = j < hv ? a.table[(uint64_t)(b0 + f) * a.ld + j]
-                                                : a.pool[(uint32_t)((h0 + (uint64_t)need0 + nb + (j - hv)) % a.pages)];
-                    p = (int32_t)at;
-                    if ((uint32_t)page < a.pages) slot = (int32_t)(((uint32_t)page << a.lbs) + (at & (bs - 1)));
+            } else {
+                s_end[tid] = in_n; s_need[tid] = in_need; s_back[tid] = in_back;
+                s_len[tid] = (int32_t)len;
+                s_flag[tid] = ok;
+                __syncthreads();
+                const uint32_t stride = T * gridDim.x, first = blockIdx.x * T + tid;
+                const auto find = [&](const uint32_t *s, uint32_t i) {              // first request whose sum exceeds i
+                    uint32_t lo = 0, hi = T - 1;
+                    while (lo < hi) {
+                        const uint32_t m = (lo + hi) / 2;
+                        if (s[m] > i) hi = m; else lo = m + 1;
+                    }
+                    return lo;
+                };
+                const uint32_t rows_here = min(total_n, a.rows - min(rows0, a.rows));
+                for (uint32_t i = first; i < rows_here; i += stride) {
+                    const uint32_t f = find(s_end, i), fl = (uint32_t)s_len[f], at = fl + i - (f ? s_end[f - 1] : 0), j = at >> a.lbs;
+                    int32_t slot = -1, p = -1;
+                    if (s_flag[f]) {
+                        // a page of this step is read from the ring: its table entry is being written
+                        const uint32_t hv = (fl + bs - 1) >> a.lbs;
+                        const int32_t page = j < hv ? a.table[(uint64_t)(b0 + f) * a.ld + j] : a.pool[ring(need0 + (f ? s_need[f - 1] : 0) + j - hv)];
+                        p = (int32_t)at;
+                        if ((uint32_t)page < a.pages) slot = (int32_t)(((uint32_t)page << a.lbs) + (at & (bs - 1)));
+                    }
+                    a.slots[rows0 + i] = slot;
+                    a.pos[rows0 + i] = p;
                 }
-                a.slots[rows0 + i] = slot;
-                a.pos[rows0 + i] = p;
+                for (uint32_t i = first; i < total_need; i += stride) {
+                    const uint32_t f = find(s_need, i);
+                    if (!s_flag[f]) continue;
+                    const uint32_t j = i - (f ? s_need[f - 1] : 0), hv = ((uint32_t)s_len[f] + bs - 1) >> a.lbs;
+                    a.table[(uint64_t)(b0 + f) * a.ld + hv + j] = a.pool[ring(need0 + i)];
+                }
+                for (uint32_t i = first; i < total_back; i += stride) {
+                    const uint32_t f = find(s_back, i), j = i - (f ? s_back[f - 1] : 0);
+                    a.pool[ring(count + back0 + i)] = a.table[(uint64_t)(b0 + f) * a.ld + j];
+                }
             }
-            __syncthreads();
         }
-        rows0 += total_n; need0 += total_np >> 32; back0 += (uint32_t)total_np;
+        if (a.commit && blockIdx.x == 0 && b < a.B) a.lens_out[b] = ok ? (int32_t)(len + n) : ad < 0 ? 0 : raw;
+        rows0 += total_n; need0 += total_need; back0 += total_back;
+        if (b0 + T < a.B) __syncthreads();                           // the next chunk's sums
     }
-    if (a.fill) {
-        for (int64_t i = rows0 + (int64_t)blockIdx.x * T + tid; i < (int64_t)a.rows; i += (int64_t)T * gridDim.x) {
+    if (a.fill)
+        for (uint64_t i = (uint64_t)rows0 + blockIdx.x * T + tid; i < a.rows; i += T * gridDim.x) {
             a.slots[i] = -1;
             a.pos[i] = -1;
         }
-        if (a.B == 0 && blockIdx.x == 0 && tid == 0) a.row_start[0] = 0;
-    }
     __syncthreads();
-    if (a.commit && tid == 0) {
-        const int64_t left = count - s_used + back0;
-        a.state_out[0] = (int32_t)((h0 + (uint64_t)s_used) % a.pages);
-        a.state_out[1] = (int32_t)min(left, (int64_t)a.pages);
-        a.state_out[2] = s_refused;
+    if (a.commit && blockIdx.x == 0 && tid == 0) {
+        a.state_out[0] = (int32_t)ring(s_used);
+        a.state_out[1] = (int32_t)min((uint64_t)count - s_used + back0, (uint64_t)a.pages);
+        a.state_out[2] = (int32_t)s_refused;
     }
 }
 
@@ -364,15 +366,21 @@ int sh_kv_slots(uint64_t table, uint32_t ld, uint64_t lens, uint64_t lens_out, u
                (int32_t *)state_out, (int32_t *)pool, (int32_t *)row_start, (int32_t *)slots, (int32_t *)pos, (int32_t *)kv_len,
                B, bs == 16 ? 4u : bs == 32 ? 5u : 6u, pages, rows, 1, 1};
     const hipStream_t st = sh_stream();
-    const uint32_t groups = rows <= 4096 ? 1u : min(sh_cdiv(rows, 1024), 256u);
-    if (groups == 1) {
+    // One workgroup reads everything before it writes lengths and state in place; several do not, so these are then written by
+    // a launch of their own unless they go elsewhere.
+    if (rows <= 2048 && B <= 256) {
+        hipLaunchKernelGGL(k_kv_slots<256>, dim3(1), dim3(256), 0, st, a);
+    } else if (rows <= 4096) {
         hipLaunchKernelGGL(k_kv_slots<1024>, dim3(1), dim3(1024), 0, st, a);
-        return sh_launch_ok("sh_kv_slots") ? 0 : SH_EHIP;
+    } else {
+        const auto meet = [](uint64_t x, uint64_t y, uint64_t n) { return x < y + n && y < x + n; };
+        const uint32_t groups = min(sh_cdiv(rows, 1024), 256u);
+        const bool apart = !meet(lens, lens_out, (uint64_t)B * 4) && !meet(state, state_out, 12);
+        a.commit = apart;
+        hipLaunchKernelGGL(k_kv_slots<1024>, dim3(groups), dim3(1024), 0, st, a);
+        a.commit = 1; a.fill = 0;
+        if (!apart) hipLaunchKernelGGL(k_kv_slots<1024>, dim3(1), dim3(1024), 0, st, a);
     }
-    a.commit = 0;
-    hipLaunchKernelGGL(k_kv_slots<1024>, dim3(groups), dim3(1024), 0, st, a);
-    a.commit = 1; a.fill = 0;
-    hipLaunchKernelGGL(k_kv_slots<1024>, dim3(1), dim3(1024), 0, st, a);
     return sh_launch_ok("sh_kv_slots") ? 0 : SH_EHIP;
 }
 
