@@ -15,6 +15,7 @@
 // met so far to 2^14 (smaller ones keep their precision until 2^-28 of it); the accumulators are brought along where cn changes.
 #include "sh_kv.h"
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -31,7 +32,7 @@ struct AttnArgs {
     uint16_t *o;
     const int32_t *table, *kv_len, *row_start;
     uint64_t ldq, ldo;
-    uint32_t ld, B, rows, max_q, grp, prow, window, groups, wide, whole;
+    uint32_t ld, B, rows, max_q, grp, prow, window, groups, wide, whole, once;
     float sc;                              // scale x log2 e
     float *part, *ml;                      // partials [groups][2][prow][dh], their (max, sum) [groups][2][prow][2]
     ChunkUnit *unit;                       // [2 CUT]
@@ -91,6 +92,16 @@ __device__ __forceinline__ uint4 keep_bytes(uint4 v, int lo, int hi) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+template <bool ONCE>                        // ONCE: not kept in the caches
+__device__ __forceinline__ uint4 ld_codes(const uint8_t *p) {
+    if constexpr (ONCE) {
+        const sh_u4v q = __builtin_nontemporal_load((const sh_u4v *)p);
+        return make_uint4(q.x, q.y, q.z, q.w);
+    } else {
+        return *(const uint4 *)p;
+    }
+}
+
 // Four consecutive outputs of a row.
 __device__ __forceinline__ void store4(uint16_t *p, float a, float b, float c, float d) {
     const sh_h2 x = {(_Float16)a, (_Float16)b}, y = {(_Float16)c, (_Float16)d};
@@ -122,9 +133,10 @@ __device__ __forceinline__ Seq lane_seq(const Seq &s, uint32_t b) {
 // (`wide`); MANY: more, the lengths are read in rounds. What runs once is kept short: its instructions come from memory, not the
 // instruction cache, and cost more than the work (with 64-bit divisions and unrolled joins, 27 KB against 12: 64 requests of 300 to 500 keys 20.3 us
 // against 16.6).
-template <int DP, bool FP8, bool FULL, int NW, bool MANY>
+// DH: the head's width, or 0: any up to DP.
+template <int DP, int DH, bool FP8, int NW, bool MANY>
 __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
-    constexpr int NP = DP / 64, MT = DP / 16;
+    constexpr int NP = DP / 64, MT = (DH ? DH : DP) / 16;
     extern __shared__ float s_o[];                                  // [2 NW][prow][DP]
     __shared__ float s_ml[2 * NW][QT][2];
     __shared__ uint32_t s_seg[2 * NW][9];                           // request (-1: none), item, first tile, end tile, tiles; first row tile row, rows, head, first row
@@ -132,7 +144,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     __shared__ Seq s_seq[MANY ? 1 : 64 * NW];
     const KvCache &c = a.c;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
-    const uint32_t dh = FULL ? DP : c.dh, wg = blockIdx.x;
+    const uint32_t dh = DH ? DH : c.dh, wg = blockIdx.x;
     const auto uni = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
     const auto at_lane = [](uint32_t v, uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
 
@@ -231,10 +243,13 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         item = uni((t - base) / s.nt);
         j0 = uni(t - base - item * s.nt);
     }
+    // Codes that the Infinity Cache (256 MB) will not hold until the next call are read without allocating (120 MB and up here, one row tile): 48 requests
+    // of up to 16384 keys, 311 MB, 72.6 -> 68.0 us; what it holds would be lost by that: 8 requests of 1000 keys 13.0 -> 14.5 us.
+    const bool stream = a.once && T * (uint64_t)(2 * KT * dh) >= (120u << 20);
     const uint32_t kg = m >> 2, kr0 = m & 3;
     uint32_t kcol[NP];                                              // columns past the head's width: read as its first ones, against zeros of Q
 #pragma unroll
-    for (int p = 0; p < NP; ++p) kcol[p] = FULL || 64 * p + 16 * g < dh ? 64 * p + 16 * g : 0;
+    for (int p = 0; p < NP; ++p) kcol[p] = 64 * p + 16 * g < dh ? 64 * p + 16 * g : 0;
     while (t < t1) {
         const uint32_t h = item / s.nqt, qt = item - h * s.nqt;
         const uint32_t j1 = min(s.nt, j0 + (t1 - t));
@@ -254,22 +269,22 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         float ksc = 0.f, vsc = 0.f;
         uint32_t kp = 0, vp = 0;
         bool bad = false;
-        const auto load_k = [&](uint32_t j) {
+        const auto load_k = [&](auto once, uint32_t j) {
             const uint32_t kt = (s.ft + j) * KT + 16 * kg, pk = kp < c.pages ? kp : 0, pv = vp < c.pages ? vp : 0;
             const uint8_t *kb = c.k + pk * c.pgk + hoff + ((kt & (c.bs - 1)) + kr0) * dh;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int p = 0; p < NP; ++p) kr[q][p] = *(const uint4 *)(kb + 4 * q * dh + kcol[p]);
+                for (int p = 0; p < NP; ++p) kr[q][p] = ld_codes<decltype(once)::value>(kb + 4 * q * dh + kcol[p]);
             ksc = c.ks[(uint64_t)pv * c.pgs + h];
             vsc = c.vs[(uint64_t)pv * c.pgs + h];
         };
-        const auto load_v = [&](uint32_t j, uint32_t page) {
+        const auto load_v = [&](auto once, uint32_t j, uint32_t page) {
             const uint32_t vt = (s.ft + j) * KT + 16 * g, pv = page < c.pages ? page : 0;
             const uint8_t *vb = c.v + pv * c.pgv + hoff + m * c.bs + (vt & (c.bs - 1));
 #pragma unroll
             for (int i = 0; i < MT; ++i)
-                if (FULL || 16u * i < dh) vr[i] = *(const uint4 *)(vb + 16 * i * c.bs);
+                if (DH || 16u * i < dh) vr[i] = ld_codes<decltype(once)::value>(vb + 16 * i * c.bs);
         };
         uint32_t vpc = 0;
         if (ja < jb) { kp = page_at(ja, 16 * kg); vp = page_at(ja, 16 * g); }
@@ -279,7 +294,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             uint4 x = make_uint4(0, 0, 0, 0), y = x;
-            if (r < nrow && (FULL || 64 * p + 16 * g < dh)) { x = sh_ld16_any(qp + 64 * p + 16 * g); y = sh_ld16_any(qp + 64 * p + 16 * g + 8); }
+            if (r < nrow && 64 * p + 16 * g < dh) { x = sh_ld16_any(qp + 64 * p + 16 * g); y = sh_ld16_any(qp + 64 * p + 16 * g + 8); }
             qf[2 * p] = __builtin_bit_cast(sh_h8, x);
             qf[2 * p + 1] = __builtin_bit_cast(sh_h8, y);
         }
@@ -287,85 +302,89 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) oa[i] = sh_f4v{0.f, 0.f, 0.f, 0.f};
         float mx = -1e30f, l = 0.f, cn = 0.f;
-        if (ja < jb) {
-            const uint32_t kn = page_at(ja + 1, 16 * kg), vn = page_at(ja + 1, 16 * g);
-            vpc = vp;
-            load_k(ja);
-            load_v(ja, vpc);
-            kp = kn;
-            vp = vn;
-        }
-        for (uint32_t j = ja; j < jb; ++j) {
-            const uint32_t k0 = (s.ft + j) * KT, vt = k0 + 16 * g;
-            bad = vpc >= c.pages;
-            sh_f4v sa[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                sa[q] = sh_f4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    sa[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(kr[q][p].x, kr[q][p].y), qf[2 * p], sa[q], 0, 0, 0);
-                    sa[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(kr[q][p].z, kr[q][p].w), qf[2 * p + 1], sa[q], 0, 0, 0);
-                }
-            }
-            float x[16], vs = vsc;
-            const float ks = fmaxf(ksc * a.sc, 1e-37f);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = sa[i >> 2][i & 3];
-            // the pages after the next tile's first (loads end in order), then its keys
-            const uint32_t vcur = vp;
-            if (j + 1 < jb) {
-                const uint32_t kn = page_at(j + 2, 16 * kg), vn = page_at(j + 2, 16 * g);
-                load_k(j + 1);
+        const auto walk = [&](auto once) {
+            if (ja < jb) {
+                const uint32_t kn = page_at(ja + 1, 16 * kg), vn = page_at(ja + 1, 16 * g);
+                vpc = vp;
+                load_k(once, ja);
+                load_v(once, ja, vpc);
                 kp = kn;
                 vp = vn;
             }
-            const bool edge = (int32_t)(k0 + KT - 1) > pmin || (a.window && (int32_t)k0 < pmax - (int32_t)a.window + 1) || __any(bad);
-            if (edge) {
-                const int32_t at = (int32_t)vt, from = a.window ? max(pos, 0) - (int32_t)a.window + 1 : 0;
+            for (uint32_t j = ja; j < jb; ++j) {
+                const uint32_t k0 = (s.ft + j) * KT, vt = k0 + 16 * g;
+                bad = vpc >= c.pages;
+                sh_f4v sa[4];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = !bad && at + i <= pos && at + i >= from ? x[i] : -INFINITY;
-                // what no row sees may hold anything: its codes and scale must not meet a probability of 0
-                const int lo = bad ? 16 : max(slo - at, 0), hi = max(pmax + 1 - at, 0);
-                if (lo >= min(hi, 16)) vs = 0.f;
+                for (int q = 0; q < 4; ++q) {
+                    sa[q] = sh_f4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < MT; ++i) vr[i] = keep_bytes(vr[i], lo, hi);
-            }
-            float tm = x[0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) tm = fmaxf(tm, x[i]);
-            tm = max_xor16_32(tm * ks);                             // (a lane's scores have one scale)
-            const float mn = fmaxf(mx, tm), vm = max_xor16_32(vs);
-            float cs = cn;
-            if (!(vm * cn <= 16384.f) || cn == 0.f) cs = __builtin_amdgcn_ldexpf(1.f, 14 - (vm > 1e-30f ? __builtin_amdgcn_frexp_expf(vm) : -99));
-            if (__any(mn > mx) || cs != cn) {
-                const float al = sh_fast_exp2(mx - mn), be = al * (cn == 0.f ? 0.f : cs / cn);
-                l *= al;
-#pragma unroll
-                for (int i = 0; i < MT; ++i) oa[i] *= be;
-                mx = mn;
-                cn = cs;
-            }
-            // probability and weight in one exponential: 2^(score - maximum + log2 w), the sum taken back from it
-            const float w = fmaxf(vs * cn, 1e-30f), z = __builtin_amdgcn_logf(w) - mx;
-            float sum = 0.f;
-            sh_h8 pf[2];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float e = sh_fast_exp2(fmaf(x[i], ks, z));
-                sum += e;
-                pf[i >> 3][i & 7] = (_Float16)e;
-            }
-            l = fmaf(sum, sh_fast_rcp(w), l);
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-                if (FULL || 16u * i < dh) {
-                    oa[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(vr[i].x, vr[i].y), pf[0], oa[i], 0, 0, 0);
-                    oa[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(vr[i].z, vr[i].w), pf[1], oa[i], 0, 0, 0);
+                    for (int p = 0; p < NP; ++p) {
+                        sa[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(kr[q][p].x, kr[q][p].y), qf[2 * p], sa[q], 0, 0, 0);
+                        sa[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(kr[q][p].z, kr[q][p].w), qf[2 * p + 1], sa[q], 0, 0, 0);
+                    }
                 }
-            vpc = vcur;
-            if (j + 1 < jb) load_v(j + 1, vpc);
-        }
+                float x[16], vs = vsc;
+                const float ks = fmaxf(ksc * a.sc, 1e-37f);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = sa[i >> 2][i & 3];
+                // the pages after the next tile's first (loads end in order), then its keys
+                const uint32_t vcur = vp;
+                if (j + 1 < jb) {
+                    const uint32_t kn = page_at(j + 2, 16 * kg), vn = page_at(j + 2, 16 * g);
+                    load_k(once, j + 1);
+                    kp = kn;
+                    vp = vn;
+                }
+                const bool edge = (int32_t)(k0 + KT - 1) > pmin || (a.window && (int32_t)k0 < pmax - (int32_t)a.window + 1) || __any(bad);
+                if (edge) {
+                    const int32_t at = (int32_t)vt, from = a.window ? max(pos, 0) - (int32_t)a.window + 1 : 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = !bad && at + i <= pos && at + i >= from ? x[i] : -INFINITY;
+                    // what no row sees may hold anything: its codes and scale must not meet a probability of 0
+                    const int lo = bad ? 16 : max(slo - at, 0), hi = max(pmax + 1 - at, 0);
+                    if (lo >= min(hi, 16)) vs = 0.f;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) vr[i] = keep_bytes(vr[i], lo, hi);
+                }
+                float tm = x[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) tm = fmaxf(tm, x[i]);
+                tm = max_xor16_32(tm * ks);                             // (a lane's scores have one scale)
+                const float mn = fmaxf(mx, tm), vm = max_xor16_32(vs);
+                float cs = cn;
+                if (!(vm * cn <= 16384.f) || cn == 0.f) cs = __builtin_amdgcn_ldexpf(1.f, 14 - (vm > 1e-30f ? __builtin_amdgcn_frexp_expf(vm) : -99));
+                if (__any(mn > mx) || cs != cn) {
+                    const float al = sh_fast_exp2(mx - mn), be = al * (cn == 0.f ? 0.f : cs / cn);
+                    l *= al;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) oa[i] *= be;
+                    mx = mn;
+                    cn = cs;
+                }
+                // probability and weight in one exponential: 2^(score - maximum + log2 w), the sum taken back from it
+                const float w = fmaxf(vs * cn, 1e-30f), z = __builtin_amdgcn_logf(w) - mx;
+                float sum = 0.f;
+                sh_h8 pf[2];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = sh_fast_exp2(fmaf(x[i], ks, z));
+                    sum += e;
+                    pf[i >> 3][i & 7] = (_Float16)e;
+                }
+                l = fmaf(sum, sh_fast_rcp(w), l);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    if (DH || 16u * i < dh) {
+                        oa[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(vr[i].x, vr[i].y), pf[0], oa[i], 0, 0, 0);
+                        oa[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_half8<FP8>(vr[i].z, vr[i].w), pf[1], oa[i], 0, 0, 0);
+                    }
+                vpc = vcur;
+                if (j + 1 < jb) load_v(once, j + 1, vpc);
+            }
+        };
+        if constexpr (DH != 0) { if (stream) walk(std::true_type{}); else walk(std::false_type{}); }
+        else walk(std::false_type{});
         l = sum_xor16_32(l);
         const float ic = cn > 0.f ? 1.f / cn : 0.f;
         if (j0 == 0 && j1 == s.nt) {
@@ -373,13 +392,13 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
             if (r < nrow)
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    if (FULL || 16u * i < dh) store4(op + 16 * i + 4 * g, oa[i][0] * f, oa[i][1] * f, oa[i][2] * f, oa[i][3] * f);
+                    if (DH || 16u * i < dh) store4(op + 16 * i + 4 * g, oa[i][0] * f, oa[i][1] * f, oa[i][2] * f, oa[i][3] * f);
         } else {
             const uint32_t sg = 2 * wave + (j0 ? 0 : 1);
             if (m < a.prow) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    if (FULL || 16u * i < dh) *(sh_f4v *)&s_o[(sg * a.prow + m) * DP + 16 * i + 4 * g] = oa[i] * ic;
+                    if (DH || 16u * i < dh) *(sh_f4v *)&s_o[(sg * a.prow + m) * DP + 16 * i + 4 * g] = oa[i] * ic;
                 if (g == 0) { s_ml[sg][m][0] = mx; s_ml[sg][m][1] = l; }
             }
             if (lane == 0) {
@@ -494,12 +513,12 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
 // the scores of keys 16 q + 8 hi + 0 .. 7 of row n, which is the second product's operand.
 // Bound by the vector pipe: for 64 keys by 32 rows a wave issues 32 matrix instructions (1024 cycles of their pipe) beside the
 // scores' multiply-add, maximum, exponential (four issues each), sum, weight and conversion (~1100 cycles) and 80 to convert codes.
-// The keys of an item are cut into parts of C tiles, C a 512th of all tiles (and at least 8): one long request among short ones, or a
+// The keys of an item are cut into parts of C tiles, C a 768th of all tiles (and at least 8): one long request among short ones, or a
 // few rows over a long context, then keep every CU busy. Units are dealt out by the hardware, the request's last row tiles first
-// (they see most). A request that is cut has more than C tiles, so cut units number at most 2 T / C <= 1024: their parts go to as many places
+// (they see most). A request that is cut has more than C tiles, so cut units number at most 2 T / C <= 1536: their parts go to as many places
 // of `part`, which k_kv_chunk_join adds up.
 constexpr uint32_t CT = 128;               // rows of a unit
-constexpr uint32_t CUT = 512;              // units that share the whole evenly: two workgroups a CU
+constexpr uint32_t CUT = 768;              // units that share the whole evenly: three workgroups a CU, two of them at a time
 constexpr uint32_t CUT_MIN = 8;            // tiles of a part at least
 template <int DP, bool FP8>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a) {
@@ -782,34 +801,41 @@ __global__ __launch_bounds__(256) void k_kv_chunk_join(AttnArgs a) {
 
 uint32_t part_rows(uint32_t max_q, uint32_t grp) { return (uint32_t)min((uint64_t)QT, (uint64_t)max_q * grp); }
 
-template <int DP, bool FP8, bool FULL, int NW, bool MANY>
+template <int DP, int DH, bool FP8, int NW, bool MANY>
 bool launch_attn_many(const AttnArgs &a, hipStream_t st) {
     static bool set = false;
     const uint32_t lds = 2 * NW * a.prow * DP * 4;
     if (!set) {
-        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_kv_attn<DP, FP8, FULL, NW, MANY>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * NW * QT * DP * 4),
+        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_kv_attn<DP, DH, FP8, NW, MANY>, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * NW * QT * DP * 4),
                        "sh_attention_kv hipFuncSetAttribute")) return false;
         set = true;
     }
-    hipLaunchKernelGGL((k_kv_attn<DP, FP8, FULL, NW, MANY>), dim3(a.groups), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL((k_kv_attn<DP, DH, FP8, NW, MANY>), dim3(a.groups), dim3(64 * NW), lds, st, a);
     if (!a.whole) hipLaunchKernelGGL(k_kv_join<DP>, dim3(a.groups, a.prow), dim3(256), 0, st, a);
     return sh_launch_ok("sh_attention_kv");
 }
-template <int DP, bool FP8, bool FULL, int NW>
+template <int DP, int DH, bool FP8, int NW>
 bool launch_attn(AttnArgs a, uint32_t tiles, hipStream_t st) {
     a.groups = DP == 128 ? GROUPS / 2 : GROUPS;
-    if (a.B > 64 * NW) return launch_attn_many<DP, FP8, false, NW, true>(a, st);
+    if (a.B > 64 * NW) return launch_attn_many<DP, 0, FP8, NW, true>(a, st);
     a.wide = a.B > 64;
     a.whole = tiles <= WHOLE_TILES * NW;
-    return launch_attn_many<DP, FP8, FULL, NW, false>(a, st);
+    a.once = (uint64_t)a.max_q * a.grp <= QT;
+    return launch_attn_many<DP, DH, FP8, NW, false>(a, st);
 }
 template <bool FP8>
 bool launch_attn_width(const AttnArgs &a, uint32_t tiles, hipStream_t st) {
-    if (a.c.dh == 64) return launch_attn<64, FP8, true, 8>(a, tiles, st);
-    if (a.c.dh == 128) return launch_attn<128, FP8, true, 8>(a, tiles, st);
-    if (a.c.dh < 64) return launch_attn<64, FP8, false, 8>(a, tiles, st);
-    if (a.c.dh < 128) return launch_attn<128, FP8, false, 8>(a, tiles, st);
-    return launch_attn<256, FP8, false, 4>(a, tiles, st);
+    switch (a.c.dh) {
+    case 32: return launch_attn<64, 32, FP8, 8>(a, tiles, st);
+    case 64: return launch_attn<64, 64, FP8, 8>(a, tiles, st);
+    case 80: return launch_attn<128, 80, FP8, 8>(a, tiles, st);
+    case 96: return launch_attn<128, 96, FP8, 8>(a, tiles, st);
+    case 128: return launch_attn<128, 128, FP8, 8>(a, tiles, st);
+    case 256: return launch_attn<256, 256, FP8, 4>(a, tiles, st);
+    }
+    if (a.c.dh < 64) return launch_attn<64, 0, FP8, 8>(a, tiles, st);
+    if (a.c.dh < 128) return launch_attn<128, 0, FP8, 8>(a, tiles, st);
+    return launch_attn<256, 0, FP8, 4>(a, tiles, st);
 }
 
 template <bool FP8>
@@ -821,8 +847,9 @@ bool launch_chunk(const AttnArgs &a, uint32_t units, hipStream_t st) {
     return sh_launch_ok("sh_attention_kv");
 }
 
-// More rows a request than CHUNK_ROWS: the kernel that shares converted keys between the rows of a workgroup.
-constexpr uint32_t CHUNK_ROWS = 32;
+// More rows a request than CHUNK_ROWS: the kernel that shares converted keys between the rows of a workgroup. 16 requests of up to 8000
+// keys, 32 heads over 8, rows by 16 (the other kernel) against by 128: 20 rows 45 against 70 us, 32 rows 47 against 74, 64 rows 77 against 79.
+constexpr uint32_t CHUNK_ROWS = 64;
 bool chunked(uint32_t max_q, uint32_t grp) { return (uint64_t)max_q * grp > CHUNK_ROWS; }
 
 }  // namespace
