@@ -176,16 +176,18 @@ struct AppendArgs {
     const uint16_t *k, *v;
     uint64_t ldk, ldv;
     const int32_t *slots;
-    uint32_t rows, rg;
-    ShDiv dch;                             // by dh / 8
+    uint32_t rows, rg, row0;
+    ShDiv dch, dheads;                     // by dh / 8, by 2 hkv
 };
 
-// |x| of a pair of halves as integers (monotone), NaN as 0, infinity as 65504.
-__device__ __forceinline__ uint32_t abs_bits(uint32_t h) {
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ us2 bits2(uint32_t w) { return __builtin_bit_cast(us2, w & 0x7FFF7FFFu); }     // a pair of halves without their signs
+// NaN as 0, infinity as the largest half.
+__device__ __forceinline__ uint32_t clean1(uint32_t h) {
     const uint32_t a = h & 0x7FFFu;
-    return a > 0x7C00u ? 0u : min(a, 0x7BFFu);
+    return a > 0x7C00u ? 0u : min(a, 0x7BFFu) | (h & 0x8000u);
 }
-__device__ __forceinline__ float clean(uint16_t h) { return sh_dev_h2f((uint16_t)(abs_bits(h) | (h & 0x8000u))); }
+__device__ __forceinline__ uint32_t clean2(uint32_t w) { return clean1(w & 0xFFFFu) | clean1(w >> 16) << 16; }
 
 // The smallest power of two s >= 2^-32 with amax <= s Q, Q = 127 or 448: amax = f 2^e with f in [0.5, 1), Q = q 2^x likewise.
 template <bool FP8>
@@ -226,7 +228,8 @@ template <bool FP8, int NT>
 __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
     __shared__ uint32_t s_top[NT / 64];
     const KvCache &c = a.c;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, r0 = blockIdx.x * a.rg, h = blockIdx.y, isv = blockIdx.z;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, gr = sh_div(blockIdx.x, a.dheads), hv = blockIdx.x - gr * (2 * c.hkv), r0 = a.row0 + gr * a.rg;
+    const uint32_t isv = hv >= c.hkv, h = isv ? hv - c.hkv : hv;
     const uint32_t cap = c.pages << c.lbs, dh = c.dh, nch = dh / 8;
     // the first row of a page's run: it begins a page, or the row before does not precede it. Lane i: row r0 + i
     const uint32_t rl = r0 + lane;
@@ -249,7 +252,6 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
         const float was = off ? *sp : 0.f;
         const uint32_t blk0 = off / 4, items = ((end + 3) / 4 - blk0) * nch;
         uint4 x[4];
-        uint32_t top = 0;
         const uint32_t bl = sh_div(tid, a.dch), ch = tid - bl * nch, t0 = 4 * (blk0 + bl);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -257,20 +259,28 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
             x[j] = make_uint4(0, 0, 0, 0);
             if (tid < items && t >= off && t < end) x[j] = sh_ld16_any(src + (uint64_t)(t - off) * ld + 8 * ch);
         }
+        // the largest |x| as an integer (halves without their sign are ordered like their bits); only if a NaN or an infinity is
+        // among them are these put right, and it is taken again
+        uint32_t top;
+        for (;;) {
+            us2 t = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+            for (int j = 0; j < 4; ++j) {
+                t = __builtin_elementwise_max(t, __builtin_elementwise_max(bits2(x[j].x), bits2(x[j].y)));
+                t = __builtin_elementwise_max(t, __builtin_elementwise_max(bits2(x[j].z), bits2(x[j].w)));
+            }
+            top = (uint32_t)sh_wave_max((float)max(t.x, t.y));      // (exact)
+            if constexpr (NT > 64) {
+                __syncthreads();                                    // the last maxima are read
+                if (lane == 0) s_top[tid / 64] = top;
+                __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, max(abs_bits(w[e] & 0xFFFFu), abs_bits(w[e] >> 16)));
-        }
+                for (int i = 0; i < NT / 64; ++i) top = max(top, s_top[i]);
+            }
+            top = __builtin_amdgcn_readfirstlane(top);
+            if (top < 0x7C00u) break;
 #pragma unroll
-        for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        if constexpr (NT > 64) {
-            __syncthreads();                                        // the last page's maxima are read
-            if (lane == 0) s_top[tid / 64] = top;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < NT / 64; ++i) top = max(top, s_top[i]);
+            for (int j = 0; j < 4; ++j) x[j] = make_uint4(clean2(x[j].x), clean2(x[j].y), clean2(x[j].z), clean2(x[j].w));
         }
         const float s = fmaxf(was, pow2_scale<FP8>(sh_dev_h2f((uint16_t)top)));
         if (off && s != was) {                                      // the page's older tokens: whole words, and the bytes beside the new ones
@@ -289,8 +299,7 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
                 }
             }
         }
-        // x / s: the reciprocal of a power of two is exact (only a caller's own scales are not one)
-        const bool p2 = (__float_as_uint(s) & 0x7FFFFFu) == 0;
+        const bool p2 = !(__builtin_amdgcn_readfirstlane(__float_as_uint(s)) & 0x7FFFFFu);      // (only a caller's own scales are not)
         const float inv = 1.f / s;
         if (tid < items) {
             float v[4][8];
@@ -298,14 +307,14 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
             for (int j = 0; j < 4; ++j) {
                 const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = clean((uint16_t)(w[e / 2] >> (16 * (e & 1))));
+                for (int e = 0; e < 8; ++e) v[j][e] = sh_dev_h2f((uint16_t)(w[e / 2] >> (16 * (e & 1))));
             }
-            if (p2) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j / 8][j % 8] *= inv;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j / 8][j % 8] /= s;
+            for (int j = 0; j < 32; ++j) {
+                // the product, and what it lacks for the correctly rounded quotient (Markstein, "Computation of elementary functions on
+                // the IBM RISC System/6000 processor", 1990): nothing where s is a power of two
+                const float f = v[j / 8][j % 8], q = f * inv;
+                v[j / 8][j % 8] = p2 ? q : fmaf(fmaf(-q, s, f), inv, q);
             }
             if (!isv) {
 #pragma unroll
@@ -332,14 +341,23 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
     }
 }
 
+// Workgroups with the heads fastest, keys then values: those that run at one time read whole rows and write whole pages.
+template <bool FP8, int NT>
+void launch_append_nt(AppendArgs a, hipStream_t st) {
+    const uint32_t heads = 2 * a.c.hkv, most = (1u << 31) / (heads * NT) * a.rg;            // (a launch has fewer than 2^32 threads)
+    a.dheads = sh_make_div(heads);
+    for (uint64_t r = 0; r < a.rows; r += most) {
+        a.row0 = (uint32_t)r;
+        hipLaunchKernelGGL((k_kv_append<FP8, NT>), dim3(sh_cdiv(min(a.rows - a.row0, most), a.rg) * heads), dim3(NT), 0, st, a);
+    }
+}
 template <bool FP8>
-void launch_append(AppendArgs &a, hipStream_t st) {
-    const dim3 grid(sh_cdiv(a.rows, a.rg), a.c.hkv, 2);
+void launch_append(const AppendArgs &a, hipStream_t st) {
     const uint32_t items = a.c.bs * a.c.dh / 32;
-    if (items <= 64) hipLaunchKernelGGL((k_kv_append<FP8, 64>), grid, dim3(64), 0, st, a);
-    else if (items <= 128) hipLaunchKernelGGL((k_kv_append<FP8, 128>), grid, dim3(128), 0, st, a);
-    else if (items <= 256) hipLaunchKernelGGL((k_kv_append<FP8, 256>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_kv_append<FP8, 512>), grid, dim3(512), 0, st, a);
+    if (items <= 64) launch_append_nt<FP8, 64>(a, st);
+    else if (items <= 128) launch_append_nt<FP8, 128>(a, st);
+    else if (items <= 256) launch_append_nt<FP8, 256>(a, st);
+    else launch_append_nt<FP8, 512>(a, st);
 }
 
 }  // namespace

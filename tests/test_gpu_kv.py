@@ -203,6 +203,30 @@ def test_append_exact(lib, gpu, case, fmt):
 
 
 @pytest.mark.parametrize("fmt", [INT8, FP8])
+def test_append_to_scales_of_another_kind(lib, gpu, fmt):
+    """Pages whose scales are no powers of two: new codes are the correctly rounded quotients, and the scale stays where it suffices."""
+    rng = np.random.default_rng(37)
+    hkv, dh, bs, pages = 4, 64, 16, 40
+    c = Cache(rng, pages, hkv, dh, bs, fmt, values=True)
+    host = list(c.before())
+    host[2], host[3] = (rng.uniform(0.004, 0.2, (pages, hkv)).astype(np.float32) for _ in "kv")
+    c.dks.copy_(dev(host[2])); c.dvs.copy_(dev(host[3]))             # noqa: E702
+    c.sc = np.stack(host[2:])
+    slot = np.concatenate([p * bs + np.arange(int(rng.integers(1, bs)), bs) for p in rng.permutation(pages)]).astype(np.int32)
+    x = rng.standard_normal((2, len(slot), hkv * dh)).astype(np.float16)
+    X, S = to_dev(x), dev(slot)
+    want = R.append(*host, x[0], x[1], slot, fmt)
+    assert (want[2] == host[2]).any() and (want[2] != host[2]).any()
+    assert lib.sh_kv_append(C.byref(c.c), A(X), A(X, x[0].size), hkv * dh, hkv * dh, A(S), len(slot)) == 0
+    for name, g, w in zip(("k", "v", "ks", "vs"), c.now(), want):
+        if fmt == FP8 and g.dtype == np.uint8:
+            g, w = (np.where(t == 128, 0, t) for t in (g, w))
+        bad = g != w
+        # the quotient is rounded to fp32 before it is rounded to a code: a value next to a code's border may fall on it
+        assert bad.mean() <= 1e-4, (name, int(bad.sum()))
+
+
+@pytest.mark.parametrize("fmt", [INT8, FP8])
 def test_append_skips_slots_outside_the_cache(lib, gpu, fmt):
     rng = np.random.default_rng(3)
     c = Cache(rng, 3, 2, 32, 16, fmt, values=True)
