@@ -9,6 +9,7 @@
 // each (one row of 4096 x 14336: 10.7 us). The pairs are the k (0, 4) and (2, 6), and (1, 5) and (3, 7) 16 times as large: of
 // two steps' words the former make one operand, the latter another with a sum of its own, and x's are put into the same order.
 #include "sh_common.h"
+#include <algorithm>
 
 namespace {
 
@@ -91,7 +92,7 @@ template <int MT, int CW, int NW, int GS, int SU>
 __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
     constexpr uint32_t LC = 16 * CW + 1;
     constexpr int NG = SU / GS;
-    constexpr bool PX = MT == 1;                                    // x's next operands too
+    constexpr bool PX = MT * CW <= 4;                               // x's next operands too
     extern __shared__ float s_z[];                                  // [NW][rows][LC]
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const uint32_t col0 = blockIdx.x * 16 * CW, m0 = blockIdx.y * 16 * MT, nrow = min(a.M - m0, 16u * MT);
@@ -137,7 +138,10 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
         uint4 x[SU][MT];
 #pragma unroll
         for (int s = 0; s < SU; ++s)
-            if constexpr (PX) x[s][0] = o.x[s][0]; else load_x(u, s, x[s]);
+            if constexpr (PX) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) x[s][i] = o.x[s][i];
+            } else load_x(u, s, x[s]);
         const bool tail = (u + 1) * 4 * SU > oct;
         if (tail)
 #pragma unroll
@@ -189,10 +193,9 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        // (the products are of like size and may cancel: first against each other, then into the sum)
-                        float t = hi[i][j][e] * s20;
+                        float t = fmaf(xs[i][e], sz, acc[i][j][e]);
                         if constexpr (GS > 1) t = fmaf(lo[i][j][e], s24, t);
-                        acc[i][j][e] += fmaf(xs[i][e], sz, t);
+                        acc[i][j][e] = fmaf(hi[i][j][e], s20, t);
                     }
             }
         }
@@ -248,16 +251,20 @@ bool launch_w4(const W4Args &a, hipStream_t st) {
     hipLaunchKernelGGL((k_w4<MT, CW, NW, GS, SU>), dim3(sh_cdiv(a.N, 16 * CW), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), lds, st, a);
     return sh_launch_ok("sh_gemm_w4");
 }
-// The widest tile that still makes 192 workgroups of the 256 CUs: columns first (a word is converted once for every 16 rows of a
-// workgroup, x is read once for every 16 CW columns), then 32 rows.
+// The tile with the least rounds of workgroups over the 256 CUs times the time of one (a tile's registers allow one a CU): wider columns
+// convert a word once for every 16 rows and read x once for every 16 CW columns, narrower ones make more workgroups. The times are
+// those of a round at K = 4096 (1 x 64 columns 7.0 us, x 32 5.2, x 16 4.5; 32 rows x 64 columns 11.5). Measured, K = 8192: 50 rows,
+// 4096 columns (256 workgroups of 16 x 64) 15.3 us against 20.5 for 32 x 32; 4160 columns 24.0 in 32 x 64 against 27.1 in 16 x 64 (260).
 template <int GS, int SU>
 bool launch_w4_tile(const W4Args &a, hipStream_t st) {
-    const uint32_t mt = sh_cdiv(a.M, 16);
-    const auto fills = [&](uint32_t m, uint32_t c) { return (uint64_t)sh_cdiv(a.N, 16 * c) * sh_cdiv(mt, m) >= 192; };
-    if (a.N >= 4 && mt > 1 && fills(2, 4)) return launch_w4<2, 4, GS, SU>(a, st);
-    if (a.N >= 4 && fills(1, 4)) return launch_w4<1, 4, GS, SU>(a, st);
-    if (a.N >= 2 && fills(1, 2)) return launch_w4<1, 2, GS, SU>(a, st);
-    return launch_w4<1, 1, GS, SU>(a, st);
+    const uint64_t mt = sh_cdiv(a.M, 16);
+    const auto cost = [&](uint64_t m, uint32_t c, uint64_t t) { return a.N < c ? ~0ull : ((sh_cdiv(a.N, 16 * c) * ((mt + m - 1) / m) + 255) / 256) * t; };
+    const uint64_t c24 = mt > 1 ? cost(2, 4, 115) : ~0ull, c14 = cost(1, 4, 70), c12 = cost(1, 2, 52), c11 = cost(1, 1, 45);
+    const uint64_t best = std::min(std::min(c24, c14), std::min(c12, c11));
+    if (best == c11) return launch_w4<1, 1, GS, SU>(a, st);
+    if (best == c12) return launch_w4<1, 2, GS, SU>(a, st);
+    if (best == c14) return launch_w4<1, 4, GS, SU>(a, st);
+    return launch_w4<2, 4, GS, SU>(a, st);
 }
 
 // Units of 128 k keep the most words in flight (one row of 4096 x 14336, groups of 64: 10.9 us against 12.1 in units of 64); with

@@ -1,7 +1,7 @@
 // The 8-bit paged key / value cache: block tables and slots of a step (sh_kv_slots) and the write of new rows
 // (sh_kv_append). The attention over it is in sh_kv_attention.hip.
 #include "sh_kv.h"
-#include <math.h>
+#include <algorithm>
 
 int sh_kv_check(const char *name, const sh_kv_cache *c, KvCache *out) {
     if (!c || !c->k || !c->v || !c->ks || !c->vs) { sh_set_error(-1, "[%s] NULL cache or cache address", name); return -1; }
@@ -348,7 +348,7 @@ void launch_append_nt(AppendArgs a, hipStream_t st) {
     a.dheads = sh_make_div(heads);
     for (uint64_t r = 0; r < a.rows; r += most) {
         a.row0 = (uint32_t)r;
-        hipLaunchKernelGGL((k_kv_append<FP8, NT>), dim3(sh_cdiv(min(a.rows - a.row0, most), a.rg) * heads), dim3(NT), 0, st, a);
+        hipLaunchKernelGGL((k_kv_append<FP8, NT>), dim3(sh_cdiv(std::min(a.rows - a.row0, most), a.rg) * heads), dim3(NT), 0, st, a);
     }
 }
 template <bool FP8>
@@ -392,7 +392,7 @@ int sh_kv_slots(uint64_t table, uint32_t ld, uint64_t lens, uint64_t lens_out, u
         hipLaunchKernelGGL(k_kv_slots<1024>, dim3(1), dim3(1024), 0, st, a);
     } else {
         const auto meet = [](uint64_t x, uint64_t y, uint64_t n) { return x < y + n && y < x + n; };
-        const uint32_t groups = min(sh_cdiv(rows, 1024), 256u);
+        const uint32_t groups = std::min(sh_cdiv(rows, 1024), 256u);
         const bool apart = !meet(lens, lens_out, (uint64_t)B * 4) && !meet(state, state_out, 12);
         a.commit = apart;
         hipLaunchKernelGGL(k_kv_slots<1024>, dim3(groups), dim3(1024), 0, st, a);

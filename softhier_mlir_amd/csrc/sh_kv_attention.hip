@@ -14,7 +14,7 @@
 // could leave the range, so they are held as p x vs x cn, cn a power of two that brings the largest value scale
 // met so far to 2^14 (smaller ones keep their precision until 2^-28 of it); the accumulators are brought along where cn changes.
 #include "sh_kv.h"
-#include <math.h>
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -799,7 +799,7 @@ __global__ __launch_bounds__(256) void k_kv_chunk_join(AttnArgs a) {
     }
 }
 
-uint32_t part_rows(uint32_t max_q, uint32_t grp) { return (uint32_t)min((uint64_t)QT, (uint64_t)max_q * grp); }
+uint32_t part_rows(uint32_t max_q, uint32_t grp) { return (uint32_t)std::min<uint64_t>(QT, (uint64_t)max_q * grp); }
 
 template <int DP, int DH, bool FP8, int NW, bool MANY>
 bool launch_attn_many(const AttnArgs &a, hipStream_t st) {
@@ -858,7 +858,7 @@ extern "C" {
 
 uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t rows, uint32_t max_q, uint32_t H, uint32_t ld_table) {
     if (!c || !B || !rows || !max_q || !c->hkv || !H || !ld_table || !c->dh) return 0;
-    max_q = min(max_q, rows);
+    max_q = std::min(max_q, rows);
     if (chunked(max_q, H / c->hkv)) return 2 * CUT * ((uint64_t)CT * (c->dh + 2) * 4 + sizeof(ChunkUnit)) + 16;
     const uint64_t prow = part_rows(max_q, H / c->hkv);
     return (uint64_t)GROUPS * (2 * prow * (c->dh + 2) * 4 + 32);
@@ -885,7 +885,7 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
         return -1;
     }
     const uint32_t grp = H / c->hkv;
-    if ((uint64_t)min(max_q, rows) * grp >= (1ull << 31)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", max_q, H); return -1; }
+    if ((uint64_t)std::min(max_q, rows) * grp >= (1ull << 31)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", max_q, H); return -1; }
     if (!(scale > 0.f && scale <= 3.4e38f)) { sh_set_error(-1, "[sh_attention_kv] scale %g must be positive and finite", (double)scale); return -1; }
     const uint64_t need = sh_attention_kv_ws_bytes(c, B, rows, max_q, H, ld_table);
     if (!ws || ws % 16) { sh_set_error(-1, "[sh_attention_kv] ws must be a 16-byte aligned address"); return -1; }
@@ -896,7 +896,7 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     a.q = (const uint16_t *)q; a.o = (uint16_t *)o;
     a.table = (const int32_t *)table; a.kv_len = (const int32_t *)kv_len; a.row_start = (const int32_t *)row_start;
     a.ldq = ldq; a.ldo = ldo; a.ld = ld_table;
-    a.B = B; a.rows = rows; a.max_q = min(max_q, rows); a.grp = grp; a.prow = part_rows(a.max_q, grp);
+    a.B = B; a.rows = rows; a.max_q = std::min(max_q, rows); a.grp = grp; a.prow = part_rows(a.max_q, grp);
     a.window = window < ld_table * c->bs ? window : 0;               // (one that no key falls out of is none)
     a.groups = GROUPS;
     a.sc = scale * 1.4426950408889634f;
@@ -904,7 +904,7 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     const hipStream_t st = sh_stream();
     if (chunked(a.max_q, grp)) {
         // units: the row tiles, each request's last one short, and at most CUT parts more
-        const uint64_t tiles = min((uint64_t)B * (((uint64_t)a.max_q * grp + CT - 1) / CT), ((uint64_t)rows * grp + CT - 1) / CT + B);
+        const uint64_t tiles = std::min<uint64_t>((uint64_t)B * (((uint64_t)a.max_q * grp + CT - 1) / CT), ((uint64_t)rows * grp + CT - 1) / CT + B);
         if (tiles * c->hkv + CUT >= (1ull << 31)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", rows, H); return -1; }
         const uint32_t units = (uint32_t)(tiles * c->hkv) + CUT;
         a.unit = (ChunkUnit *)(ws + 16);
@@ -915,7 +915,7 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     a.part = (float *)(ws + GROUPS * 32);
     a.ml = a.part + (uint64_t)GROUPS * 2 * a.prow * c->dh;
     uint64_t tiles = ((uint64_t)ld_table * c->bs + KT - 1) / KT + 1;                     // an item's, at most
-    if (a.window) tiles = min(tiles, ((uint64_t)a.window + a.max_q) / KT + 2);
+    if (a.window) tiles = std::min<uint64_t>(tiles, ((uint64_t)a.window + a.max_q) / KT + 2);
     const uint64_t items = (uint64_t)c->hkv * (((uint64_t)a.max_q * grp + QT - 1) / QT);
     if (tiles * items >= (1ull << 32) / B) {                        // (tile counts of 32 bits)
         sh_set_error(-1, "[sh_attention_kv] %u requests of up to %llu tokens and %u heads", B, (unsigned long long)ld_table * c->bs, H);

@@ -398,6 +398,8 @@ def test_attention_max_q_and_rows_bound_what_is_written(lib, gpu):
     table = _table(rng, [100, 90], 16, 20)
     q = rng.standard_normal((60, 4 * 64)).astype(np.float16)
     _attend(lib, c, q, table, [100, 90], np.array([0, 40, 60]), 4, 0.125, max_q=7)
+    _attend(lib, c, q, table, [100, 90], np.array([0, 40, 60]), 4, 0.125, max_q=0xFFFFFFFF)
+    _attend(lib, c, q[:5], table, [100, 90], np.array([0, 3, 5]), 4, 0.125, max_q=0xFFFFFFFF, window=0xFFFFFFFF)
     import torch
     O = torch.full((60, 256), 7.0, dtype=torch.float16, device="cuda")
     Q, T, Ln, Rs = to_dev(q), dev(table), dev(np.array([100, 90], np.int32)), dev(np.array([0, 40, 60], np.int32))

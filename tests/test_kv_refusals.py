@@ -68,6 +68,8 @@ def test_attention_workspace_grows_with_the_rows_and_heads(lib):
     n = [lib.sh_attention_kv_ws_bytes(c, 64, 64, q, h, 64) for q, h in ((1, 2), (1, 8), (4, 8), (100, 8))]
     assert n[0] < n[1] < n[2] <= n[3]
     assert lib.sh_attention_kv_ws_bytes(None, 1, 1, 1, 2, 1) == 0
+    for rows in (1, 64, 5000):                                              # no bound on a request's rows: theirs
+        assert lib.sh_attention_kv_ws_bytes(c, 64, rows, 0xFFFFFFFF, 8, 64) == lib.sh_attention_kv_ws_bytes(c, 64, rows, rows, 8, 64)
 
 
 def test_slots_refusals(lib):
