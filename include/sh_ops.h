@@ -372,8 +372,10 @@ uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t row
  * (uint32, leading dim ldw), bits 4 j .. 4 j + 3 of word (i, n) the code of k = 8 i + j. scale: fp16 [ceil(K / group)][N],
  * zero: one byte (0 .. 15) each, same shape and leading dim lds; zero = 0: 8 throughout. K a multiple of 8, group a multiple of 32
  * (the last group may be short). epi: bias, act, residual as sh_gemm_ex (splits 0 or 1, no LayerNorm fold, no row
- * partials). fp32 sums, scales applied in fp32. Written for M up to 64; more rows read the weight again for every 64. A
- * row's bits do not depend on M or on the other rows. 0, -1 for bad arguments, SH_EHIP. */
+ * partials). fp32 sums, scales applied in fp32: z = sum over groups of scale (x . code - zero sum x), so a row with an infinity
+ * gives NaN. Written for M up to 64: the weight is read again (from cache) for every 16 or 32 rows. A row's bits do not depend on M
+ * or on the other rows. M <= 2^19, N <= 2^26. 0, -1 for bad arguments, SH_EHIP. softhier_mlir_amd/w4.py makes words, scales and zeros of
+ * an fp16 weight. */
 int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero, uint64_t z, uint32_t M, uint32_t N, uint32_t K, uint32_t group,
                uint32_t ldx, uint32_t ldw, uint32_t lds, uint32_t ldz, const sh_gemm_epi *epi);
 

@@ -427,14 +427,16 @@ def test_attention_scales_far_apart(lib, gpu, fmt):
     assert np.isfinite(o).all()
 
 
-def test_attention_many_requests(lib, gpu):
-    """More requests than a workgroup has threads, most without keys or rows."""
-    rng = np.random.default_rng(23)
-    B, bs, dh = 700, 16, 32
+@pytest.mark.parametrize("B,dh", [(65, 64), (300, 32), (512, 128), (700, 32), (256, 256), (257, 256), (600, 80)])
+@pytest.mark.parametrize("longest", [500, 5000])
+def test_attention_many_requests(lib, gpu, B, dh, longest):
+    """More requests than a wave has lanes, or a workgroup threads, most without keys or rows; items that are cut and that are not."""
+    rng = np.random.default_rng(B)
+    bs = 16
     L = np.where(rng.random(B) < 0.7, 0, rng.integers(1, 60, B))
-    L[299], L[699] = 500, 90
+    L[B // 3], L[B - 1] = longest, 90
     new = np.where(rng.random(B) < 0.5, 0, rng.integers(1, 4, B))
-    new[299] = new[699] = 2
+    new[B // 3] = new[B - 1] = 2
     start = np.concatenate([[0], np.cumsum(new)])
     pages = int(sum(-(-n // bs) for n in L)) + 1
     c = Cache(rng, pages, 1, dh, bs, INT8)

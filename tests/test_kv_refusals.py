@@ -87,7 +87,7 @@ def test_w4_refusals(lib):
     e = lambda **kw: C.byref(shops.epi(**kw))  # noqa: E731
     good = [ONE, ONE, ONE, 0, ONE, 2, 64, 128, 32, 128, 64, 64, 64, None]
     bad = [(0, 0), (1, 0), (2, 0), (4, 0), (7, 0), (7, 100), (8, 0), (8, 16), (8, 48), (9, 127), (10, 63), (11, 63), (12, 63), (0, ONE + 1),
-           (1, ONE + 2), (2, ONE + 1), (4, ONE + 1), (5, 1 << 22), (13, e(act=2)), (13, e(bias=ONE, bias_fmt=2)), (13, e(bias=ONE + 1)),
+           (1, ONE + 2), (2, ONE + 1), (4, ONE + 1), (5, (1 << 19) + 1), (13, e(act=2)), (13, e(bias=ONE, bias_fmt=2)), (13, e(bias=ONE + 1)),
            (13, e(bias=ONE + 2, bias_fmt=shops.SH_BIAS_FP32)), (13, e(residual=ONE, ldr=63)), (13, e(residual=ONE + 1, ldr=64)), (13, e(splits=2)),
            (13, e(ln_stats=ONE)), (13, e(ln_c=ONE)), (13, e(stats_out=ONE)), (13, e(ln_parts=4))]
     for i, v in bad:
