@@ -287,7 +287,7 @@ extern "C" int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero,
         return -1;
     }
     if ((x | scale | z) % 2 || w % 4) { sh_set_error(-1, "[sh_gemm_w4] words must be 4-byte aligned, halves 2-byte aligned"); return -1; }
-    if (M > (1u << 19) || N > (1u << 26)) {                         // (the grid's limits) sh_set_error(-1, "[sh_gemm_w4] M=%u N=%u too large", M, N); return -1; }
+    if (M > (1u << 19) || N > (1u << 26)) { sh_set_error(-1, "[sh_gemm_w4] M=%u N=%u too large", M, N); return -1; }
     if (epi) {
         if (epi->act > SH_ACT_GELU) { sh_set_error(-1, "[sh_gemm_w4] unknown act %u", epi->act); return -1; }
         if (epi->bias && (epi->bias_fmt > SH_BIAS_FP32 || epi->bias % (epi->bias_fmt == SH_BIAS_FP32 ? 4 : 2))) {
