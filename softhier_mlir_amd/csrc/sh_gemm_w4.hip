@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
         for (int k = 0; k < NG; ++k) {
             const uint64_t gi = (uint64_t)min((u * NG + k) / a.per, a.groups - 1) * a.lds + col;
             ld_scales<CW>(a.scale + gi, o.sc[k]);
-            o.zr[k] = a.zero ? ld_zeros<CW>(a.zero + gi) : 0x08080808u;
+            o.zr[k] = ld_zeros<CW>(a.zero ? a.zero + gi : (const uint8_t *)(a.scale + gi));       // (read either way: see below)
         }
     };
     const auto multiply = [&](uint32_t u, Ops &o) {
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
             }
 #pragma unroll
             for (int j = 0; j < CW; ++j) {
-                const float sc = o.sc[k][j], sz = -sc * (float)((o.zr[k] >> (8 * j)) & 15u), s24 = sc * 0x1p24f, s20 = sc * 0x1p20f;
+                const float sc = o.sc[k][j], sz = -sc * (a.zero ? (float)((o.zr[k] >> (8 * j)) & 15u) : 8.f), s24 = sc * 0x1p24f, s20 = sc * 0x1p20f;
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -200,17 +200,24 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
             }
         }
     };
+    // (The next loads are made without a condition, behind the last unit of it again: under one the compiler would wait for all of
+    // them before each product.)
     Ops o0, o1;
     uint32_t u = wave;
-    if (u < units) load(u, o0);
-    while (u < units) {
-        if (u + NW < units) load(u + NW, o1);
-        multiply(u, o0);
-        u += NW;
-        if (u >= units) break;
-        if (u + NW < units) load(u + NW, o0);
-        multiply(u, o1);
-        u += NW;
+    if (u < units) {
+        load(u, o0);
+        for (;;) {
+            uint32_t v = u + NW;
+            load(v < units ? v : u, o1);
+            multiply(u, o0);
+            u = v;
+            if (u >= units) break;
+            v = u + NW;
+            load(v < units ? v : u, o0);
+            multiply(u, o1);
+            u = v;
+            if (u >= units) break;
+        }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -238,9 +245,9 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
     }
 }
 
-template <int MT, int CW, int GS, int SU>
+template <int MT, int CW, int GS, int SU, uint32_t NW = 8>
 bool launch_w4(const W4Args &a, hipStream_t st) {
-    constexpr uint32_t NW = 8, most = NW * 16 * MT * (16 * CW + 1) * 4;
+    constexpr uint32_t most = NW * 16 * MT * (16 * CW + 1) * 4;
     static bool set = false;
     if (!set && most > 65536) {
         if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_w4<MT, CW, NW, GS, SU>, hipFuncAttributeMaxDynamicSharedMemorySize, most),
@@ -259,6 +266,9 @@ template <int GS, int SU>
 bool launch_w4_tile(const W4Args &a, hipStream_t st) {
     const uint64_t mt = sh_cdiv(a.M, 16);
     const auto cost = [&](uint64_t m, uint32_t c, uint64_t t) { return a.N < c ? ~0ull : ((sh_cdiv(a.N, 16 * c) * ((mt + m - 1) / m) + 255) / 256) * t; };
+    // A long chain of units over few columns: sixteen waves share it (by N and K alone, so that a row's bits do not depend on M). One
+    // row, groups of 64: 12248 x 700 14.0 us with eight, 10.6 with sixteen.
+    if (SU == 4 && a.K >= 2048 && a.N <= 2048) return launch_w4<1, 1, GS, SU, 16>(a, st);
     const uint64_t c24 = mt > 1 ? cost(2, 4, 115) : ~0ull, c14 = cost(1, 4, 70), c12 = cost(1, 2, 52), c11 = cost(1, 1, 45);
     const uint64_t best = std::min(std::min(c24, c14), std::min(c12, c11));
     if (best == c11) return launch_w4<1, 1, GS, SU>(a, st);
