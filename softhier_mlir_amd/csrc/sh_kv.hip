@@ -31,7 +31,7 @@ namespace {
 // one write for each new row, new page and returned page. Requests are scanned in chunks of the workgroup's threads. Where a chunk's
 // requests add a few rows each, a thread writes its own; else rows and pages are spread evenly over the threads of all
 // workgroups (a binary search in the chunk's sums finds a row's request), so one long prompt costs as much as many short requests.
-// Bound by latency: a launch, the lengths, then a page, then the writes.
+// Bound by latency: a launch, the lengths, then a page, then the writes (64 single tokens 4.6 us, 1024 requests with 44 thousand rows 7.0).
 struct SlotArgs {
     int32_t *table; uint32_t ld;
     const int32_t *lens, *add, *state;
@@ -223,7 +223,8 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
 // the other. A thread holds four tokens by eight columns of the page (one such item), the tokens at the page's own multiples of
 // four: four 16-byte loads; after the page's largest value is known, the codes of a key's eight columns are one 8-byte store a
 // token, those of a value's four tokens one 4-byte store a column (a page of values has its tokens consecutive). At most 64 x 256
-// values a page: 512 items. Bound by HBM: 2 bytes read and 1 written a value; written pages are whole lines in L2.
+// values a page: 512 items. Bound by HBM: 2 bytes read and 1 written a value; written pages are whole lines in L2 (17 thousand rows of 8 heads
+// of 64: 13.5 us, 3.9 TB/s; 64 single rows 4.8 us, one launch).
 template <bool FP8, int NT>
 __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
     __shared__ uint32_t s_top[NT / 64];

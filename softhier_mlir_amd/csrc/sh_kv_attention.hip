@@ -13,6 +13,9 @@
 // The scales of a page: the key's multiplies the scores of a lane (one page), the value's the probabilities. In fp16 p x vs
 // could leave the range, so they are held as p x vs x cn, cn a power of two that brings the largest value scale
 // met so far to 2^14 (smaller ones keep their precision until 2^-28 of it); the accumulators are brought along where cn changes.
+//
+// Single tokens are bound by HBM once the keys are many (two requests of 131 thousand keys, 516 MB: 89 us, 5.8 TB/s) and by latency
+// below (one request of 937 keys 8.8 us): the lengths, a page, its codes, the join, one after the other.
 #include "sh_kv.h"
 #include <algorithm>
 #include <type_traits>
@@ -513,8 +516,10 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
 // buffers, the codes after the next in flight. S^T and O^T on v_mfma_f32_32x32x16_f16. As above no operand moves between
 // lanes: row m of a score tile's A operand is key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that the lane (n, hi) gets
 // the scores of keys 16 q + 8 hi + 0 .. 7 of row n, which is the second product's operand.
-// Bound by the vector pipe: for 64 keys by 32 rows a wave issues 32 matrix instructions (1024 cycles of their pipe) beside the
-// scores' multiply-add, maximum, exponential (four issues each), sum, weight and conversion (~1100 cycles) and 80 to convert codes.
+// Bound by the vector pipe: for 64 keys by 32 rows a wave issues 32 matrix instructions (1024 cycles of their pipe) beside ~380 vector
+// issues (1520 cycles): a multiply-add, an exponential (four issues) and an addition a score, half a maximum and half a
+// conversion, and the codes of its share. Measured: 512 rows each of four requests of 8000 keys, 32 heads over 8, 395 us, 700 TFLOP/s; 4096
+// rows of one prompt 218 us, 630 TFLOP/s; LDS reads (32 KB a wave and tile) come next.
 // The keys of an item are cut into parts of C tiles, C a 768th of all tiles (and at least 8): one long request among short ones, or a
 // few rows over a long context, then keep every CU busy. Units are dealt out by the hardware, the request's last row tiles first
 // (they see most). A request that is cut has more than C tiles, so cut units number at most 2 T / C <= 1536: their parts go to as many places

@@ -195,6 +195,36 @@ def test_two_graphs_beside_each_other(lib, gpu):
             assert torch.equal(o, want)
 
 
+def test_first_call_under_capture(lib, gpu):
+    """A graph whose capture is the first call of its kernels (a head width nothing else here decodes with)."""
+    import torch
+    rng = np.random.default_rng(4)
+    la = Layer(13, B=3, H=4, hkv=2, dh=112, D=64, bs=32, ld=4, pages=12, rows=3, fmt=shops.SH_INT8)
+    la.gc[0].copy_(torch.from_numpy(rng.integers(0, 256, la.gc[0].shape).astype(np.uint8)))
+    la.gc[1].copy_(torch.from_numpy(rng.integers(0, 256, la.gc[1].shape).astype(np.uint8)))
+    la.b["q"].copy_(torch.from_numpy(rng.standard_normal((3, 4 * 112)).astype(np.float16)))
+    table = rng.permutation(12).astype(np.int32).reshape(3, 4)
+    la.g["table"].copy_(torch.from_numpy(table))
+    la.b["kv_len"].copy_(torch.from_numpy(np.array([128, 5, 77], np.int32)))
+    need = int(lib.sh_attention_kv_ws_bytes(C.byref(la.c), 3, 3, 1, 4, 4))
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    s, g, prev = torch.cuda.Stream(), torch.cuda.CUDAGraph(), lib.sh_get_stream()
+    with torch.cuda.graph(g, stream=s):
+        lib.sh_set_stream(s.cuda_stream)
+        assert lib.sh_attention_kv(A(la.b["q"]), A(la.b["o"]), C.byref(la.c), A(la.g["table"]), 4, A(la.b["kv_len"]), 0, 3, 3, 1, 4, 448, 448, 0.1, 0,
+                                   A(ws), need) == 0, shops.last_error()
+    lib.sh_set_stream(prev)
+    k, v, ks, vs = (to_np(c) for c in la.gc)
+    want = R.attention(to_np(la.b["q"]), k, v, ks, vs, table, [128, 5, 77], None, 4, 0.1, shops.SH_INT8)[0]
+    for _ in range(3):
+        la.b["o"].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        bad, err, _ = refs.close(to_np(la.b["o"]), want)
+        assert bad == 0, err
+
+
 def test_on_a_stream_of_its_own(lib, gpu):
     import torch
     rng = np.random.default_rng(9)
