@@ -779,30 +779,31 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
     }
 }
 
-// The parts of a cut item, in order: this block's unit is its first, the others follow `step` places apart.
+// The parts of a cut item, in order: its first unit, the others follow `step` places apart. A block takes every gridDim.x-th unit, and
+// of its rows the blockIdx.y-th share.
 __global__ __launch_bounds__(256) void k_kv_chunk_join(AttnArgs a) {
-    const uint32_t cut = blockIdx.x;
-    if (cut >= (uint32_t)a.meta[0].x) return;
-    const ChunkUnit u = a.unit[cut];
-    const uint32_t dh = a.c.dh, qn = dh / 4, half = CT / gridDim.y;
-    if (!u.parts) return;
-    for (uint32_t e = threadIdx.x; e < half * qn; e += 256) {
-        const uint32_t row = blockIdx.y * half + e / qn, d = 4 * (e % qn), r = u.qt * CT + row;
-        if (r >= u.nrow) break;
-        float M = -1e30f, l = 0.f;
-        sh_f4v o = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t i = 0; i < u.parts; ++i) {
-            const uint64_t at = (uint64_t)(cut + i * u.step) * CT + row;
-            const float m = a.ml[at * 2], s = a.ml[at * 2 + 1];
-            const sh_f4v v = *(const sh_f4v *)&a.part[at * dh + d];
-            const float mn = fmaxf(M, m), f = sh_fast_exp2(M - mn), g = sh_fast_exp2(m - mn);
-            o = o * f + v * g;
-            l = l * f + s * g;
-            M = mn;
+    const uint32_t cuts = (uint32_t)a.meta[0].x, dh = a.c.dh, qn = dh / 4, share = CT / gridDim.y;
+    for (uint32_t cut = blockIdx.x; cut < cuts; cut += gridDim.x) {
+        const ChunkUnit u = a.unit[cut];
+        if (!u.parts) continue;
+        for (uint32_t e = threadIdx.x; e < share * qn; e += 256) {
+            const uint32_t row = blockIdx.y * share + e / qn, d = 4 * (e % qn), r = u.qt * CT + row;
+            if (r >= u.nrow) break;
+            float M = -1e30f, l = 0.f;
+            sh_f4v o = {0.f, 0.f, 0.f, 0.f};
+            for (uint32_t i = 0; i < u.parts; ++i) {
+                const uint64_t at = (uint64_t)(cut + i * u.step) * CT + row;
+                const float m = a.ml[at * 2], s = a.ml[at * 2 + 1];
+                const sh_f4v v = *(const sh_f4v *)&a.part[at * dh + d];
+                const float mn = fmaxf(M, m), f = sh_fast_exp2(M - mn), g = sh_fast_exp2(m - mn);
+                o = o * f + v * g;
+                l = l * f + s * g;
+                M = mn;
+            }
+            const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+            const uint32_t qi = r / a.grp, qh = u.h * a.grp + (r - qi * a.grp);
+            store4(a.o + (uint64_t)(u.r0 + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
         }
-        const float f = l > 0.f || l != l ? 1.f / l : 0.f;
-        const uint32_t qi = r / a.grp, qh = u.h * a.grp + (r - qi * a.grp);
-        store4(a.o + (uint64_t)(u.r0 + qi) * a.ldo + (uint64_t)qh * dh + d, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
     }
 }
 
@@ -850,7 +851,7 @@ bool launch_chunk(const AttnArgs &a, uint32_t units, hipStream_t st) {
     if (a.c.dh <= 64) hipLaunchKernelGGL((k_kv_chunk<64, FP8>), dim3(units), dim3(256), 0, st, a);
     else if (a.c.dh <= 128) hipLaunchKernelGGL((k_kv_chunk<128, FP8>), dim3(units), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_kv_chunk<256, FP8>), dim3(units), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(k_kv_chunk_join, dim3(2 * CUT, 4), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_kv_chunk_join, dim3(768, 8), dim3(256), 0, st, a);
     return sh_launch_ok("sh_attention_kv");
 }
 
