@@ -360,7 +360,8 @@ int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uin
  * request are left as they are, as are a request's rows beyond its first max_q. max_q: an upper bound of a request's rows. ws: scratch
  * of at least sh_attention_kv_ws_bytes(c, B, rows, max_q, H, ld_table) bytes, 16-byte aligned, that no call running at the same
  * time uses (another stream, or a graph replayed beside this one, needs its own); what it holds need not be kept.
- * B x (ld_table bs / 64 + 1) x hkv x ceil(max_q (H / hkv) / 16) below 2^32. 0, -1 for bad arguments, -2 for too small a ws, SH_EHIP. Deterministic; how keys are shared out depends on the whole
+ * B x (ld_table bs / 64 + 1) x hkv x ceil(max_q (H / hkv) / 16) below 2^32, for chunks (rows H / 128 + B hkv) below 2^24.
+ * 0, -1 for bad arguments, -2 for too small a ws, SH_EHIP. Deterministic; how keys are shared out depends on the whole
  * batch, so a request's low bits may differ with its neighbours. */
 int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table, uint32_t ld_table, uint64_t kv_len, uint64_t row_start,
                     uint32_t B, uint32_t rows, uint32_t max_q, uint32_t H, uint32_t ldq, uint32_t ldo, float scale, uint32_t window,

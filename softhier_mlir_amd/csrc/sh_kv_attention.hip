@@ -913,7 +913,8 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     if (chunked(a.max_q, grp)) {
         // units: the row tiles, each request's last one short, and at most CUT parts more
         const uint64_t tiles = std::min<uint64_t>((uint64_t)B * (((uint64_t)a.max_q * grp + CT - 1) / CT), ((uint64_t)rows * grp + CT - 1) / CT + B);
-        if (tiles * c->hkv + CUT >= (1ull << 31)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", rows, H); return -1; }
+        // (a launch has fewer than 2^32 threads)
+        if (tiles * c->hkv + CUT >= (1ull << 24)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", rows, H); return -1; }
         const uint32_t units = (uint32_t)(tiles * c->hkv) + CUT;
         a.unit = (ChunkUnit *)(ws + 16);
         a.part = (float *)(ws + 16 + 2 * CUT * sizeof(ChunkUnit));
@@ -923,12 +924,12 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     a.part = (float *)(ws + GROUPS * 32);
     a.ml = a.part + (uint64_t)GROUPS * 2 * a.prow * c->dh;
     uint64_t tiles = ((uint64_t)ld_table * c->bs + KT - 1) / KT + 1;                     // an item's, at most
-    if (a.window) tiles = std::min<uint64_t>(tiles, ((uint64_t)a.window + a.max_q) / KT + 2);
     const uint64_t items = (uint64_t)c->hkv * (((uint64_t)a.max_q * grp + QT - 1) / QT);
     if (tiles * items >= (1ull << 32) / B) {                        // (tile counts of 32 bits)
         sh_set_error(-1, "[sh_attention_kv] %u requests of up to %llu tokens and %u heads", B, (unsigned long long)ld_table * c->bs, H);
         return -1;
     }
+    if (a.window) tiles = std::min<uint64_t>(tiles, ((uint64_t)a.window + a.max_q) / KT + 2);
     const bool ok = c->fmt == SH_FP8 ? launch_attn_width<true>(a, (uint32_t)tiles, st) : launch_attn_width<false>(a, (uint32_t)tiles, st);
     return ok ? 0 : SH_EHIP;
 }

@@ -63,6 +63,15 @@ def test_attention_refusals(lib):
         assert lib.sh_attention_kv(*a) == 0
 
 
+@pytest.mark.parametrize("B,rows,max_q,ld,window", [(1, 1 << 29, 1 << 29, 4, 0),       # chunk units: rows H / 128 = 2^24
+                                                    (65536, 65536, 1, 1 << 20, 0),      # tiles: 2^16 requests x 2^18 x 2 heads or more
+                                                    (65536, 65536, 1, 1 << 20, 64)])    # and a window leaves the bound as it is
+def test_attention_sizes_refused(lib, B, rows, max_q, ld, window):
+    c = C.byref(_cache())
+    assert lib.sh_attention_kv(ONE, ONE, c, ONE, ld, ONE, ONE, B, rows, max_q, 4, 256, 256, 0.125, window, ONE, 1 << 62) == -1
+    assert "of 4 heads" in shops.last_error()[1] or "and 4 heads" in shops.last_error()[1]
+
+
 def test_attention_workspace_grows_with_the_rows_and_heads(lib):
     c = C.byref(_cache())
     n = [lib.sh_attention_kv_ws_bytes(c, 64, 64, q, h, 64) for q, h in ((1, 2), (1, 8), (4, 8), (100, 8))]
