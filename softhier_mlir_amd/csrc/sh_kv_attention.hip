@@ -251,6 +251,13 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     // Codes that the Infinity Cache (256 MB) will not hold until the next call are read without allocating (120 MB and up here, one row tile): 48 requests
     // of up to 16384 keys, 311 MB, 72.6 -> 68.0 us; what it holds would be lost by that: 8 requests of 1000 keys 13.0 -> 14.5 us.
     const bool stream = a.once && T * (uint64_t)(2 * KT * dh) >= (120u << 20);
+    // A probability's fp16 operand is off by up to 2^-11 of it, which shows where values cancel (a quarter more error in all). Where an item has
+    // at most half the tile's rows (most single tokens), columns 8 .. 15 are the same rows again, and their operand of the second
+    // product is what the rounding of the first eight's took off: the two columns' sum keeps 22 bits (48 requests of up to 16384 keys
+    // 60.0 -> 61.6 us, 937 keys 8.8 -> 9.15). More rows keep the one: a second product of their own took 48 requests to 70.0, four drafts of 24
+    // requests from 13.0 to 13.8.
+    const bool two = a.prow <= QT / 2;
+    const float rest = two && m >= QT / 2 ? 1.f : 0.f;
     const uint32_t kg = m >> 2, kr0 = m & 3;
     uint32_t kcol[NP];                                              // columns past the head's width: read as its first ones, against zeros of Q
 #pragma unroll
@@ -259,7 +266,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         const uint32_t h = item / s.nqt, qt = item - h * s.nqt;
         const uint32_t j1 = min(s.nt, j0 + (t1 - t));
         // ---- rows
-        const uint32_t r = qt * QT + m, nrow = s.n * a.grp;
+        const uint32_t r = qt * QT + (two ? m & 7 : m), nrow = s.n * a.grp;
         const uint32_t qi = r / a.grp, qh = h * a.grp + (r - qi * a.grp);
         const int32_t first = s.L - (int32_t)s.nf;                                      // position of the request's first row
         const int32_t pos = r < nrow ? first + (int32_t)qi : -1;
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
                 for (int i = 0; i < 16; ++i) {
                     const float e = sh_fast_exp2(fmaf(x[i], ks, z));
                     sum += e;
-                    pf[i >> 3][i & 7] = (_Float16)e;
+                    pf[i >> 3][i & 7] = (_Float16)fmaf(-(float)(_Float16)e, rest, e);
                 }
                 l = fmaf(sum, sh_fast_rcp(w), l);
 #pragma unroll
@@ -391,10 +398,16 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         if constexpr (DH != 0) { if (stream) walk(std::true_type{}); else walk(std::false_type{}); }
         else walk(std::false_type{});
         l = sum_xor16_32(l);
+        if (two)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)                         // (row_ror:8)
+                    oa[i][k] += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(oa[i][k]), 0x128, 0xf, 0xf, true));
         const float ic = cn > 0.f ? 1.f / cn : 0.f;
         if (j0 == 0 && j1 == s.nt) {
             const float f = l > 0.f || l != l ? ic / l : 0.f;
-            if (r < nrow)
+            if (r < nrow && (m < 8 || !two))
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
                     if (DH || 16u * i < dh) store4(op + 16 * i + 4 * g, oa[i][0] * f, oa[i][1] * f, oa[i][2] * f, oa[i][3] * f);

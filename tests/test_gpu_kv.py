@@ -427,6 +427,38 @@ def test_attention_scales_far_apart(lib, gpu, fmt):
     assert np.isfinite(o).all()
 
 
+@pytest.mark.parametrize("fmt", [INT8, FP8])
+@pytest.mark.parametrize("H,hkv,dh", [(4, 2, 32), (15, 5, 64), (4, 4, 80), (7, 1, 112), (8, 1, 128), (2, 1, 256)])
+def test_attention_probabilities_keep_their_precision(lib, gpu, fmt, H, hkv, dh):
+    """Values of +-1 by turns and nearly equal scores: outputs near 0 whose terms are not, so that a probability held in fp16 (off by
+    up to 2^-11 of it) shows. The bound: the result's rounding; scores as in `bound`; 2^-19 for a page's log2 weight (one step of
+    2^-20 at 14), its difference to the maximum and the exponential's argument (2^-21 each); exp2 and the two halves, 2^-21; fp32
+    sums, 2^-24 of reach a key."""
+    import torch
+    rng = np.random.default_rng(dh)
+    L, bs = [2, 3, 17, 40], 16
+    pages = sum(-(-n // bs) for n in L)
+    c = Cache(rng, pages, hkv, dh, bs, fmt, values=True)
+    one = 64 if fmt == INT8 else 0x38                               # 64 x 2^-6, 1.0 x 2^0
+    v = np.where(np.arange(bs) % 2, (-one & 255) if fmt == INT8 else one | 128, one).astype(np.uint8)
+    host = list(c.before())
+    host[1] = np.broadcast_to(v, host[1].shape).copy()
+    host[2], host[3] = np.full_like(host[2], 2.0 ** -7), np.full_like(host[3], 2.0 ** -6 if fmt == INT8 else 1.0)
+    c.dv.copy_(dev(host[1].reshape(pages, -1)))
+    c.dks.copy_(dev(host[2])); c.dvs.copy_(dev(host[3]))             # noqa: E702
+    q = (rng.standard_normal((4, H * dh)) * 0.02).astype(np.float16)
+    table = _table(rng, L, bs, pages)
+    Q, T, Ln = to_dev(q), dev(table), dev(np.array(L, np.int32))
+    O = torch.zeros(4, H * dh, dtype=torch.float16, device="cuda")
+    need = int(lib.sh_attention_kv_ws_bytes(C.byref(c.c), 4, 4, 1, H, table.shape[1]))
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    assert lib.sh_attention_kv(A(Q), A(O), C.byref(c.c), A(T), table.shape[1], A(Ln), 0, 4, 4, 1, H, H * dh, H * dh, dh ** -0.5, 0, A(ws), need) == 0
+    o, reach, spread = R.attention(q, *host, table, L, None, H, dh ** -0.5, fmt)
+    d = (dh + 8) * 2.0 ** -23 * spread + 2.0 ** -19 + 2.0 ** -21
+    err = np.abs(to_np(O) - o)
+    assert (err <= 2.0 ** -11 * np.abs(o) + reach * (2 * d + max(L) * 2.0 ** -24) + 2.0 ** -24).all(), float((err / reach).max())
+
+
 @pytest.mark.parametrize("B,dh", [(65, 64), (300, 32), (512, 128), (700, 32), (256, 256), (257, 256), (600, 80)])
 @pytest.mark.parametrize("longest", [500, 5000])
 def test_attention_many_requests(lib, gpu, B, dh, longest):
