@@ -361,6 +361,7 @@ int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uin
  * of at least sh_attention_kv_ws_bytes(c, B, rows, max_q, H, ld_table) bytes, 16-byte aligned, that no call running at the same
  * time uses (another stream, or a graph replayed beside this one, needs its own); what it holds need not be kept.
  * B x (ld_table bs / 64 + 1) x hkv x ceil(max_q (H / hkv) / 16) below 2^32, for chunks (rows H / 128 + B hkv) below 2^24.
+ * Scores, scale q k, stay within fp32. A row of q with an infinity or a NaN in a head gives NaN there wherever it sees a key.
  * A probability is held to 22 bits where max_q (H / hkv) <= 8, with more rows in fp16: off by up to 2^-11 of it, so an output by up to 2^-11 of
  * sum p |v|, besides its own rounding.
  * 0, -1 for bad arguments, -2 for too small a ws, SH_EHIP. Deterministic; how keys are shared out depends on the whole

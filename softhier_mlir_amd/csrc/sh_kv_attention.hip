@@ -107,6 +107,23 @@ __device__ __forceinline__ uint4 ld_codes(const uint8_t *p) {
     }
 }
 
+// Eight halves of a row of q, infinities as NaN (x + 0 x): a score is then NaN for every key that the row sees and -inf for the others, so that
+// a row whose scores are all -inf is not taken for one that sees no key.
+__device__ __forceinline__ sh_h8 row8(uint4 v) {
+    const sh_h8 x = __builtin_bit_cast(sh_h8, v);
+    return __builtin_elementwise_fma(x, (sh_h8)(_Float16)0.f, x);
+}
+// The running maximum of a row that has seen no key, and the magnitude from which a maximum is `far` (below): 2^(x ks - mx) in one
+// multiply-add is off by the rounding of mx = x ks, half a step: 2^-5 at 2^20, a factor of 2^32 at 2^30. There x ks is rounded before mx is
+// taken off, and log2 w, which -mx would swallow, is added last.
+constexpr float LOWEST = -3.4028234663852886e38f, FAR = 1048576.f;
+__device__ __forceinline__ bool is_far(float mx) { return fabsf(mx) > FAR && mx != LOWEST; }
+__device__ __forceinline__ float less_max(float x, float ks, float mx) {
+#pragma clang fp contract(off)
+    const float y = x * ks;
+    return y - mx;
+}
+
 // Four consecutive outputs of a row.
 __device__ __forceinline__ void store4(uint16_t *p, float a, float b, float c, float d) {
     const sh_h2 x = {(_Float16)a, (_Float16)b}, y = {(_Float16)c, (_Float16)d};
@@ -307,13 +324,14 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         for (int p = 0; p < NP; ++p) {
             uint4 x = make_uint4(0, 0, 0, 0), y = x;
             if (r < nrow && 64 * p + 16 * g < dh) { x = sh_ld16_any(qp + 64 * p + 16 * g); y = sh_ld16_any(qp + 64 * p + 16 * g + 8); }
-            qf[2 * p] = __builtin_bit_cast(sh_h8, x);
-            qf[2 * p + 1] = __builtin_bit_cast(sh_h8, y);
+            qf[2 * p] = row8(x);
+            qf[2 * p + 1] = row8(y);
         }
         sh_f4v oa[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) oa[i] = sh_f4v{0.f, 0.f, 0.f, 0.f};
-        float mx = -1e30f, l = 0.f, cn = 0.f;
+        float mx = LOWEST, l = 0.f, cn = 0.f;
+        bool far = false;
         const auto walk = [&](auto once) {
             if (ja < jb) {
                 const uint32_t kn = page_at(ja + 1, 16 * kg), vn = page_at(ja + 1, 16 * g);
@@ -366,21 +384,25 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
                 const float mn = fmaxf(mx, tm), vm = max_xor16_32(vs);
                 float cs = cn;
                 if (!(vm * cn <= 16384.f) || cn == 0.f) cs = __builtin_amdgcn_ldexpf(1.f, 14 - (vm > 1e-30f ? __builtin_amdgcn_frexp_expf(vm) : -99));
-                if (__any(mn > mx) || cs != cn) {
+                if (__any(mn > mx) || cs != cn || far) {
                     const float al = sh_fast_exp2(mx - mn), be = al * (cn == 0.f ? 0.f : cs / cn);
                     l *= al;
 #pragma unroll
                     for (int i = 0; i < MT; ++i) oa[i] *= be;
                     mx = mn;
                     cn = cs;
+                    far = __any(is_far(mx));
+                    if (far)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] = less_max(x[i], ks, mx);
                 }
                 // probability and weight in one exponential: 2^(score - maximum + log2 w), the sum taken back from it
-                const float w = fmaxf(vs * cn, 1e-30f), z = __builtin_amdgcn_logf(w) - mx;
+                const float w = fmaxf(vs * cn, 1e-30f), z = __builtin_amdgcn_logf(w) - (far ? 0.f : mx), kx = far ? 1.f : ks;
                 float sum = 0.f;
                 sh_h8 pf[2];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float e = sh_fast_exp2(fmaf(x[i], ks, z));
+                    const float e = sh_fast_exp2(fmaf(x[i], kx, z));
                     sum += e;
                     pf[i >> 3][i & 7] = (_Float16)fmaf(-(float)(_Float16)e, rest, e);
                 }
@@ -453,7 +475,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         for (; turn < blocks; turn += NW) {
             const uint32_t e = turn * 64 + lane, row = e / qn, d = 4 * (e - row * qn), r = q0 + row;
             if (row >= a.prow || r >= nrow) continue;
-            float M = -1e30f, l = 0.f;
+            float M = LOWEST, l = 0.f;
             sh_f4v o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
             for (uint64_t k = in; k; k &= k - 1) {
@@ -494,7 +516,7 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
     // the workgroup of the item's last tile
     const uint32_t x = (uint32_t)me.x, share = (uint32_t)at_.y, more = (uint32_t)at_.z, big = more * (share + 1);
     const uint32_t end = x < big ? x / (share + 1) : more + (x - big) / share;
-    float M = -1e30f, l = 0.f;
+    float M = LOWEST, l = 0.f;
     sh_f4v o = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t i = wg + y; i <= end; i += P) {
         const uint64_t at = ((uint64_t)i * 2 + (i == wg ? 1 : 0)) * a.prow + row;
@@ -509,7 +531,7 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
     if (d == 0) { s_m[y] = M; s_l[y] = l; }
     __syncthreads();
     if (y) return;
-    float X = -1e30f, t = 0.f;
+    float X = LOWEST, t = 0.f;
     for (uint32_t i = 0; i < P; ++i) X = fmaxf(X, s_m[i]);
     o = sh_f4v{0.f, 0.f, 0.f, 0.f};
     for (uint32_t i = 0; i < P; ++i) {
@@ -622,7 +644,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
     for (int k = 0; k < KS; ++k) {
         uint4 x = make_uint4(0, 0, 0, 0);
         if (r < nrow && 16u * k < dh) x = sh_ld16_any(qp + 16 * k + 8 * hi);
-        qf[k] = __builtin_bit_cast(sh_h8, x);
+        qf[k] = row8(x);
     }
 
     // ---- staging: K chunk i of the wave is keys (64 wave + 256 i) / (DP / 16) on (16 at most, of one page), a lane 16 columns of one;
@@ -684,7 +706,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
     sh_f16v oa[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) oa[i] = sh_f16v{};
-    float mx = -1e30f, l = 0.f, cn = 0.f;
+    float mx = LOWEST, l = 0.f, cn = 0.f;
+    bool far = false;
     if (ja < jb) {
         pages(ja);
         load(ja);
@@ -737,23 +760,32 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
         const float mn = fmaxf(mx, sh_max_xor32(tm)), vm = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
         float cs = cn;
         if (!(vm * cn <= 16384.f) || cn == 0.f) cs = __builtin_amdgcn_ldexpf(1.f, 14 - (vm > 1e-30f ? __builtin_amdgcn_frexp_expf(vm) : -99));
-        if (__any(mn > mx) || cs != cn) {
+        if (__any(mn > mx) || cs != cn || far) {
             const float al = sh_fast_exp2(mx - mn), be = al * (cn == 0.f ? 0.f : cs / cn);
             l *= al;
 #pragma unroll
             for (int i = 0; i < DT; ++i) oa[i] *= be;
             mx = mn;
             cn = cs;
+            far = __any(is_far(mx));
+            if (far)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float &x = ((float *)&sa[q >> 1])[8 * (q & 1) + e];
+                        x = less_max(x, ks[q], mx);
+                    }
         }
         // probability and weight in one exponential: 2^(score - maximum + log2 w), the sum taken back from it
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float w = fmaxf(vs[q] * cn, 1e-30f), z = __builtin_amdgcn_logf(w) - mx;
+            const float w = fmaxf(vs[q] * cn, 1e-30f), z = __builtin_amdgcn_logf(w) - (far ? 0.f : mx), kx = far ? 1.f : ks[q];
             float sum = 0.f;
             sh_h8 pf;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float p = sh_fast_exp2(fmaf(sa[q >> 1][8 * (q & 1) + e], ks[q], z));
+                const float p = sh_fast_exp2(fmaf(sa[q >> 1][8 * (q & 1) + e], kx, z));
                 sum += p;
                 pf[e] = (_Float16)p;
             }
@@ -802,7 +834,7 @@ __global__ __launch_bounds__(256) void k_kv_chunk_join(AttnArgs a) {
         for (uint32_t e = threadIdx.x; e < share * qn; e += 256) {
             const uint32_t row = blockIdx.y * share + e / qn, d = 4 * (e % qn), r = u.qt * CT + row;
             if (r >= u.nrow) break;
-            float M = -1e30f, l = 0.f;
+            float M = LOWEST, l = 0.f;
             sh_f4v o = {0.f, 0.f, 0.f, 0.f};
             for (uint32_t i = 0; i < u.parts; ++i) {
                 const uint64_t at = (uint64_t)(cut + i * u.step) * CT + row;
@@ -907,7 +939,8 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     }
     const uint32_t grp = H / c->hkv;
     if ((uint64_t)std::min(max_q, rows) * grp >= (1ull << 31)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", max_q, H); return -1; }
-    if (!(scale > 0.f && scale <= 3.4e38f)) { sh_set_error(-1, "[sh_attention_kv] scale %g must be positive and finite", (double)scale); return -1; }
+    a.sc = scale * 1.4426950408889634f;
+    if (!(scale > 0.f && a.sc <= 3.4e38f)) { sh_set_error(-1, "[sh_attention_kv] scale %g must be positive and finite", (double)scale); return -1; }
     const uint64_t need = sh_attention_kv_ws_bytes(c, B, rows, max_q, H, ld_table);
     if (!ws || ws % 16) { sh_set_error(-1, "[sh_attention_kv] ws must be a 16-byte aligned address"); return -1; }
     if (ws_bytes < need) {
@@ -920,7 +953,6 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     a.B = B; a.rows = rows; a.max_q = std::min(max_q, rows); a.grp = grp; a.prow = part_rows(a.max_q, grp);
     a.window = window < ld_table * c->bs ? window : 0;               // (one that no key falls out of is none)
     a.groups = GROUPS;
-    a.sc = scale * 1.4426950408889634f;
     a.meta = (int4 *)ws;
     const hipStream_t st = sh_stream();
     if (chunked(a.max_q, grp)) {

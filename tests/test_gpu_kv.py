@@ -459,6 +459,84 @@ def test_attention_probabilities_keep_their_precision(lib, gpu, fmt, H, hkv, dh)
     assert (err <= 2.0 ** -11 * np.abs(o) + reach * (2 * d + max(L) * 2.0 ** -24) + 2.0 ** -24).all(), float((err / reach).max())
 
 
+def _call(lib, c, q, table, kv_len, row_start, H, scale, window=0, max_q=1):
+    import torch
+    rows, D = q.shape
+    Q, T, Ln = to_dev(q), dev(table), dev(np.asarray(kv_len, np.int32))
+    Rs = dev(np.asarray(row_start, np.int32)) if row_start is not None else None
+    O = torch.full((rows, D), 7.0, dtype=torch.float16, device="cuda")
+    need = int(lib.sh_attention_kv_ws_bytes(C.byref(c.c), len(kv_len), rows, max_q, H, table.shape[1]))
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    rc = lib.sh_attention_kv(A(Q), A(O), C.byref(c.c), A(T), table.shape[1], A(Ln), A(Rs) if Rs is not None else 0, len(kv_len), rows, max_q, H, D, D,
+                             scale, window, A(ws), need)
+    assert rc == 0, shops.last_error()
+    return to_np(O).astype(np.float64)
+
+
+FEW_AND_MANY = [(4, 2, 64, [40, 0, 700], None), (2, 1, 128, [6000, 3, 90], None), (16, 1, 64, [5000, 100, 2], None),       # single tokens, whole and cut
+                (4, 2, 80, [60, 300, 5], [40, 2, 9]), (4, 1, 64, [2500, 90, 31], [30, 90, 1])]                             # chunks, whole and cut
+
+
+@pytest.mark.parametrize("fmt", [INT8, FP8])
+@pytest.mark.parametrize("H,hkv,dh,L,new", FEW_AND_MANY)
+def test_attention_rows_with_infinities(lib, gpu, fmt, H, hkv, dh, L, new):
+    """An infinity or NaN in a head's row of q makes that head's output NaN wherever it sees a key, also where all of its scores are -inf
+    (every code of that channel has one sign); heads that see none give zeros, and the others their own values."""
+    rng = np.random.default_rng(dh + len(L))
+    bs = 16
+    pages = sum(-(-n // bs) for n in L) + 1
+    c = Cache(rng, pages, hkv, dh, bs, fmt, values=True)
+    host = list(c.before())
+    host[0][..., 0] = 0x30                                          # positive in both formats
+    c.dk.copy_(dev(host[0].reshape(pages, -1)))
+    start = None if new is None else np.concatenate([[0], np.cumsum(new)])
+    rows = 3 if new is None else sum(new)
+    q = rng.standard_normal((rows, H, dh)).astype(np.float16)
+    clean = q.copy()
+    bad = np.zeros((rows, H), bool)
+    for i, x in enumerate((-np.inf, np.inf, np.nan, -np.inf)):
+        r, h = (i * 7) % rows, i % H
+        q[r, h, 0 if i != 3 else dh - 1] = x
+        bad[r, h] = True
+    table = _table(rng, L, bs, pages)
+    o = _call(lib, c, q.reshape(rows, -1), table, L, start, H, dh ** -0.5, max_q=1 if new is None else max(new)).reshape(rows, H, dh)
+    want, reach, spread = (x.reshape(rows, H, dh) for x in R.attention(clean.reshape(rows, -1), *host, table, L, start, H, dh ** -0.5, fmt))
+    sees = reach.any(2) > 0
+    assert np.isnan(o[bad & sees]).all() and (o[bad & ~sees] == 0).all() and (bad & sees).any()
+    tol = bound(want, reach, spread, dh, max(L), (127 if fmt == INT8 else 448) * host[3].max())
+    assert (np.abs(o - want) <= tol)[~bad].all()
+
+
+@pytest.mark.parametrize("fmt", [INT8, FP8])
+@pytest.mark.parametrize("top", [3e6, -3e6, 1e9, -1e9, -4e30, 1e36, -1e36])
+@pytest.mark.parametrize("H,hkv,dh,L,new", FEW_AND_MANY)
+def test_attention_scores_of_any_size(lib, gpu, fmt, top, H, hkv, dh, L, new):
+    """Scores of one channel, -1/16 to 1 times or 1 to 16 times `top`, far enough apart that the largest alone counts; where several keys share it
+    (in pages of other value scales, too) their values are averaged. Bound: result and probability to fp16, 2^-11 each, log2 of a weight
+    (2^-19), sums (2^-24 a key)."""
+    rng = np.random.default_rng(dh + len(L))
+    bs = 16
+    pages = sum(-(-n // bs) for n in L) + 1
+    c = Cache(rng, pages, hkv, dh, bs, fmt, values=True)
+    host = list(c.before())
+    codes = np.array([8, 32, 64, 127]) if fmt == INT8 else np.array([0x20, 0x38, 0x40, 0x48])        # 8 .. 127; 1/8, 1, 2, 4
+    if top < 0:
+        codes = (-codes) & 255 if fmt == INT8 else codes | 128
+    host[0][..., 0] = codes[rng.integers(0, 4, host[0].shape[:3])]
+    host[2] = np.full_like(host[2], abs(top) / (127 if fmt == INT8 else 4))
+    c.dk.copy_(dev(host[0].reshape(pages, -1)))
+    c.dks.copy_(dev(host[2]))
+    start = None if new is None else np.concatenate([[0], np.cumsum(new)])
+    rows = 3 if new is None else sum(new)
+    q = np.zeros((rows, H, dh), np.float16)
+    q[..., 0] = 1
+    table = _table(rng, L, bs, pages)
+    o = _call(lib, c, q.reshape(rows, -1), table, L, start, H, 1.0, max_q=1 if new is None else max(new))
+    want, reach, _ = R.attention(q.reshape(rows, -1), *host, table, L, start, H, 1.0, fmt)
+    err = np.abs(o - want)
+    assert (err <= 2.0 ** -11 * np.abs(want) + reach * (2.0 ** -11 + 2.0 ** -19 + max(L) * 2.0 ** -24) + 2.0 ** -24).all(), float(err.max())
+
+
 @pytest.mark.parametrize("B,dh", [(65, 64), (300, 32), (512, 128), (700, 32), (256, 256), (257, 256), (600, 80)])
 @pytest.mark.parametrize("longest", [500, 5000])
 def test_attention_many_requests(lib, gpu, B, dh, longest):

@@ -108,3 +108,10 @@ def test_w4_refusals(lib):
         a = list(good)
         a[i] = 0
         assert lib.sh_gemm_w4(*a) == 0
+
+
+def test_attention_scale_times_log2_e_is_finite(lib):
+    c = C.byref(_cache())
+    need = lib.sh_attention_kv_ws_bytes(c, 2, 2, 1, 4, 4)
+    assert lib.sh_attention_kv(ONE, ONE, c, ONE, 4, ONE, 0, 2, 2, 1, 4, 256, 256, 3e38, 0, ONE, need) == -1
+    assert "scale" in shops.last_error()[1]
