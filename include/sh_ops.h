@@ -353,7 +353,7 @@ int sh_kv_slots(uint64_t table, uint32_t ld, uint64_t lens, uint64_t lens_out, u
 int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uint32_t ldv, uint64_t slots, uint32_t rows);
 
 /* Causal attention of new rows over the cache: o = softmax(scale q k^T) v per head, scale > 0, fp32 sums. Request b's rows are
- * row_start[b] .. row_start[b + 1] - 1 of q / o (fp16, [rows][H dh]; row_start = 0: row b), its keys the first kv_len[b]
+ * row_start[b] .. row_start[b + 1] - 1 of q / o (fp16, [rows][H dh]; row_start, which does not decrease; 0: row b), its keys the first kv_len[b]
  * tokens of its table row, and its last row sees all of them, each earlier row one key less. window > 0: a row sees
  * only its last `window` keys; pages wholly before every row's window are not read. Head h reads key / value head h / (H / hkv). Keys
  * in pages outside the cache (table entries < 0 or >= pages) are left out. A row that sees no key gets zeros; rows of no

@@ -558,7 +558,8 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
 // The keys of an item are cut into parts of C tiles, C a 768th of all tiles (and at least 8): one long request among short ones, or a
 // few rows over a long context, then keep every CU busy. Units are dealt out by the hardware, the request's last row tiles first
 // (they see most). A request that is cut has more than C tiles, so cut units number at most 2 T / C <= 1536: their parts go to as many places
-// of `part`, which k_kv_chunk_join adds up.
+// of `part`, which k_kv_chunk_join adds up. The launch has enough blocks while row_start does not decrease; where it does (an error of the
+// caller's), the units behind the last block do not exist, and an item that lacks parts for that is not joined.
 constexpr uint32_t CT = 128;               // rows of a unit
 constexpr uint32_t CUT = 768;              // units that share the whole evenly: three workgroups a CU, two of them at a time
 constexpr uint32_t CUT_MIN = 8;            // tiles of a part at least
@@ -584,6 +585,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
     all = wave_sum64(all);
     const uint32_t C = (uint32_t)max((all + CUT - 1) / CUT, (uint64_t)CUT_MIN);
     uint32_t idx = blockIdx.x, b = 0, parts = 1, cut0 = 0;           // cut0: cut units before this request
+    uint32_t base = 0, cuts = 0;                                     // block 0: units of the earlier rounds, cut units that this launch has
     Seq s{};
     bool found = false;
     for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
@@ -603,24 +605,23 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
             cut0 += i ? last(cu, i - 1) : 0u;
             found = true;
             if (blockIdx.x) break;
-            if (tid == 0) a.meta[0].x = (int)(cut0 - (i ? last(cu, i - 1) : 0u) + last(cu, 63));        // (block 0 finds the first request with rows)
         } else if (!found) {
             idx -= last(up, 63);
             cut0 += last(cu, 63);
-        } else if (tid == 0) {
-            a.meta[0].x += (int)last(cu, 63);
+        }
+        if (!blockIdx.x) {
+            const uint32_t z = base + up - w;
+            cuts += last(wave_scan32(p > 1 && z < gridDim.x ? min(w, gridDim.x - z) : 0u), 63);
+            base = min(base + last(up, 63), gridDim.x);
         }
     }
-    if (!found) {
-        if (blockIdx.x == 0 && tid == 0) a.meta[0].x = 0;
-        return;
-    }
+    if (!blockIdx.x && tid == 0) a.meta[0].x = (int)cuts;
+    if (!found) return;
     // (all of it is uniform: kept in scalar registers)
     const auto uni = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
     s = Seq{uni(s.r0), uni(s.n), uni(s.nf), uni(s.nqt), uni(s.ft), uni(s.nt), (int32_t)uni((uint32_t)s.L)};
     b = uni(b); parts = uni(parts); idx = uni(idx); cut0 = uni(cut0);
     const uint32_t h = idx % c.hkv, sp = idx / c.hkv % parts, qt = s.nqt - 1 - idx / c.hkv / parts, cut = cut0 + idx;
-    if (parts > 1 && cut >= 2 * CUT) return;                        // (row ranges that overlap beyond measure: nothing outside ws)
 
     // ---- rows
     const uint32_t nrow = s.n * a.grp, w0 = qt * CT + 32 * wave, r = w0 + n;
@@ -824,13 +825,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
     }
 }
 
-// The parts of a cut item, in order: its first unit, the others follow `step` places apart. A block takes every gridDim.x-th unit, and
+// The parts of a cut item, in order: its first unit, the others follow `step` places apart, all among the launch's `cuts`. A block takes every gridDim.x-th unit, and
 // of its rows the blockIdx.y-th share.
 __global__ __launch_bounds__(256) void k_kv_chunk_join(AttnArgs a) {
     const uint32_t cuts = (uint32_t)a.meta[0].x, dh = a.c.dh, qn = dh / 4, share = CT / gridDim.y;
     for (uint32_t cut = blockIdx.x; cut < cuts; cut += gridDim.x) {
         const ChunkUnit u = a.unit[cut];
-        if (!u.parts) continue;
+        if (!u.parts || cut + (u.parts - 1) * u.step >= cuts) continue;
         for (uint32_t e = threadIdx.x; e < share * qn; e += 256) {
             const uint32_t row = blockIdx.y * share + e / qn, d = 4 * (e % qn), r = u.qt * CT + row;
             if (r >= u.nrow) break;

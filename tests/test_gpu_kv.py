@@ -570,6 +570,35 @@ def test_attention_many_chunks(lib, gpu, B):
     _attend(lib, c, q, _table(rng, L.tolist(), bs, pages), L.tolist(), start, 2, 0.2)
 
 
+def test_attention_row_ranges_that_decrease(lib, gpu):
+    """150 requests over the same 512 rows (row_start 0, 512, 0, 512, ...): more units than a call of 512 rows has, one of them a request
+    that is cut and of whose parts only some exist. What is written is some request's result, and nothing else is written."""
+    import torch
+    rng = np.random.default_rng(41)
+    R_, H, hkv, dh, bs, B, long = 512, 4, 2, 32, 16, 300, 2 * 83
+    c = Cache(rng, 200, hkv, dh, bs, INT8)
+    kv_len = np.full(B, 64, np.int32)
+    kv_len[long] = 3000
+    table = np.tile(np.arange(188, dtype=np.int32), (B, 1))
+    start = np.where(np.arange(B + 1) % 2, R_, 0).astype(np.int32)
+    q = rng.standard_normal((R_, H * dh)).astype(np.float16)
+    need = int(lib.sh_attention_kv_ws_bytes(C.byref(c.c), B, R_, R_, H, 188))
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    O = torch.full((R_ + 64, H * dh), 7.0, dtype=torch.float16, device="cuda")
+    Q, T, Ln, Rs = to_dev(q), dev(table), dev(kv_len), dev(start)
+    for _ in range(3):
+        rc = lib.sh_attention_kv(A(Q), A(O, 32 * H * dh), C.byref(c.c), A(T), 188, A(Ln), A(Rs), B, R_, R_, H, H * dh, H * dh, 0.2, 0, A(ws), need)
+        assert rc == 0, shops.last_error()
+    o = to_np(O).astype(np.float64)
+    assert (o[:32] == 7.0).all() and (o[-32:] == 7.0).all() and (to_np(ws)[need:] == 255).all()
+    o = o[32:-32].reshape(R_, H, dh)
+    ok = np.zeros((R_, H), bool)
+    for n in (64, 3000):
+        want, reach, spread = (x.reshape(R_, H, dh) for x in R.attention(q, *c.before(), table[:1], [n], np.array([0, R_]), H, 0.2, INT8))
+        ok |= (np.abs(o - want) <= bound(want, reach, spread, dh, n, 127 * c.sc.max())).all(2)
+    assert ok.all()
+
+
 def test_attention_repeats_its_bits(lib, gpu):
     rng = np.random.default_rng(29)
     L = [5000, 40, 900]
