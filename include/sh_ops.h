@@ -338,7 +338,9 @@ typedef struct {
  *   kv_len [B]        keys that a request's rows see with themselves (lens + add); 0 for an ended or refused request
  * Requests take pages in order. One that needs more than are left, whose rows end behind `rows` or whose tokens exceed
  * ld x bs is refused: its length and table stay, and those after it that need pages are served only if the pages that
- * it and they ask for together are there. Pages of ended requests can be taken from the next call on. The sum of `add` stays
+ * it and they ask for together are there. Pages of ended requests can be taken from the next call on: all of its table row's, so a
+ * page is in one row only. Rows that share pages (a common prefix) are not for this call: the caller keeps table, lengths
+ * and pages of such requests itself, and sh_attention_kv reads them like others. The sum of `add` stays
  * below 2^31. B x ld and pages x bs below 2^31, B <= 65536. 0, -1 for bad arguments, SH_EHIP. */
 int sh_kv_slots(uint64_t table, uint32_t ld, uint64_t lens, uint64_t lens_out, uint64_t add, uint64_t pool, uint64_t state, uint64_t state_out,
                 uint64_t row_start, uint64_t slots, uint64_t pos, uint64_t kv_len, uint32_t B, uint32_t bs, uint32_t pages, uint32_t rows);

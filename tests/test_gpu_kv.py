@@ -599,6 +599,36 @@ def test_attention_row_ranges_that_decrease(lib, gpu):
     assert ok.all()
 
 
+@pytest.mark.parametrize("fmt", [INT8, FP8])
+def test_pages_shared_in_a_table_of_the_callers(lib, gpu, fmt):
+    """Three requests over the same two pages of a prefix, each with pages of its own behind: new tokens go into those, the shared pages keep
+    their bytes, and attention gives the bits of a table with a copy of the prefix for each."""
+    rng = np.random.default_rng(43)
+    H, hkv, dh, bs = 6, 2, 64, 16
+    c = Cache(rng, 14, hkv, dh, bs, fmt, values=True)
+    table = np.array([[3, 9, 0, 1], [3, 9, 2, 4], [3, 9, 5, 0]], np.int32)
+    held, new = [40, 48, 32], [3, 9, 1]
+    slot = np.array([table[b, p // bs] * bs + p % bs for b in range(3) for p in range(held[b], held[b] + new[b])], np.int32)
+    x = rng.standard_normal((2, len(slot), hkv * dh)).astype(np.float16)
+    X, S = to_dev(x), dev(slot)
+    assert lib.sh_kv_append(C.byref(c.c), A(X), A(X, x[0].size), hkv * dh, hkv * dh, A(S), len(slot)) == 0
+    now = c.now()
+    for g, w, old in zip(now, R.append(*c.before(), x[0], x[1], slot, fmt), c.before()):
+        assert np.array_equal(*(np.where(t == 128, 0, t) if t.dtype == np.uint8 else t for t in (g, w)))
+        assert np.array_equal(g[[3, 9]], old[[3, 9]])
+    q = rng.standard_normal((len(slot), H * dh)).astype(np.float16)
+    start, L = np.concatenate([[0], np.cumsum(new)]), [h + n for h, n in zip(held, new)]
+    one = _call(lib, c, q, table, L, start, H, 0.125, max_q=max(new))
+    apart = table.copy()
+    for b, (i, j) in ((1, (10, 11)), (2, (12, 13))):
+        apart[b, :2] = i, j
+        for t in (c.dk, c.dv, c.dks, c.dvs):
+            t[[i, j]] = t[[3, 9]]
+    assert np.array_equal(one, _call(lib, c, q, apart, L, start, H, 0.125, max_q=max(new)))
+    want, reach, spread = R.attention(q, *now, table, L, start, H, 0.125, fmt)
+    assert (np.abs(one - want) <= bound(want, reach, spread, dh, max(L), 448 * now[3].max())).all()
+
+
 def test_attention_repeats_its_bits(lib, gpu):
     rng = np.random.default_rng(29)
     L = [5000, 40, 900]
