@@ -349,8 +349,8 @@ int sh_kv_slots(uint64_t table, uint32_t ld, uint64_t lens, uint64_t lens_out, u
  * slot outside the cache are skipped). The scale of a page and head is the smallest power of two s >= 2^-32 with
  * |x| <= 127 s (448 s for SH_FP8) for its tokens, and never smaller than the one its older tokens have; where it grows, they are
  * rounded to it again. Codes round to nearest even. NaN is stored as 0, infinities as +-65504. A request's new tokens are
- * consecutive rows with ascending slots within a page, and a page that is written belongs to one request: rows that
- * put two requests, or one slot twice, into one page leave that page undefined. A first token at offset 0 starts a
+ * consecutive rows and, within a page, consecutive slots, and a page that is written belongs to one request: rows that put two
+ * requests, one slot twice, or slots with others (or skipped rows) between them into one page leave that page undefined. A first token at offset 0 starts a
  * page anew; other codes of the page are left as they are. 0, -1, SH_EHIP. */
 int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uint32_t ldv, uint64_t slots, uint32_t rows);
 
