@@ -310,9 +310,10 @@ int sh_attention_batched_prefetch(uint64_t q, uint64_t k, uint64_t v, uint64_t o
  * value = code x scale. A request's tokens 0, 1, ... lie in the pages its row of the block table names, bs to a page.
  * SH_INT8: two's complement, -127 .. 127. SH_FP8: OCP e4m3 (finite, largest 448). Values are stored with the tokens of a
  * page consecutive, as the product with the probabilities reads them.
- * A serving step: sh_kv_slots (where the new tokens go), the projections, sh_rope at the positions it gives,
- * sh_kv_append, sh_attention_kv. The calls need no device memory of the library's own and no host synchronisation, so a
- * step captures into a HIP graph whose replays read the lengths of that moment. */
+ * A serving step: sh_kv_slots (where the new tokens go), the projections, sh_rope, sh_kv_append, sh_attention_kv. (sh_rope takes a
+ * cos / sin row for each row and no positions: the caller gathers its table's rows at `pos`, any row where that is -1.) The
+ * calls need no device memory of the library's own and no host synchronisation, so a step captures into a HIP graph whose replays
+ * read the lengths of that moment. */
 typedef struct {
     uint64_t k;           /* codes: pages of [hkv][bs][dh], 16-byte aligned */
     uint64_t v;           /* codes: pages of [hkv][dh][bs], 16-byte aligned */
