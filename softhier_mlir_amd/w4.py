@@ -24,19 +24,26 @@ def unpack(words: np.ndarray) -> np.ndarray:
 
 def quantize(w: np.ndarray, group: int = 128) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
     """(words [K / 8, N], fp16 scales [G, N], zeros [G, N] uint8): for each group and column the range of its values, zero
-    among them, on 15 steps of `scale`; code = round(w / scale) + zero. A value is off by at most half a step, a step where the
-    range's end falls beyond the last code by the zero's rounding."""
+    among them, on 15 steps of `scale`, the smallest fp16 number that covers it (2^-24 at least); code = round(w / scale) + zero.
+    A value is off by at most half a step. Values that are not finite, and ranges beyond 15 x 65504, are refused."""
     K, N = w.shape
     if K % 8 or group % 32 or group <= 0:
         raise ValueError(f"K {K} must be a multiple of 8 and group {group} of 32")
     w = w.astype(np.float32)
+    if not np.isfinite(w).all():
+        raise ValueError("the weight has values that are not finite")
     G = -(-K // group)
     scale, zero = np.empty((G, N), np.float16), np.empty((G, N), np.uint8)
     codes = np.empty((K, N), np.uint8)
     for g in range(G):
         x = w[g * group:(g + 1) * group]
         lo, hi = np.minimum(x.min(0), 0), np.maximum(x.max(0), 0)
-        s = np.maximum((hi - lo) / 15, 2.0 ** -24).astype(np.float16)
+        step = np.maximum((hi.astype(np.float64) - lo) / 15, 2.0 ** -24)
+        if step.max(initial=0) > 65504:
+            raise ValueError(f"a group's range, {15 * step.max():g}, is beyond 15 steps of the largest fp16 scale")
+        s = step.astype(np.float16)
+        up = s < step                                                       # (fp16 against fp64: exact)
+        s[up] = np.nextafter(s[up], np.float16(np.inf))
         sf = s.astype(np.float32)
         z = np.clip(np.rint(-lo / sf), 0, 15)
         codes[g * group:(g + 1) * group] = np.clip(np.rint(x / sf) + z, 0, 15)

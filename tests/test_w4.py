@@ -40,6 +40,39 @@ def test_quantize_error(K, N, group):
         w4.quantize(w, 48)
 
 
+@pytest.mark.parametrize("std", [1e-8, 1e-6, 3e-6, 1e-5, 0.05, 1e3, 1e5])
+@pytest.mark.parametrize("side", ["both", "above", "below"])
+def test_quantize_is_off_by_half_a_step(std, side):
+    """Scales from the subnormal ones to the largest. The scale covers its group's range, so no code is clipped; the quotient w / scale in
+    fp32 is off by 15 * 2^-24 steps at most."""
+    rng = np.random.default_rng(int(np.log10(std) + 20))
+    w = (rng.standard_normal((256, 300)) * std).astype(np.float32)
+    w = np.abs(w) if side == "above" else -np.abs(w) if side == "below" else w
+    w[:32, 0], w[32:64, 1], w[5, 2] = 0, std, -15 * std
+    if 15 * std > 15 * 65504:                                       # (the row of -15 std is beyond the largest scale)
+        with pytest.raises(ValueError):
+            w4.quantize(w, 32)
+        w[5, 2] = 0
+    words, s, z = w4.quantize(w, 32)
+    step = s.astype(np.float64)[np.arange(256) // 32]
+    assert np.isfinite(step).all() and z.max() <= 15
+    err = np.abs(w4.dequantize(words, s, z, 32).astype(np.float64) - w)
+    assert (err <= step * (0.5 + 2.0 ** -20)).all(), float((err / step).max())
+
+
+def test_quantize_refuses_what_has_no_scale():
+    w = np.zeros((64, 4), np.float32)
+    for bad in (np.nan, np.inf, -np.inf, 15 * 65504 * 1.001):
+        w[33, 2] = bad
+        with pytest.raises(ValueError):
+            w4.quantize(w, 32)
+    w[33, 2], w[34, 2] = 15 * 65504 * 0.6, -15 * 65504 * 0.6             # each in range, not both
+    with pytest.raises(ValueError):
+        w4.quantize(w, 32)
+    w[34, 2], w[33, 2] = 0, 15 * 65504
+    assert w4.dequantize(*w4.quantize(w, 32), 32)[33, 2] == 15 * 65504
+
+
 def test_reference_codes_are_e4m3():
     import torch
     c = np.arange(256, dtype=np.uint8)
