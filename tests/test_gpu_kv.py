@@ -629,6 +629,61 @@ def test_pages_shared_in_a_table_of_the_callers(lib, gpu, fmt):
     assert (np.abs(one - want) <= bound(want, reach, spread, dh, max(L), 448 * now[3].max())).all()
 
 
+WINDOWS = [   # H, hkv, dh, bs, lengths, new rows, window
+    (4, 2, 128, 16, [6500, 3000, 40, 2600], None, 2500),            # single tokens, cut between workgroups: 40 key tiles each
+    (8, 1, 64, 64, [9000, 2501, 2499], None, 2500),
+    (16, 1, 64, 16, [7000, 64], None, 4000),                        # sixteen rows a tile
+    (2, 1, 80, 32, [6100, 5000], [4, 3], 2500),                     # drafts
+    (4, 1, 256, 16, [6000], [3], 2600),
+    (4, 1, 48, 16, [6500, 2600], [1, 4], 2500),
+    (8, 2, 64, 16, [6000, 700, 3000], [40, 20, 1], 2500),           # chunks whose keys are cut into parts
+    (4, 1, 128, 32, [5000, 300], [90, 300], 1000),
+    (2, 1, 32, 16, [3000], [700], 600),                             # row tiles that see few of the request's key tiles: empty parts
+    (4, 1, 256, 16, [2800], [50], 2000),
+]
+
+
+@pytest.mark.parametrize("fmt", [INT8, FP8])
+@pytest.mark.parametrize("H,hkv,dh,bs,L,new,window", WINDOWS)
+def test_attention_window_over_long_contexts(lib, gpu, fmt, H, hkv, dh, bs, L, new, window):
+    """A first key tile behind 0 with keys that are shared between workgroups and joined. Pages before every window hold NaN codes and
+    scales."""
+    rng = np.random.default_rng(window + sum(L))
+    pages = sum(-(-n // bs) for n in L) + 3
+    c = Cache(rng, pages, hkv, dh, bs, fmt, values=True)
+    table = _table(rng, L, bs, pages)
+    host = c.before()
+    clean = [h.copy() for h in host]
+    for b, n in enumerate(L):
+        for pg in table[b, : max(0, n - (new[b] if new else 1) + 1 - window) // bs]:
+            host[0][pg], host[1][pg], host[2][pg], host[3][pg] = 0x7F, 0xFF, np.nan, np.nan
+            clean[2][pg], clean[3][pg] = 0, 0
+    c.dk.copy_(dev(host[0].reshape(pages, -1))); c.dv.copy_(dev(host[1].reshape(pages, -1)))   # noqa: E702
+    c.dks.copy_(dev(host[2])); c.dvs.copy_(dev(host[3]))                                       # noqa: E702
+    start = None if new is None else np.concatenate([[0], np.cumsum(new)])
+    q = rng.standard_normal((len(L) if new is None else sum(new), H * dh)).astype(np.float16)
+    _attend(lib, c, q, table, L, start, H, dh ** -0.5, window=window, host=clean)
+
+
+@pytest.mark.parametrize("B", [65, 300, 600, 1500])
+@pytest.mark.parametrize("window,longest,rows", [(100, 900, 3), (2500, 6000, 3), (1000, 4000, 90)])
+def test_attention_window_of_many_requests(lib, gpu, B, window, longest, rows):
+    """More requests than a wave has lanes or a workgroup threads, runs of idle ones between them, under a window; single tokens, drafts and
+    (90 rows) chunks."""
+    rng = np.random.default_rng(B + window)
+    bs, dh = 16, 32
+    new = np.where(rng.random(B) < 0.6, 0, rng.integers(1, 4, B))
+    new[B // 4:B // 2] = 0
+    new[B // 3], new[B - 1] = rows, 2
+    L = np.where(rng.random(B) < 0.5, 0, rng.integers(1, 60, B))
+    L[B // 3], L[B - 1], L[7] = longest, longest // 2, window + 1
+    start = np.concatenate([[0], np.cumsum(new)])
+    pages = int(sum(-(-n // bs) for n in L)) + 1
+    c = Cache(rng, pages, 1, dh, bs, FP8, values=True)
+    q = rng.standard_normal((int(start[-1]), 2 * dh)).astype(np.float16)
+    _attend(lib, c, q, _table(rng, L.tolist(), bs, pages), L.tolist(), start, 2, 0.2, window=window)
+
+
 def test_attention_repeats_its_bits(lib, gpu):
     rng = np.random.default_rng(29)
     L = [5000, 40, 900]

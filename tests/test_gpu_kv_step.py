@@ -225,6 +225,83 @@ def test_first_call_under_capture(lib, gpu):
         assert bad == 0, err
 
 
+@pytest.mark.parametrize("H,hkv,dh,longest,window", [(8, 1, 64, 1, 0), (16, 1, 128, 1, 3000), (4, 2, 96, 4, 0), (8, 1, 128, 20, 0), (4, 1, 64, 40, 2000)])
+def test_lengths_that_move_between_replays(lib, gpu, H, hkv, dh, longest, window):
+    """Tables, the cache's write and attention in one graph, with a table wide enough that keys are shared between workgroups (8192
+    tokens). From replay to replay lengths grow by tokens and by thousands, pass page ends, and requests end and begin; every replay gives the bits
+    of the same calls made eagerly on other buffers."""
+    import torch
+    rng = np.random.default_rng(H + dh + longest)
+    B, bs, ld, rows = 4, 16, 512, 4 * longest
+    pages = 4 * ld
+    kw = dict(B=B, H=H, hkv=hkv, dh=dh, D=32, bs=bs, ld=ld, pages=pages, rows=rows, fmt=shops.SH_FP8)
+    both = [Layer(21, **kw), Layer(21, **kw)]
+    codes = [rng.integers(0, 256, c.shape).astype(np.uint8) for c in both[0].gc[:2]]
+    for c in codes:
+        c[(c & 127) == 127] = 1
+    kv = rng.standard_normal((rows, H * dh + 2 * hkv * dh)).astype(np.float16)
+    stride = kv.shape[1]
+    prev, calls = lib.sh_get_stream(), []
+    for la in both:
+        for t, c in zip(la.gc, codes):
+            t.copy_(torch.from_numpy(c))
+        la.gc[2].fill_(2.0 ** -7)
+        la.gc[3].fill_(2.0 ** -6)
+        la.qkv = torch.from_numpy(kv).cuda()
+        need = int(lib.sh_attention_kv_ws_bytes(C.byref(la.c), B, rows, longest, H, ld))
+        la.ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        la.o = torch.zeros(rows, H * dh, dtype=torch.float16, device="cuda")
+
+        def call(la=la, need=need):
+            b, g = la.b, la.g
+            rc = [lib.sh_kv_slots(A(g["table"]), ld, A(g["lens"]), A(g["lens"]), A(b["add"]), A(g["pool"]), A(g["state"]), A(g["state"]),
+                                  A(b["row_start"]), A(b["slots"]), A(b["pos"]), A(b["kv_len"]), B, bs, pages, rows),
+                  lib.sh_kv_append(C.byref(la.c), A(la.qkv, H * dh), A(la.qkv, (H + hkv) * dh), stride, stride, A(b["slots"]), rows),
+                  lib.sh_attention_kv(A(la.qkv), A(la.o), C.byref(la.c), A(g["table"]), ld, A(b["kv_len"]), A(b["row_start"]), B, rows, longest, H,
+                                      stride, H * dh, dh ** -0.5, window, A(la.ws), need)]
+            assert rc == [0, 0, 0], (rc, shops.last_error())
+        calls.append(call)
+    # the requests' tables for the longest lengths, so that lengths can be set from outside: request b has pages b ld .. (b + 1) ld - 1
+    for la in both:
+        la.g["table"].copy_(torch.arange(pages, dtype=torch.int32).view(B, ld))
+        la.g["state"].copy_(torch.tensor([0, 0, 0], dtype=torch.int32))
+    torch.cuda.synchronize()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        lib.sh_set_stream(s.cuda_stream)
+        calls[1]()
+    lib.sh_set_stream(prev)
+    lens = [[15, 0, 6000, 31], None, [47, 16, 8000, 4000], None, [8192 - longest, 1, 100, 3200], [0, 0, 0, 0], None, [5000, 5000, 5000, 5000]]
+    for i, at in enumerate(lens):
+        add = [longest, max(1, longest // 2), 1, 0 if i % 3 == 1 else longest]
+        for la in both:
+            if at is not None:
+                la.g["lens"].copy_(torch.tensor(at, dtype=torch.int32))
+            head = la.g["lens"].cpu()
+            # the step's new pages come from the ring: it is given those of the table's next entries, in order
+            fresh = [int(la.g["table"][b, j]) for b in range(B) for j in range(-(-int(head[b]) // bs), -(-(int(head[b]) + add[b]) // bs))]
+            la.g["pool"][: len(fresh)] = torch.tensor(fresh, dtype=torch.int32, device="cuda")
+            la.g["state"].copy_(torch.tensor([0, len(fresh), 0], dtype=torch.int32))
+            la.b["add"].copy_(torch.tensor(add, dtype=torch.int32))
+            la.o.fill_(7.0)
+        torch.cuda.synchronize()
+        calls[0]()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        one, two = both
+        assert int(one.g["state"][2]) == 0 and int(one.b["kv_len"].min()) > 0
+        for x, y in [(one.g[k], two.g[k]) for k in ("table", "lens", "pool", "state")] + [(one.b[k], two.b[k]) for k in ("slots", "pos", "row_start", "kv_len")]:
+            assert torch.equal(x, y), i
+        for x, y in list(zip(one.gc, two.gc)) + [(one.o, two.o)]:
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), i
+        n = int(one.b["row_start"][-1])
+        want = R.attention(kv[:n, : H * dh], *(to_np(t) for t in one.gc), to_np(one.g["table"]), to_np(one.b["kv_len"]), to_np(one.b["row_start"]), H,
+                           dh ** -0.5, shops.SH_FP8, window)[0]
+        bad, err, _ = refs.close(to_np(one.o)[:n], want)
+        assert bad == 0, (i, err)
+
+
 def test_on_a_stream_of_its_own(lib, gpu):
     import torch
     rng = np.random.default_rng(9)
