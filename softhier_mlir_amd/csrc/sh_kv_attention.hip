@@ -251,11 +251,20 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         b = owner(t);
         base = before(b);
     }
+    uint32_t from = 0;                                              // MANY: lane i holds request from + i
+    const auto take = [&](uint32_t i) {
+        from = i;
+        mine = Seq{};
+        if (i + lane < a.B) mine = seq_of<QT>(a, i + lane);
+    };
     const auto get = [&](uint32_t i) {
         if constexpr (!MANY)
             if (!a.wide) return lane_seq(mine, i);
-        Seq q;
-        if constexpr (MANY) q = seq_of<QT>(a, i); else q = s_seq[i];
+        if constexpr (MANY) {
+            take(i);
+            return lane_seq(mine, 0);
+        }
+        const Seq q = s_seq[i];
         return Seq{uni(q.r0), uni(q.n), uni(q.nf), uni(q.nqt), uni(q.ft), uni(q.nt), (int32_t)uni((uint32_t)q.L)};
     };
     Seq s{};
@@ -451,7 +460,18 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         if (j1 == s.nt && t < t1) {
             if (++item == s.nqt * c.hkv) {
                 item = 0;
-                do { s = get(++b); } while (s.nt == 0 && b + 1 < a.B);
+                if constexpr (MANY) {                               // the next request with tiles, 64 at a time: idle ones may be thousands
+                    uint64_t has = 0;
+                    for (++b; b < a.B && !has;) {
+                        if (b - from >= 64) take(b);
+                        has = __ballot(mine.nt != 0) >> (b - from);
+                        b = has ? b + __builtin_ctzll(has) : from + 64;
+                    }
+                    if (!has) break;                                // (lengths that changed while the kernel ran)
+                    s = lane_seq(mine, b - from);
+                } else {
+                    do { s = get(++b); } while (s.nt == 0 && b + 1 < a.B);
+                }
             }
         }
     }

@@ -684,6 +684,24 @@ def test_attention_window_of_many_requests(lib, gpu, B, window, longest, rows):
     _attend(lib, c, q, _table(rng, L.tolist(), bs, pages), L.tolist(), start, 2, 0.2, window=window)
 
 
+@pytest.mark.parametrize("B,active", [(65536, [0, 1, 63, 64, 20000, 20128, 65535]), (513, [512]), (2000, [700]), (4096, list(range(0, 4096, 129)))])
+def test_attention_slots_mostly_idle(lib, gpu, B, active):
+    """A batch of fixed slots of which few have a request; the others add no row (and some hold keys all the same)."""
+    rng = np.random.default_rng(B)
+    bs, ld, dh = 16, 64, 64
+    L, new = np.zeros(B, np.int32), np.zeros(B, np.int64)
+    L[::97] = 100
+    L[active], new[active] = rng.integers(1, ld * bs + 1, len(active)), rng.integers(1, 4, len(active))
+    c = Cache(rng, 200, 1, dh, bs, INT8)
+    table = rng.integers(0, 200, (B, ld)).astype(np.int32)
+    start = np.concatenate([[0], np.cumsum(new)])
+    q = rng.standard_normal((int(start[-1]), 2 * dh)).astype(np.float16)
+    o = _call(lib, c, q, table, L, start, 2, 0.125, max_q=3)
+    some = np.array(active)
+    want, reach, spread = R.attention(q, *c.before(), table[some], L[some], np.concatenate([start[some], start[-1:]]), 2, 0.125, INT8)
+    assert (np.abs(o - want) <= bound(want, reach, spread, dh, ld * bs, 127 * c.sc.max())).all()
+
+
 def test_attention_repeats_its_bits(lib, gpu):
     rng = np.random.default_rng(29)
     L = [5000, 40, 900]
