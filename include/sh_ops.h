@@ -362,7 +362,8 @@ int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uin
  * in pages outside the cache (table entries < 0 or >= pages) are left out. A row that sees no key gets zeros; rows of no
  * request are left as they are, as are a request's rows beyond its first max_q. max_q: an upper bound of a request's rows. ws: scratch
  * of at least sh_attention_kv_ws_bytes(c, B, rows, max_q, H, ld_table) bytes, 16-byte aligned, that no call running at the same
- * time uses (another stream, or a graph replayed beside this one, needs its own); what it holds need not be kept.
+ * time uses (another stream, or a graph replayed beside this one, needs its own); what it holds need not be kept, and what is
+ * enough for some B, rows, max_q and ld_table is enough for smaller ones.
  * B x (ld_table bs / 64 + 1) x hkv x ceil(max_q (H / hkv) / 16) below 2^32, for chunks (rows H / 128 + B hkv) below 2^24.
  * Scores, scale q k, stay within fp32. A row of q with an infinity or a NaN in a head gives NaN there wherever it sees a key.
  * A probability is held to 22 bits where max_q (H / hkv) <= 8, with more rows in fp16: off by up to 2^-11 of it, so an output by up to 2^-11 of

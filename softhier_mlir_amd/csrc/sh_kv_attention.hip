@@ -40,7 +40,8 @@ struct AttnArgs {
     uint32_t ld, B, rows, max_q, grp, prow, window, groups, wide, whole, once;
     float sc;                              // scale x log2 e
     float *part, *ml;                      // partials [groups][2][prow][dh], their (max, sum) [groups][2][prow][2]
-    ChunkUnit *unit;                       // [2 CUT]
+    ChunkUnit *unit;                       // [places]
+    uint32_t places;                       // cut units of a call of chunks, at most
     int4 *meta;                            // [groups][2]: of the item begun here and not ended: its last tile (-1: none), first row, rows, head;
                                            // the request's first row, tiles of a workgroup, workgroups with one more
 };
@@ -577,9 +578,10 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
 // rows of one prompt 218 us, 630 TFLOP/s; LDS reads (32 KB a wave and tile) come next.
 // The keys of an item are cut into parts of C tiles, C a 768th of all tiles (and at least 8): one long request among short ones, or a
 // few rows over a long context, then keep every CU busy. Units are dealt out by the hardware, the request's last row tiles first
-// (they see most). A request that is cut has more than C tiles, so cut units number at most 2 T / C <= 1536: their parts go to as many places
-// of `part`, which k_kv_chunk_join adds up. The launch has enough blocks while row_start does not decrease; where it does (an error of the
-// caller's), the units behind the last block do not exist, and an item that lacks parts for that is not joined.
+// (they see most). A request that is cut has more than C tiles, so cut units number at most 2 T / C <= 1536, and no more than all units cut
+// at the table's width: their parts go to as many places of `part`, which k_kv_chunk_join adds up. The launch has enough blocks, and
+// `part` enough places, while row_start does not decrease; where it does (an error of the caller's), the units behind the last block
+// or place do not exist, and an item that lacks parts for that is not joined.
 constexpr uint32_t CT = 128;               // rows of a unit
 constexpr uint32_t CUT = 768;              // units that share the whole evenly: three workgroups a CU, two of them at a time
 constexpr uint32_t CUT_MIN = 8;            // tiles of a part at least
@@ -635,13 +637,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
             base = min(base + last(up, 63), gridDim.x);
         }
     }
-    if (!blockIdx.x && tid == 0) a.meta[0].x = (int)cuts;
+    if (!blockIdx.x && tid == 0) a.meta[0].x = (int)min(cuts, a.places);
     if (!found) return;
     // (all of it is uniform: kept in scalar registers)
     const auto uni = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
     s = Seq{uni(s.r0), uni(s.n), uni(s.nf), uni(s.nqt), uni(s.ft), uni(s.nt), (int32_t)uni((uint32_t)s.L)};
     b = uni(b); parts = uni(parts); idx = uni(idx); cut0 = uni(cut0);
     const uint32_t h = idx % c.hkv, sp = idx / c.hkv % parts, qt = s.nqt - 1 - idx / c.hkv / parts, cut = cut0 + idx;
+    if (parts > 1 && cut >= a.places) return;                       // (only where row_start decreases)
 
     // ---- rows
     const uint32_t nrow = s.n * a.grp, w0 = qt * CT + 32 * wave, r = w0 + n;
@@ -926,6 +929,15 @@ bool launch_chunk(const AttnArgs &a, uint32_t units, hipStream_t st) {
 constexpr uint32_t CHUNK_ROWS = 64;
 bool chunked(uint32_t max_q, uint32_t grp) { return (uint64_t)max_q * grp > CHUNK_ROWS; }
 
+// Row tiles of a call of chunks, each request's last one short; and its cut units, at most.
+uint64_t chunk_tiles(uint32_t B, uint32_t rows, uint32_t max_q, uint32_t grp) {
+    return std::min<uint64_t>((uint64_t)B * (((uint64_t)max_q * grp + CT - 1) / CT), ((uint64_t)rows * grp + CT - 1) / CT + B);
+}
+uint64_t chunk_places(const sh_kv_cache &c, uint32_t B, uint32_t rows, uint32_t max_q, uint32_t grp, uint32_t ld) {
+    const uint64_t nt = ((uint64_t)ld * c.bs + KT - 1) / KT, units = chunk_tiles(B, rows, max_q, grp) * c.hkv;
+    return nt <= CUT_MIN ? 0 : std::min<uint64_t>(2 * CUT, units * ((nt + CUT_MIN - 1) / CUT_MIN));
+}
+
 }  // namespace
 
 extern "C" {
@@ -933,9 +945,11 @@ extern "C" {
 uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t rows, uint32_t max_q, uint32_t H, uint32_t ld_table) {
     if (!c || !B || !rows || !max_q || !c->hkv || !H || !ld_table || !c->dh) return 0;
     max_q = std::min(max_q, rows);
-    if (chunked(max_q, H / c->hkv)) return 2 * CUT * ((uint64_t)CT * (c->dh + 2) * 4 + sizeof(ChunkUnit)) + 16;
-    const uint64_t prow = part_rows(max_q, H / c->hkv);
-    return (uint64_t)GROUPS * (2 * prow * (c->dh + 2) * 4 + 32);
+    const uint32_t grp = H / c->hkv;
+    const uint64_t prow = part_rows(max_q, grp), few = (uint64_t)GROUPS * (2 * prow * (c->dh + 2) * 4 + 32);
+    if (!chunked(max_q, grp)) return few;
+    // (never less than a call of fewer rows needs)
+    return std::max(few, chunk_places(*c, B, rows, max_q, grp, ld_table) * ((uint64_t)CT * (c->dh + 2) * 4 + sizeof(ChunkUnit)) + 16);
 }
 
 int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table, uint32_t ld_table, uint64_t kv_len, uint64_t row_start,
@@ -977,14 +991,14 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
     a.meta = (int4 *)ws;
     const hipStream_t st = sh_stream();
     if (chunked(a.max_q, grp)) {
-        // units: the row tiles, each request's last one short, and at most CUT parts more
-        const uint64_t tiles = std::min<uint64_t>((uint64_t)B * (((uint64_t)a.max_q * grp + CT - 1) / CT), ((uint64_t)rows * grp + CT - 1) / CT + B);
-        // (a launch has fewer than 2^32 threads)
+        // units: the row tiles, and at most CUT parts more (a launch has fewer than 2^32 threads)
+        const uint64_t tiles = chunk_tiles(B, rows, a.max_q, grp);
         if (tiles * c->hkv + CUT >= (1ull << 24)) { sh_set_error(-1, "[sh_attention_kv] %u rows of %u heads", rows, H); return -1; }
         const uint32_t units = (uint32_t)(tiles * c->hkv) + CUT;
+        a.places = (uint32_t)chunk_places(*c, B, rows, a.max_q, grp, ld_table);
         a.unit = (ChunkUnit *)(ws + 16);
-        a.part = (float *)(ws + 16 + 2 * CUT * sizeof(ChunkUnit));
-        a.ml = a.part + (uint64_t)2 * CUT * CT * c->dh;
+        a.part = (float *)(ws + 16 + a.places * sizeof(ChunkUnit));
+        a.ml = a.part + (uint64_t)a.places * CT * c->dh;
         return (c->fmt == SH_FP8 ? launch_chunk<true>(a, units, st) : launch_chunk<false>(a, units, st)) ? 0 : SH_EHIP;
     }
     a.part = (float *)(ws + GROUPS * 32);

@@ -115,3 +115,23 @@ def test_attention_scale_times_log2_e_is_finite(lib):
     need = lib.sh_attention_kv_ws_bytes(c, 2, 2, 1, 4, 4)
     assert lib.sh_attention_kv(ONE, ONE, c, ONE, 4, ONE, 0, 2, 2, 1, 4, 256, 256, 3e38, 0, ONE, need) == -1
     assert "scale" in shops.last_error()[1]
+
+
+def test_attention_workspace_of_chunks_follows_the_table(lib):
+    """A call of chunks holds parts only where keys can be cut: 104 MB at most here, a few where the table is short; and the size for the
+    largest call is enough for every smaller one."""
+    c = C.byref(_cache(hkv=8, dh=128))
+    n = [lib.sh_attention_kv_ws_bytes(c, 8, 4096, 2048, 32, ld) for ld in (1, 32, 33, 64, 1 << 20)]
+    few = lib.sh_attention_kv_ws_bytes(c, 8, 4096, 4, 32, 1)
+    assert n[0] == n[1] == few < n[2] <= n[3] <= n[4] == 1536 * (128 * 130 * 4 + 32) + 16
+    assert lib.sh_attention_kv_ws_bytes(c, 1, 20, 20, 32, 64) < n[4] // 16
+    steps = dict(B=(1, 2, 9, 300), rows=(1, 17, 64, 1000), max_q=(1, 2, 16, 17, 900), ld=(1, 40, 5000))
+    at = lambda B, rows, max_q, ld: lib.sh_attention_kv_ws_bytes(c, B, rows, max_q, 32, ld)  # noqa: E731
+    for name, v in steps.items():
+        for lo, hi in zip(v, v[1:]):
+            for B in steps["B"]:
+                for rows in steps["rows"]:
+                    for q in steps["max_q"]:
+                        for ld in steps["ld"]:
+                            a = dict(B=B, rows=rows, max_q=q, ld=ld)
+                            assert at(**{**a, name: lo}) <= at(**{**a, name: hi}), (a, name, lo, hi)
