@@ -258,17 +258,23 @@ bool launch_w4(const W4Args &a, hipStream_t st) {
     hipLaunchKernelGGL((k_w4<MT, CW, NW, GS, SU>), dim3(sh_cdiv(a.N, 16 * CW), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), lds, st, a);
     return sh_launch_ok("sh_gemm_w4");
 }
-// The tile with the least rounds of workgroups over the 256 CUs times the time of one (a tile's registers allow one a CU): wider columns
-// convert a word once for every 16 rows and read x once for every 16 CW columns, narrower ones make more workgroups. The times are
-// those of a round at K = 4096 (1 x 64 columns 7.0 us, x 32 5.2, x 16 4.5; 32 rows x 64 columns 11.5). Measured, K = 8192: 50 rows,
-// 4096 columns (256 workgroups of 16 x 64) 15.3 us against 20.5 for 32 x 32; 4160 columns 24.0 in 32 x 64 against 27.1 in 16 x 64 (260).
+// The tile with the least rounds of workgroups over the 256 CUs times the time of one, counted as one workgroup a CU (which is what the
+// registers of the 64-column tiles allow; of the 16- and 32-column ones two fit): wider columns convert a word once for every 16 rows
+// and read x once for every 16 CW columns, narrower ones make more workgroups. The times are those of a round at K = 4096 in groups
+// of 128 (1 x 64 columns 7.0 us, x 32 5.2, x 16 4.5; 32 rows x 64 columns 11.5). Measured: 50 rows, K = 8192,
+// 4096 columns (256 workgroups of 16 x 64) 15.3 us against 20.5 for 32 x 32; 64 rows, K = 4096, 4160 columns in 32 x 64 13.3 against 18.0
+// in tiles of 16 rows, in groups of 32 15.2 against 23.3.
 template <int GS, int SU>
 bool launch_w4_tile(const W4Args &a, hipStream_t st) {
     const uint64_t mt = sh_cdiv(a.M, 16);
     const auto cost = [&](uint64_t m, uint32_t c, uint64_t t) { return a.N < c ? ~0ull : ((sh_cdiv(a.N, 16 * c) * ((mt + m - 1) / m) + 255) / 256) * t; };
-    // A long chain of units over few columns: sixteen waves share it (by N and K alone, so that a row's bits do not depend on M). One
-    // row, groups of 64: 12248 x 700 14.0 us with eight, 10.6 with sixteen.
-    if (SU == 4 && a.K >= 2048 && a.N <= 2048) return launch_w4<1, 1, GS, SU, 16>(a, st);
+    // A long chain of units over few columns: sixteen waves share it (by N and K alone, so that a row's bits do not depend on M). With eight
+    // and with sixteen, 1, 16 and 64 rows: 12248 x 700 12.0 / 14.5 / 15.0 us against 10.3 / 15.5 / 15.9, 16384 x 256 11.5 / 18.6 / 18.9
+    // against 10.3 / 19.4 / 20.0: a row or few gain what the longer sum over the waves costs many. At 8192 x 1024 they gain less than
+    // that (7.0 / 11.0 / 11.1 against 6.6 / 12.2 / 12.4), at 4096 x 720 nothing (4.7 / 7.0 / 7.5 against 4.6 / 8.0 / 8.7), and more columns leave
+    // workgroups of sixteen waves that do not fit at once (64 rows, 16264 x 1055 20.9 against 36.4).
+    if constexpr (SU == 4)
+        if (a.K > 8192 && a.N <= 1024) return launch_w4<1, 1, GS, SU, 16>(a, st);
     const uint64_t c24 = mt > 1 ? cost(2, 4, 115) : ~0ull, c14 = cost(1, 4, 70), c12 = cost(1, 2, 52), c11 = cost(1, 1, 45);
     const uint64_t best = std::min(std::min(c24, c14), std::min(c12, c11));
     if (best == c11) return launch_w4<1, 1, GS, SU>(a, st);

@@ -134,3 +134,16 @@ def test_w4_rows_do_not_depend_on_each_other(lib, gpu):
     x[5] = np.nan
     z = _run(lib, x, *w, 128)
     assert np.isnan(z[5]).all() and np.array_equal(np.delete(z, 5, 0), np.delete(all_rows, 5, 0))
+
+
+@pytest.mark.parametrize("N,K,group", [(72, 8200, 128), (700, 12248, 64), (1024, 8192, 128), (1025, 8200, 128), (40, 16384, 32), (2048, 2048, 128)])
+def test_w4_long_chains_of_few_columns(lib, gpu, N, K, group):
+    """Either side of where sixteen waves share a chain: the product, and a row's bits alone and among others."""
+    rng = np.random.default_rng(N + K)
+    w = _weights(rng, K, N, group, True)
+    x = rng.standard_normal((35, K)).astype(np.float16)
+    all_rows = _run(lib, x, *w, group)
+    _check(all_rows, x, *w, group)
+    for m in (0, 33):
+        assert np.array_equal(_run(lib, x[m:m + 1], *w, group)[0], all_rows[m])
+    assert np.array_equal(_run(lib, x[:20], *w, group), all_rows[:20])
