@@ -702,6 +702,33 @@ def test_attention_slots_mostly_idle(lib, gpu, B, active):
     assert (np.abs(o - want) <= bound(want, reach, spread, dh, ld * bs, 127 * c.sc.max())).all()
 
 
+@pytest.mark.parametrize("window", [0, 200])
+def test_tokens_and_chunks_of_a_step_in_two_calls(lib, gpu, window):
+    """The requests of a step in two calls over the same rows: single tokens first, then the chunks, whose row_start begins behind them."""
+    import torch
+    rng = np.random.default_rng(47)
+    H, hkv, dh, bs, nd = 8, 2, 64, 16, 5
+    L, new = [300, 1, 77, 900, 16, 150, 400, 90], [1, 1, 1, 1, 1, 150, 33, 1]
+    start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    rows, D = int(start[-1]), H * dh
+    pages = sum(-(-n // bs) for n in L) + 1
+    c = Cache(rng, pages, hkv, dh, bs, FP8, values=True)
+    table = _table(rng, L, bs, pages)
+    ld, B = table.shape[1], len(L)
+    q = rng.standard_normal((rows, D)).astype(np.float16)
+    Q, T, Ln, Rs = to_dev(q), dev(table), dev(np.array(L, np.int32)), dev(start)
+    O = torch.full((rows, D), 7.0, dtype=torch.float16, device="cuda")
+    need = int(lib.sh_attention_kv_ws_bytes(C.byref(c.c), B, rows, max(new), H, ld))
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    for first, n, max_q in ((0, nd, 1), (nd, B - nd, max(new))):
+        rc = lib.sh_attention_kv(A(Q), A(O), C.byref(c.c), A(T, first * ld), ld, A(Ln, first), A(Rs, first), n, rows, max_q, H, D, D, 0.125, window, A(ws), need)
+        assert rc == 0, shops.last_error()
+        if first == 0:
+            assert (to_np(O)[nd:] == 7.0).all()
+    want, reach, spread = R.attention(q, *c.before(), table, L, start, H, 0.125, FP8, window)
+    assert (np.abs(to_np(O) - want) <= bound(want, reach, spread, dh, max(L), 448 * c.sc.max())).all()
+
+
 def test_attention_repeats_its_bits(lib, gpu):
     rng = np.random.default_rng(29)
     L = [5000, 40, 900]
