@@ -12,6 +12,17 @@ struct KvCache {
 // 0 and *out, or -1 with the message set.
 int sh_kv_check(const char *name, const sh_kv_cache *c, KvCache *out);
 
+// Sum of the lanes up to this one (v_add with DPP moves: shifts within rows of 16, then the rows' last lanes broadcast).
+__device__ __forceinline__ uint32_t kv_wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // The eight (four) bytes of two (one) words to fp16, exactly. INT8: with the sign bit flipped a byte u = code + 128 under
 // the high byte 0x64 is the half 1024 + u; minus 1152. FP8: the hardware's e4m3 conversion.
 template <bool FP8>

@@ -42,24 +42,14 @@ struct SlotArgs {
 };
 constexpr uint32_t OWN = 4;                // rows of a request up to which its thread writes them
 
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
-    return v;
-}
-
 // Inclusive sum over the workgroup, and its total; `part` holds one value a wave.
 template <int T>
 __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t *part, uint32_t &total) {
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    v = wave_scan(v);
+    v = kv_wave_scan(v);
     if (lane == 63) part[wave] = v;
     __syncthreads();
-    const uint32_t p = wave_scan(lane < T / 64 ? part[lane] : 0u);
+    const uint32_t p = kv_wave_scan(lane < T / 64 ? part[lane] : 0u);
     total = (uint32_t)__builtin_amdgcn_readlane((int)p, 63);
     return v + (wave ? (uint32_t)__builtin_amdgcn_readlane((int)p, (int)__builtin_amdgcn_readfirstlane(wave) - 1) : 0u);
 }

@@ -131,16 +131,6 @@ __device__ __forceinline__ void store4(uint16_t *p, float a, float b, float c, f
     *(sh_u2v_a2 *)p = (sh_u2v_a2){__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
 }
 
-// Sum of the lanes up to this one (v_add with DPP moves: shifts within rows of 16, then the rows' last lanes broadcast).
-__device__ __forceinline__ uint32_t wave_scan32(uint32_t v) {
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
-    return v;
-}
 __device__ __forceinline__ Seq lane_seq(const Seq &s, uint32_t b) {
     const auto rl = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)b); };
     return Seq{rl(s.r0), rl(s.n), rl(s.nf), rl(s.nqt), rl(s.ft), rl(s.nt), (int32_t)rl((uint32_t)s.L)};
@@ -178,7 +168,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     if constexpr (MANY) {
         uint32_t sum = 0;
         for (uint32_t i = tid; i < a.B; i += 64 * NW) { const Seq q = seq_of<QT>(a, i); sum += q.nt * q.nqt * c.hkv; }
-        sum = wave_scan32(sum);
+        sum = kv_wave_scan(sum);
         if (lane == 63) s_sum[wave] = sum;
         __syncthreads();
         for (uint32_t i = 0; i < NW; ++i) T += s_sum[i];
@@ -186,7 +176,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     } else {
         const uint32_t ix = a.wide ? tid : lane;
         if (ix < a.B) mine = seq_of<QT>(a, ix);
-        up = wave_scan32(mine.nt * mine.nqt * c.hkv);
+        up = kv_wave_scan(mine.nt * mine.nqt * c.hkv);
         T = at_lane(up, 63);
         if (a.wide) {
             if (lane == 63) s_sum[wave] = up;
@@ -234,7 +224,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
             const uint32_t i = b0 + tid;
             uint32_t w = 0;
             if (i < a.B) { const Seq q = seq_of<QT>(a, i); w = q.nt * q.nqt * c.hkv; }
-            uint32_t v = wave_scan32(w);
+            uint32_t v = kv_wave_scan(w);
             __syncthreads();
             if (lane == 63) s_sum[wave] = v;
             __syncthreads();
@@ -615,7 +605,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
             q = Seq{};
             if (b0 + lane < a.B) q = seq_of<CT>(a, b0 + lane);
         }
-        const uint32_t p = (q.nt + C - 1) / C, w = q.nqt * c.hkv * p, up = wave_scan32(w), cu = wave_scan32(p > 1 ? w : 0u);
+        const uint32_t p = (q.nt + C - 1) / C, w = q.nqt * c.hkv * p, up = kv_wave_scan(w), cu = kv_wave_scan(p > 1 ? w : 0u);
         const auto last = [](uint32_t v, uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
         const uint64_t hit = found ? 0 : __ballot(up > idx);
         if (hit) {
@@ -633,7 +623,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
         }
         if (!blockIdx.x) {
             const uint32_t z = base + up - w;
-            cuts += last(wave_scan32(p > 1 && z < gridDim.x ? min(w, gridDim.x - z) : 0u), 63);
+            cuts += last(kv_wave_scan(p > 1 && z < gridDim.x ? min(w, gridDim.x - z) : 0u), 63);
             base = min(base + last(up, 63), gridDim.x);
         }
     }
