@@ -316,7 +316,7 @@ extern "C" int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero,
             return -1;
         }
     }
-    W4Args a{(const uint16_t *)x, (const uint16_t *)scale, (const uint32_t *)w, (const uint8_t *)zero, (uint16_t *)z, M, N, K, (K + group - 1) / group, 0,
+    W4Args a{(const uint16_t *)x, (const uint16_t *)scale, (const uint32_t *)w, (const uint8_t *)zero, (uint16_t *)z, M, N, K, (K - 1) / group + 1, 0,
              ldx, ldw, lds, ldz, 0, nullptr, nullptr, 0, 0};
     if (epi) {
         a.bias = (const void *)epi->bias; a.bias_fp32 = epi->bias_fmt == SH_BIAS_FP32;
