@@ -368,8 +368,8 @@ int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uin
  * Scores, scale q k, stay within fp32. A row of q with an infinity or a NaN in a head gives NaN there wherever it sees a key.
  * max_q chooses the kernel for the whole call: single tokens beside chunks (max_q (H / hkv) > 64) are best a call of their own, over the same
  * rows: the requests of few rows first, then table, kv_len and row_start from the first chunk on (row_start's values stay as they are).
- * A probability is held to 22 bits where max_q (H / hkv) <= 8, with more rows in fp16: off by up to 2^-11 of it, so an output by up to 2^-11 of
- * sum p |v|, besides its own rounding.
+ * A probability is held to 22 bits where max_q (H / hkv) <= 8. With more rows it may be held in fp16: off by up to 2^-11 of it, so an output
+ * by up to 2^-11 of sum p |v|, besides its own rounding.
  * 0, -1 for bad arguments, -2 for too small a ws, SH_EHIP. Deterministic; how keys are shared out depends on the whole
  * batch, so a request's low bits may differ with its neighbours. */
 int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table, uint32_t ld_table, uint64_t kv_len, uint64_t row_start,

@@ -37,7 +37,7 @@ struct AttnArgs {
     uint16_t *o;
     const int32_t *table, *kv_len, *row_start;
     uint64_t ldq, ldo;
-    uint32_t ld, B, rows, max_q, grp, prow, window, groups, wide, whole, once;
+    uint32_t ld, B, rows, max_q, grp, prow, lq, window, groups, wide, whole, once;
     float sc;                              // scale x log2 e
     float *part, *ml;                      // partials [groups][2][prow][dh], their (max, sum) [groups][2][prow][2]
     ChunkUnit *unit;                       // [places]
@@ -51,8 +51,8 @@ struct Seq {
     int32_t L;
 };
 
-template <uint32_t QTILE>
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, uint32_t b) {
+// lq: log2 of a tile's rows.
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, uint32_t b, uint32_t lq) {
     Seq s;
     int32_t r0 = (int32_t)b, r1 = (int32_t)b + 1;
     if (a.row_start) { r0 = a.row_start[b]; r1 = a.row_start[b + 1]; }
@@ -61,7 +61,7 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, uint32_t b) {
     s.nf = r1 > r0 ? (uint32_t)(r1 - r0) : 0u;
     s.n = min(min(s.nf, a.max_q), s.r0 < a.rows ? a.rows - s.r0 : 0u);
     s.L = min(max(a.kv_len[b], 0), (int32_t)(a.ld << a.c.lbs));
-    s.nqt = (s.n * a.grp + QTILE - 1) / QTILE;
+    s.nqt = (s.n * a.grp + (1u << lq) - 1) >> lq;
     const int64_t lo = a.window ? max((int64_t)s.L - s.nf + 1 - a.window, (int64_t)0) : 0;
     s.ft = (uint32_t)lo / KT;
     s.nt = s.n ? max((uint32_t)(s.L + KT - 1) / KT, s.ft + 1) - s.ft : 0u;
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     if (lane < 2) s_seg[2 * wave + lane][0] = ~0u;                  // (only this wave writes these two until the barrier)
     if constexpr (MANY) {
         uint32_t sum = 0;
-        for (uint32_t i = tid; i < a.B; i += 64 * NW) { const Seq q = seq_of<QT>(a, i); sum += q.nt * q.nqt * c.hkv; }
+        for (uint32_t i = tid; i < a.B; i += 64 * NW) { const Seq q = seq_of(a, i, a.lq); sum += q.nt * q.nqt * c.hkv; }
         sum = kv_wave_scan(sum);
         if (lane == 63) s_sum[wave] = sum;
         __syncthreads();
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         __syncthreads();
     } else {
         const uint32_t ix = a.wide ? tid : lane;
-        if (ix < a.B) mine = seq_of<QT>(a, ix);
+        if (ix < a.B) mine = seq_of(a, ix, a.lq);
         up = kv_wave_scan(mine.nt * mine.nqt * c.hkv);
         T = at_lane(up, 63);
         if (a.wide) {
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         for (uint32_t b0 = 0; b0 < a.B; b0 += 64 * NW) {
             const uint32_t i = b0 + tid;
             uint32_t w = 0;
-            if (i < a.B) { const Seq q = seq_of<QT>(a, i); w = q.nt * q.nqt * c.hkv; }
+            if (i < a.B) { const Seq q = seq_of(a, i, a.lq); w = q.nt * q.nqt * c.hkv; }
             uint32_t v = kv_wave_scan(w);
             __syncthreads();
             if (lane == 63) s_sum[wave] = v;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     const auto take = [&](uint32_t i) {
         from = i;
         mine = Seq{};
-        if (i + lane < a.B) mine = seq_of<QT>(a, i + lane);
+        if (i + lane < a.B) mine = seq_of(a, i + lane, a.lq);
     };
     const auto get = [&](uint32_t i) {
         if constexpr (!MANY)
@@ -268,12 +268,11 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
     // Codes that the Infinity Cache (256 MB) will not hold until the next call are read without allocating (120 MB and up here, one row tile): 48 requests
     // of up to 16384 keys, 311 MB, 72.6 -> 68.0 us; what it holds would be lost by that: 8 requests of 1000 keys 13.0 -> 14.5 us.
     const bool stream = a.once && T * (uint64_t)(2 * KT * dh) >= (120u << 20);
-    // A probability's fp16 operand is off by up to 2^-11 of it, which shows where values cancel (a quarter more error in all). Where an item has
-    // at most half the tile's rows (most single tokens), columns 8 .. 15 are the same rows again, and their operand of the second
-    // product is what the rounding of the first eight's took off: the two columns' sum keeps 22 bits (48 requests of up to 16384 keys
-    // 60.0 -> 61.6 us, 937 keys 8.8 -> 9.15). More rows keep the one: a second product of their own took 48 requests to 70.0, four drafts of 24
-    // requests from 13.0 to 13.8.
-    const bool two = a.prow <= QT / 2;
+    // A probability's fp16 operand is off by up to 2^-11 of it, which shows where values cancel (a quarter more error in all). In items of
+    // eight rows columns 8 .. 15 are the same rows again, and their operand of the second product is what the rounding of the first
+    // eight's took off: the two columns' sum keeps 22 bits (48 requests of up to 16384 keys 60.1 -> 61.6 us, 937 keys 8.9 -> 9.4).
+    // Items of sixteen keep the one: a second product of their own took 48 requests to 70.0.
+    const bool two = a.lq == 3;
     const float rest = two && m >= QT / 2 ? 1.f : 0.f;
     const uint32_t kg = m >> 2, kr0 = m & 3;
     uint32_t kcol[NP];                                              // columns past the head's width: read as its first ones, against zeros of Q
@@ -283,11 +282,11 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
         const uint32_t h = item / s.nqt, qt = item - h * s.nqt;
         const uint32_t j1 = min(s.nt, j0 + (t1 - t));
         // ---- rows
-        const uint32_t r = qt * QT + (two ? m & 7 : m), nrow = s.n * a.grp;
+        const uint32_t q0 = qt << a.lq, r = q0 + (two ? m & 7 : m), nrow = s.n * a.grp;
         const uint32_t qi = r / a.grp, qh = h * a.grp + (r - qi * a.grp);
         const int32_t first = s.L - (int32_t)s.nf;                                      // position of the request's first row
         const int32_t pos = r < nrow ? first + (int32_t)qi : -1;
-        const int32_t pmin = first + (int32_t)(qt * QT / a.grp), pmax = first + (int32_t)((min(qt * QT + QT, nrow) - 1) / a.grp);
+        const int32_t pmin = first + (int32_t)(q0 / a.grp), pmax = first + (int32_t)((min(q0 + (1u << a.lq), nrow) - 1) / a.grp);
         const int32_t slo = a.window ? max(max(pmin, 0) - (int32_t)a.window + 1, 0) : 0;        // keys that any row sees: slo .. pmax
         // ---- key tiles that any row sees
         const uint32_t ja = max(j0, (uint32_t)slo / KT - s.ft), jb = pmax < 0 ? 0u : min(j1, (uint32_t)pmax / KT + 1 - s.ft);
@@ -443,7 +442,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attn(AttnArgs a) {
             }
             if (lane == 0) {
                 s_seg[sg][0] = b; s_seg[sg][1] = item; s_seg[sg][2] = j0; s_seg[sg][3] = j1; s_seg[sg][4] = s.nt;
-                s_seg[sg][5] = qt * QT; s_seg[sg][6] = nrow; s_seg[sg][7] = h; s_seg[sg][8] = s.r0;
+                s_seg[sg][5] = q0; s_seg[sg][6] = nrow; s_seg[sg][7] = h; s_seg[sg][8] = s.r0;
             }
         }
         t += j1 - j0;
@@ -572,7 +571,7 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
 // at the table's width: their parts go to as many places of `part`, which k_kv_chunk_join adds up. The launch has enough blocks, and
 // `part` enough places, while row_start does not decrease; where it does (an error of the caller's), the units behind the last block
 // or place do not exist, and an item that lacks parts for that is not joined.
-constexpr uint32_t CT = 128;               // rows of a unit
+constexpr uint32_t LCT = 7, CT = 1u << LCT;  // rows of a unit
 constexpr uint32_t CUT = 768;              // units that share the whole evenly: three workgroups a CU, two of them at a time
 constexpr uint32_t CUT_MIN = 8;            // tiles of a part at least
 template <int DP, bool FP8>
@@ -591,7 +590,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
     Seq q{};
     for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
         q = Seq{};
-        if (b0 + lane < a.B) q = seq_of<CT>(a, b0 + lane);
+        if (b0 + lane < a.B) q = seq_of(a, b0 + lane, LCT);
         all += (uint64_t)q.nt * q.nqt * c.hkv;
     }
     all = wave_sum64(all);
@@ -603,7 +602,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_kv_chunk(AttnArgs a)
     for (uint32_t b0 = 0; b0 < a.B; b0 += 64) {
         if (a.B > 64) {
             q = Seq{};
-            if (b0 + lane < a.B) q = seq_of<CT>(a, b0 + lane);
+            if (b0 + lane < a.B) q = seq_of(a, b0 + lane, LCT);
         }
         const uint32_t p = (q.nt + C - 1) / C, w = q.nqt * c.hkv * p, up = kv_wave_scan(w), cu = kv_wave_scan(p > 1 ? w : 0u);
         const auto last = [](uint32_t v, uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
@@ -883,11 +882,19 @@ bool launch_attn_many(const AttnArgs &a, hipStream_t st) {
 }
 template <int DP, int DH, bool FP8, int NW>
 bool launch_attn(AttnArgs a, uint32_t tiles, hipStream_t st) {
+    const uint64_t rows = (uint64_t)a.max_q * a.grp;
     a.groups = GROUPS;
+    a.lq = rows <= QT / 2 ? 3 : 4;
     if (a.B > 64 * NW) return launch_attn_many<DP, 0, FP8, NW, true>(a, st);
     a.wide = a.B > 64;
     a.whole = tiles <= WHOLE_TILES * NW;
-    a.once = (uint64_t)a.max_q * a.grp <= QT;
+    a.once = rows <= QT;
+    // Nine rows and more in items of eight, for the precision of those, where that does not make more of them than workgroups (24 requests of
+    // four drafts, 16 heads over 4: 13.2 us against 13.5): more would read keys twice that one item of sixteen reads once.
+    if (a.whole && (uint64_t)a.B * a.c.hkv * ((rows + 7) / 8) <= GROUPS) {
+        a.lq = 3;
+        a.prow = std::min(a.prow, QT / 2);
+    }
     return launch_attn_many<DP, DH, FP8, NW, false>(a, st);
 }
 template <bool FP8>

@@ -428,7 +428,7 @@ def test_attention_scales_far_apart(lib, gpu, fmt):
 
 
 @pytest.mark.parametrize("fmt", [INT8, FP8])
-@pytest.mark.parametrize("H,hkv,dh", [(4, 2, 32), (15, 5, 64), (4, 4, 80), (7, 1, 112), (8, 1, 128), (2, 1, 256)])
+@pytest.mark.parametrize("H,hkv,dh", [(4, 2, 32), (15, 5, 64), (4, 4, 80), (7, 1, 112), (8, 1, 128), (2, 1, 256), (16, 1, 64), (24, 2, 80)])
 def test_attention_probabilities_keep_their_precision(lib, gpu, fmt, H, hkv, dh):
     """Values of +-1 by turns and nearly equal scores: outputs near 0 whose terms are not, so that a probability held in fp16 (off by
     up to 2^-11 of it) shows. The bound: the result's rounding; scores as in `bound`; 2^-19 for a page's log2 weight (one step of
