@@ -14,8 +14,9 @@
 // could leave the range, so they are held as p x vs x cn, cn a power of two that brings the largest value scale
 // met so far to 2^14 (smaller ones keep their precision until 2^-28 of it); the accumulators are brought along where cn changes.
 //
-// Single tokens are bound by HBM once the keys are many (two requests of 131 thousand keys, 516 MB: 89 us, 5.8 TB/s) and by latency
-// below (one request of 937 keys 8.8 us): the lengths, a page, its codes, the join, one after the other.
+// Single tokens are bound by HBM once the keys are many (two requests of 131 thousand keys, 516 MB: 90 us, 5.7 TB/s) and by latency
+// below: the lengths, a page, its codes, the join, one after the other (one request of 937 keys 9.4 us; in a table of 128 pages and more, where
+// items are cut and joined by a second launch, 11.2).
 #include "sh_kv.h"
 #include <algorithm>
 #include <type_traits>
@@ -561,10 +562,11 @@ __global__ __launch_bounds__(256) void k_kv_join(AttnArgs a) {
 // buffers, the codes after the next in flight. S^T and O^T on v_mfma_f32_32x32x16_f16. As above no operand moves between
 // lanes: row m of a score tile's A operand is key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that the lane (n, hi) gets
 // the scores of keys 16 q + 8 hi + 0 .. 7 of row n, which is the second product's operand.
-// Bound by the vector pipe: for 64 keys by 32 rows a wave issues 32 matrix instructions (1024 cycles of their pipe) beside ~380 vector
-// issues (1520 cycles): a multiply-add, an exponential (four issues) and an addition a score, half a maximum and half a
-// conversion, and the codes of its share. Measured: 512 rows each of four requests of 8000 keys, 32 heads over 8, 395 us, 700 TFLOP/s; 4096
-// rows of one prompt 218 us, 630 TFLOP/s; LDS reads (32 KB a wave and tile) come next.
+// Bound by no one pipe: 512 rows each of four requests of 8000 keys, 32 heads over 8, take 370 us (700 TFLOP/s), of which the vector pipe
+// is busy half (a multiply-add, an exponential and an addition a score, half a maximum, half a conversion, the codes of its share), the
+// matrix pipe 31 % (32 instructions for 64 keys by 32 rows), LDS 30 % (32 KB read a wave and tile). One comes after the other: two waves a SIMD,
+// 1.7 on average, and a barrier a tile overlap them little, and of its time a wave waits 25 % for data and barriers and 27 % to
+// issue. 4096 rows of one prompt 220 us, 620 TFLOP/s.
 // The keys of an item are cut into parts of C tiles, C a 768th of all tiles (and at least 8): one long request among short ones, or a
 // few rows over a long context, then keep every CU busy. Units are dealt out by the hardware, the request's last row tiles first
 // (they see most). A request that is cut has more than C tiles, so cut units number at most 2 T / C <= 1536, and no more than all units cut
