@@ -98,8 +98,8 @@ def _draw(rng) -> dict:
     if kind == "quant":
         cols = rng.choice([_log(rng, 1, 16384), 32 * _log(rng, 1, 512)])
         return dict(kind=kind, rows=_log(rng, 1, 8192), cols=cols, ldx=cols + rng.choice([0, 0, 1, 8, cols]))
-    M = rng.choice([1, _log(rng, 1, 64), _log(rng, 1, 64), _log(rng, 64, 8192), _log(rng, 64, 8192)])
-    return dict(kind=kind, f16=M <= 64 and rng.random() < 0.5, M=M, N=_log(rng, 16, 16384), K=rng.choice([_log(rng, 16, 16384), 32 * _log(rng, 1, 512)]),
+    M = rng.choice([1, _log(rng, 1, 16), _log(rng, 2, 64), _log(rng, 64, 8192), _log(rng, 64, 8192)])
+    return dict(kind=kind, f16=M <= 16 and rng.random() < 0.5, M=M, N=_log(rng, 16, 16384), K=rng.choice([_log(rng, 16, 16384), 32 * _log(rng, 1, 512)]),
                 bias=rng.random() < 0.5, gelu=rng.random() < 0.3, residual=rng.random() < 0.5)
 
 
