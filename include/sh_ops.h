@@ -377,6 +377,43 @@ int sh_attention_kv(uint64_t q, uint64_t o, const sh_kv_cache *c, uint64_t table
                     uint64_t ws, uint64_t ws_bytes);
 uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t rows, uint32_t max_q, uint32_t H, uint32_t ld_table);
 
+/* ---- rotary positions (no counterpart in the reference but sh_rope's formula) ---------------------------------------
+ * The first `rot` columns of a head are turned in pairs by an angle that grows with the row's position: pair i by a =
+ * 2 pi position step[i] / 2^64 (whole turns fall off), (x1, x2) -> (x1 c - x2 s, x2 c + x1 s) with c, s = mscale (cos a, sin a); the other
+ * columns stay. Cosine and sine are rounded to fp32 from 64 bits, products and sums to fp32, the result to fp16, so no position is too far. */
+enum { SH_ROPE_HALF = 0,      /* pair i: columns i and i + rot / 2 */
+       SH_ROPE_PAIRS = 1 };   /* pair i: columns 2 i and 2 i + 1 */
+enum { SH_ROPE_NONE = 0, SH_ROPE_LINEAR = 1, SH_ROPE_BANDS = 2, SH_ROPE_RAMP = 3 };
+typedef struct {
+    uint64_t step;        /* uint64 [rot / 2] in GPU memory, 8-byte aligned: turns per position x 2^64, of sh_rope_steps or the caller's */
+    uint32_t rot;         /* turned columns of a head: even, 2 .. the head's width */
+    uint32_t layout;      /* SH_ROPE_HALF | SH_ROPE_PAIRS */
+    float mscale;         /* 1: cosine and sine as they are */
+    uint32_t reserved;    /* 0 */
+} sh_rope_plan;
+
+/* The steps of a model, once: w_i = base^(-2 i / rot) radians a position (base > 1), for contexts `factor` times longer than the
+ * first one of `ctx` positions brought to w_i (keep + (1 - keep) / factor), where keep is
+ *   SH_ROPE_NONE    1 (factor, lo, hi, ctx are not read)
+ *   SH_ROPE_LINEAR  0: every position counts 1 / factor
+ *   SH_ROPE_BANDS   by the pair's turns n = ctx w_i / (2 pi) in the first context: 0 for n <= lo, 1 for n >= hi, linear in n between
+ *   SH_ROPE_RAMP    by its index: 1 up to the index (rounded down, at least 0) whose pair turns hi times in it, 0 from that (rounded up, at most
+ *                   rot - 1) of lo turns, linear in the index between
+ * 0, -1 for bad arguments (0 < lo < hi), SH_EHIP. */
+int sh_rope_steps(uint64_t step, uint32_t rot, double base, uint32_t scaling, double factor, double lo, double hi, uint32_t ctx);
+
+/* `heads` heads of dh columns (dh even) of each row, turned by pos[row] (int32): y = the turned x (fp16, leading dims ldy / ldx). A row with a
+ * negative position is left as it is in y. y is x (with the same leading dim: in place) or does not overlap it. Query and key heads that lie
+ * side by side in a projection's rows are one call. 0, -1, SH_EHIP. */
+int sh_rope_pos(uint64_t y, uint64_t x, uint64_t pos, const sh_rope_plan *p, uint32_t rows, uint32_t heads, uint32_t dh, uint32_t ldy, uint32_t ldx);
+
+/* sh_kv_append of keys turned on the way, the values as they are, and the step's queries turned into yq (H heads; 0: none; yq as y of
+ * sh_rope_pos), in one launch: the bits of sh_rope_pos on q and k, then sh_kv_append. rot a multiple of 8. A row with a negative position
+ * counts as one with a slot outside the cache, and its queries are left as they are in yq; the queries of other rows with such a slot are turned. yq does not
+ * overlap k or v. 0, -1, SH_EHIP. */
+int sh_kv_append_rope(const sh_kv_cache *c, const sh_rope_plan *p, uint64_t yq, uint64_t q, uint64_t k, uint64_t v, uint64_t pos, uint64_t slots, uint32_t rows,
+                      uint32_t H, uint32_t ldyq, uint32_t ldq, uint32_t ldk, uint32_t ldv);
+
 /* Few rows times a weight of 4-bit codes (no counterpart in the reference): z = act(x . W + bias) rounded to fp16, then
  * [+ residual, rounded again], W[k][n] = (code[k][n] - zero[k / group][n]) scale[k / group][n]. w: words [K / 8][N]
  * (uint32, leading dim ldw), bits 4 j .. 4 j + 3 of word (i, n) the code of k = 8 i + j. scale: fp16 [ceil(K / group)][N],
@@ -388,6 +425,29 @@ uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t row
  * an fp16 weight. */
 int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero, uint64_t z, uint32_t M, uint32_t N, uint32_t K, uint32_t group,
                uint32_t ldx, uint32_t ldw, uint32_t lds, uint32_t ldz, const sh_gemm_epi *epi);
+
+/* ---- microscaled 4-bit floating point (no counterpart in the reference) -----------------------------------------------
+ * A row of K numbers as codes and scales, both operands of a product alike (a weight W [K, N] as the N rows of W^T): codes of e2m1 (sign,
+ * 2 bits of exponent, 1 of fraction: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two to a byte, the lower k in the low four bits, 16 bytes for each
+ * block of 32 k; a scale byte e for each block, 2^(e - 127), 255: NaN. Codes: 16-byte aligned, leading dim in bytes a multiple of 16, at least 16
+ * ceil(K / 32). Scales: 4-byte aligned, leading dim in bytes a multiple of 4, at least ceil(K / 32). */
+
+/* Rows x (fp16 [rows][cols], leading dim ldx) as codes and scales. The scale of a block is the smallest power of two s >= 2^-32 with |x| <= 6 s; codes
+ * are nearest, ties to even; a block with a NaN or an infinity has scale 255 and codes of 0. Codes behind `cols` in the last block are 0; bytes
+ * behind the last block and the last scale are left as they are. 0, -1, SH_EHIP. */
+int sh_mx4_quant(uint64_t codes, uint64_t scales, uint64_t x, uint32_t rows, uint32_t cols, uint32_t ldc, uint32_t lds, uint32_t ldx);
+
+/* z = act(x . W + bias) rounded to fp16, then [+ residual, rounded again], of rows in 4 bits: xc, xs [M], wc, ws [N] (the rows of W^T). fp32
+ * sums of exact products. Codes behind K in the last block count where both operands' are not 0 (sh_mx4_quant's are 0); scale bytes behind the last block are
+ * not used. A row of x or W with a scale of 255 gives NaN. epi: bias, act, residual as sh_gemm_ex (splits 0 or 1, no LayerNorm
+ * fold, no row partials). M, N <= 2^26. 0, -1 for bad arguments, SH_EHIP. Deterministic; which kernel runs depends on M, so a row's low bits may. */
+int sh_gemm_mx4(uint64_t xc, uint64_t xs, uint64_t wc, uint64_t ws, uint64_t z, uint32_t M, uint32_t N, uint32_t K,
+                uint32_t ldxc, uint32_t ldxs, uint32_t ldwc, uint32_t ldws, uint32_t ldz, const sh_gemm_epi *epi);
+
+/* The same for up to 16 rows x of fp16 [M][K] (leading dim ldx), brought into 4 bits on the way as sh_mx4_quant does: one launch for single tokens,
+ * and the bits of the two calls. */
+int sh_gemm_mx4_f16(uint64_t x, uint64_t wc, uint64_t ws, uint64_t z, uint32_t M, uint32_t N, uint32_t K,
+                    uint32_t ldx, uint32_t ldwc, uint32_t ldws, uint32_t ldz, const sh_gemm_epi *epi);
 
 /* LayerNorm with separate input / output leading dims (fused residual stream layouts). */
 void sh_layernorm_ld(uint64_t y, uint64_t x, uint64_t gamma, uint64_t beta, uint32_t rows, uint32_t cols,

@@ -77,6 +77,10 @@ __device__ __forceinline__ sh_h2 sh_gelu_h2(sh_h2 x) {
 __device__ __forceinline__ uint32_t sh_gelu_u32(uint32_t pair) {   // two fp16 codes in a 32-bit word
     return __builtin_bit_cast(uint32_t, sh_gelu_h2(__builtin_bit_cast(sh_h2, pair)));
 }
+// The same form in fp32 throughout (the products with 4-bit weights).
+__device__ __forceinline__ float sh_gelu_f32(float x) {
+    return x * sh_fast_rcp(1.f + sh_fast_exp2(x * fmaf(SH_GELU_K1 * x, x, SH_GELU_K0)));
+}
 
 // Reduction over groups of W consecutive lanes (W = 8 to 64, whole groups active), the result in every lane: the butterfly
 // over lanes l ^ W/2, ..., l ^ 1. A row operator's two reductions lie between its loads and its store, so their latency

@@ -80,10 +80,6 @@ __device__ __forceinline__ XPairs x_pairs(uint4 v) {
                   __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
 }
 
-__device__ __forceinline__ float gelu(float x) {          // x / (1 + 2^{x (k0 + k1 x^2)}), fp32
-    return x * sh_fast_rcp(1.f + sh_fast_exp2(x * fmaf(SH_GELU_K1 * x, x, SH_GELU_K0)));
-}
-
 // A workgroup of NW waves: 16 CW columns (lane n has CW consecutive ones), 16 MT rows; wave i takes the units (SU
 // steps of 32 k) i, i + NW, ..., the next one's words in flight while it multiplies; the waves' sums are added in LDS in wave order. Every
 // GS steps of a unit the sums are scaled: GS = 4, 2, 1 for groups that are multiples of 128, 64, 32. Columns and octets past the end
@@ -238,7 +234,7 @@ __global__ __launch_bounds__(64 * NW) void k_w4(W4Args a) {
 #pragma unroll
         for (int k = 0; k < NW; ++k) v += s_z[(k * nrow + r) * LC + c];
         if (a.bias) v += a.bias_fp32 ? ((const float *)a.bias)[nn] : sh_dev_h2f(((const uint16_t *)a.bias)[nn]);
-        if (a.act == SH_ACT_GELU) v = gelu(v);
+        if (a.act == SH_ACT_GELU) v = sh_gelu_f32(v);
         uint16_t hz = sh_dev_f2h_rr(v);
         if (a.res) hz = sh_dev_f2h_rr(sh_dev_h2f(hz) + sh_dev_h2f(a.res[m * a.ldr + nn]));
         a.z[m * a.ldz + nn] = hz;

@@ -1,6 +1,7 @@
 // The 8-bit paged key / value cache: block tables and slots of a step (sh_kv_slots) and the write of new rows
-// (sh_kv_append). The attention over it is in sh_kv_attention.hip.
+// (sh_kv_append, and sh_kv_append_rope for keys that are turned by their positions). The attention over it is in sh_kv_attention.hip.
 #include "sh_kv.h"
+#include "sh_rope.h"
 #include <algorithm>
 
 int sh_kv_check(const char *name, const sh_kv_cache *c, KvCache *out) {
@@ -209,6 +210,117 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
         return codes4<FP8>((float)(int8_t)w * ratio, (float)(int8_t)(w >> 8) * ratio, (float)(int8_t)(w >> 16) * ratio, (float)(int8_t)(w >> 24) * ratio);
 }
 
+// One page's new rows: first row, page, offsets [off, end).
+struct AppendRun { uint32_t r, page, off, end; };
+
+// What a thread holds of a page: four tokens from t0 by eight columns, four of them from ca and four from cb (SPLIT), or all from ca. `items`
+// threads hold something. Finds the scale, rounds older tokens again where it grew, and stores the codes.
+template <bool FP8, int NT, bool SPLIT>
+__device__ __forceinline__ void append_page(const KvCache &c, uint32_t isv, uint32_t h, const AppendRun &u, uint32_t blk0, uint32_t t0, uint32_t ca, uint32_t cb,
+                                            bool mine, uint4 (&x)[4], uint32_t *s_top) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, dh = c.dh, off = u.off, end = u.end;
+    uint8_t *dst = (isv ? c.v + u.page * c.pgv : c.k + u.page * c.pgk) + (uint64_t)h * c.bs * dh;
+    float *sp = (isv ? c.vs : c.ks) + (uint64_t)u.page * c.pgs + h;
+    const float was = off ? *sp : 0.f;
+    // the largest |x| as an integer (halves without their sign are ordered like their bits); only if a NaN or an infinity is
+    // among them are these put right, and it is taken again
+    uint32_t top;
+    for (;;) {
+        us2 t = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            t = __builtin_elementwise_max(t, __builtin_elementwise_max(bits2(x[j].x), bits2(x[j].y)));
+            t = __builtin_elementwise_max(t, __builtin_elementwise_max(bits2(x[j].z), bits2(x[j].w)));
+        }
+        top = (uint32_t)sh_wave_max((float)max(t.x, t.y));      // (exact)
+        if constexpr (NT > 64) {
+            __syncthreads();                                    // the last maxima are read
+            if (lane == 0) s_top[tid / 64] = top;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NT / 64; ++i) top = max(top, s_top[i]);
+        }
+        top = __builtin_amdgcn_readfirstlane(top);
+        if (top < 0x7C00u) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = make_uint4(clean2(x[j].x), clean2(x[j].y), clean2(x[j].z), clean2(x[j].w));
+    }
+    const float s = fmaxf(was, pow2_scale<FP8>(sh_dev_h2f((uint16_t)top)));
+    if (off && s != was) {                                      // the page's older tokens: whole words, and the bytes beside the new ones
+        const float ratio = was / s;
+        uint32_t *d32 = (uint32_t *)dst;
+        if (!isv) {
+            for (uint32_t i = tid; i < off * dh / 4; i += NT) d32[i] = rescale4<FP8>(d32[i], ratio);
+        } else {
+            for (uint32_t i = tid; i < blk0 * dh; i += NT) {
+                uint32_t *p = d32 + (i / blk0) * (c.bs / 4) + i % blk0;
+                *p = rescale4<FP8>(*p, ratio);
+            }
+            for (uint32_t i = tid; i < (off & 3) * dh; i += NT) {
+                uint8_t *p = dst + (i % dh) * c.bs + 4 * blk0 + i / dh;
+                *p = (uint8_t)rescale4<FP8>(*p, ratio);
+            }
+        }
+    }
+    const bool p2 = !(__builtin_amdgcn_readfirstlane(__float_as_uint(s)) & 0x7FFFFFu);      // (only a caller's own scales are not)
+    const float inv = 1.f / s;
+    if (mine) {
+        float v[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = sh_dev_h2f((uint16_t)(w[e / 2] >> (16 * (e & 1))));
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            // the product, and what it lacks for the correctly rounded quotient (Markstein, "Computation of elementary functions on
+            // the IBM RISC System/6000 processor", 1990): nothing where s is a power of two
+            const float f = v[j / 8][j % 8], q = f * inv;
+            v[j / 8][j % 8] = p2 ? q : fmaf(fmaf(-q, s, f), inv, q);
+        }
+        if (!isv) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t t = t0 + j;
+                if (t >= off && t < end) {
+                    const uint32_t lo = codes4<FP8>(v[j][0], v[j][1], v[j][2], v[j][3]), hi = codes4<FP8>(v[j][4], v[j][5], v[j][6], v[j][7]);
+                    if constexpr (SPLIT) {
+                        *(uint32_t *)(dst + t * dh + ca) = lo;
+                        *(uint32_t *)(dst + t * dh + cb) = hi;
+                    } else *(uint2 *)(dst + t * dh + ca) = make_uint2(lo, hi);
+                }
+            }
+        } else {
+            const bool whole = t0 >= off && t0 + 4 <= end;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                uint8_t *p = dst + (ca + e) * c.bs + t0;
+                const uint32_t w = codes4<FP8>(v[0][e], v[1][e], v[2][e], v[3][e]);
+                if (whole) *(uint32_t *)p = w;
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (t0 + j >= off && t0 + j < end) p[j] = (uint8_t)(w >> (8 * j));
+            }
+        }
+    }
+    if (tid == 0) *sp = s;
+}
+
+// The next page of a workgroup's rows r0 ... (lane i: row r0 + i): its first row is lane f, its rows are among those read, or are read
+// again (`slot`: a row's slot).
+template <typename Slot>
+__device__ __forceinline__ AppendRun append_run(const KvCache &c, uint32_t rows, uint32_t r0, uint32_t f, uint32_t sl, Slot slot) {
+    const uint32_t lane = threadIdx.x & 63, r = r0 + f;
+    const uint32_t s0 = (uint32_t)__builtin_amdgcn_readlane((int)sl, (int)f), off = s0 & (c.bs - 1);
+    uint64_t has;                                                    // the run's rows, a page's rest of at most 64
+    if (f + c.bs - off <= 64) has = __ballot(lane >= f && lane - f < c.bs - off && sl == s0 + lane - f) >> f;
+    else has = __ballot(lane < c.bs - off && r + lane < rows && slot(min(r + lane, rows - 1)) == s0 + lane);
+    const uint32_t n = ~has ? (uint32_t)__builtin_ctzll(~has) : 64u;
+    return AppendRun{r, s0 >> c.lbs, off, off + n};
+}
+
 // A workgroup takes RG rows, one head and keys or values, and does the pages whose first new row is among its rows, one after
 // the other. A thread holds four tokens by eight columns of the page (one such item), the tokens at the page's own multiples of
 // four: four 16-byte loads; after the page's largest value is known, the codes of a key's eight columns are one 8-byte store a
@@ -229,106 +341,94 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
     uint64_t lead = __ballot(lane < a.rg && sl < cap && (!(sl & (c.bs - 1)) || !rl || sb != sl - 1));
     const uint64_t ld = isv ? a.ldv : a.ldk;
     while (lead) {
-        const uint32_t f = __builtin_ctzll(lead), r = r0 + f;
+        const uint32_t f = __builtin_ctzll(lead);
         lead &= lead - 1;
-        const uint32_t s0 = (uint32_t)__builtin_amdgcn_readlane((int)sl, (int)f), off = s0 & (c.bs - 1), page = s0 >> c.lbs;
-        // the run's rows, a page's rest of at most 64: among the rows read, or read again
-        uint64_t has;
-        if (f + c.bs - off <= 64) has = __ballot(lane >= f && lane - f < c.bs - off && sl == s0 + lane - f) >> f;
-        else has = __ballot(lane < c.bs - off && r + lane < a.rows && (uint32_t)a.slots[min(r + lane, a.rows - 1)] == s0 + lane);
-        const uint32_t n = ~has ? (uint32_t)__builtin_ctzll(~has) : 64u, end = off + n;
-        const uint16_t *src = (isv ? a.v : a.k) + (uint64_t)r * ld + (uint64_t)h * dh;
-        uint8_t *dst = (isv ? c.v + page * c.pgv : c.k + page * c.pgk) + (uint64_t)h * c.bs * dh;
-        float *sp = (isv ? c.vs : c.ks) + (uint64_t)page * c.pgs + h;
-        const float was = off ? *sp : 0.f;
-        const uint32_t blk0 = off / 4, items = ((end + 3) / 4 - blk0) * nch;
+        const AppendRun u = append_run(c, a.rows, r0, f, sl, [&](uint32_t r) { return (uint32_t)a.slots[r]; });
+        const uint16_t *src = (isv ? a.v : a.k) + (uint64_t)u.r * ld + (uint64_t)h * dh;
         uint4 x[4];
+        const uint32_t blk0 = u.off / 4, items = ((u.end + 3) / 4 - blk0) * nch;
         const uint32_t bl = sh_div(tid, a.dch), ch = tid - bl * nch, t0 = 4 * (blk0 + bl);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t t = t0 + j;
             x[j] = make_uint4(0, 0, 0, 0);
-            if (tid < items && t >= off && t < end) x[j] = sh_ld16_any(src + (uint64_t)(t - off) * ld + 8 * ch);
+            if (tid < items && t >= u.off && t < u.end) x[j] = sh_ld16_any(src + (uint64_t)(t - u.off) * ld + 8 * ch);
         }
-        // the largest |x| as an integer (halves without their sign are ordered like their bits); only if a NaN or an infinity is
-        // among them are these put right, and it is taken again
-        uint32_t top;
-        for (;;) {
-            us2 t = {0, 0};
+        append_page<FP8, NT, false>(c, isv, h, u, blk0, t0, 8 * ch, 0, tid < items, x, s_top);
+    }
+}
+
+// ---- sh_kv_append_rope ----------------------------------------------------------------------------------------------
+// The same with keys turned by their rows' positions before they are codes, and the queries' heads turned in the launch's last
+// workgroups. A thread's eight columns of a key are four pairs of each of its four tokens, and it keeps their cosines and sines for `kh` heads:
+// they cost more than all else here (fp64, about 180 cycles a wave each).
+struct AppendRopeArgs {
+    AppendArgs a;
+    RopeArgs q;                            // rows turned for themselves
+    uint32_t kh, kg, blocks;               // heads of a workgroup of keys, such workgroups of a group of rows, workgroups that append
+};
+
+template <bool FP8, int NT>
+__global__ __launch_bounds__(NT) void k_kv_append_rope(AppendRopeArgs g) {
+    __shared__ uint32_t s_top[NT / 64];
+    if (blockIdx.x >= g.blocks) {
+        rope_rows<4>(g.q, (blockIdx.x - g.blocks) * NT + threadIdx.x);
+        return;
+    }
+    const AppendArgs &a = g.a;
+    const KvCache &c = a.c;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, gr = sh_div(blockIdx.x, a.dheads), hv = blockIdx.x - gr * a.dheads.d, r0 = a.row0 + gr * a.rg;
+    const uint32_t isv = hv >= g.kg, h0 = isv ? hv - g.kg : hv * g.kh, h1 = isv ? h0 + 1 : min(h0 + g.kh, c.hkv);
+    const uint32_t cap = c.pages << c.lbs, dh = c.dh, nch = dh / 8;
+    const auto slot = [&](uint32_t r) { return g.q.pos[r] < 0 ? ~0u : (uint32_t)a.slots[r]; };
+    const uint32_t rl = r0 + lane;
+    const uint32_t sl = rl < a.rows ? slot(rl) : ~0u;
+    const uint32_t sb = rl < a.rows && rl ? slot(rl - 1) : ~0u;
+    uint64_t lead = __ballot(lane < a.rg && sl < cap && (!(sl & (c.bs - 1)) || !rl || sb != sl - 1));
+    const uint64_t ld = isv ? a.ldv : a.ldk;
+    while (lead) {
+        const uint32_t f = __builtin_ctzll(lead);
+        lead &= lead - 1;
+        const AppendRun u = append_run(c, a.rows, r0, f, sl, slot);
+        const uint16_t *src = (isv ? a.v : a.k) + (uint64_t)u.r * ld + (uint64_t)h0 * dh;
+        const uint32_t blk0 = u.off / 4, items = ((u.end + 3) / 4 - blk0) * nch;
+        const uint32_t bl = sh_div(tid, a.dch), ch = tid - bl * nch, t0 = 4 * (blk0 + bl);
+        const bool mine = tid < items;
+        if (isv) {
+            uint4 x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                t = __builtin_elementwise_max(t, __builtin_elementwise_max(bits2(x[j].x), bits2(x[j].y)));
-                t = __builtin_elementwise_max(t, __builtin_elementwise_max(bits2(x[j].z), bits2(x[j].w)));
+                const uint32_t t = t0 + j;
+                x[j] = make_uint4(0, 0, 0, 0);
+                if (mine && t >= u.off && t < u.end) x[j] = sh_ld16_any(src + (uint64_t)(t - u.off) * ld + 8 * ch);
             }
-            top = (uint32_t)sh_wave_max((float)max(t.x, t.y));      // (exact)
-            if constexpr (NT > 64) {
-                __syncthreads();                                    // the last maxima are read
-                if (lane == 0) s_top[tid / 64] = top;
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < NT / 64; ++i) top = max(top, s_top[i]);
-            }
-            top = __builtin_amdgcn_readfirstlane(top);
-            if (top < 0x7C00u) break;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = make_uint4(clean2(x[j].x), clean2(x[j].y), clean2(x[j].z), clean2(x[j].w));
+            append_page<FP8, NT, false>(c, 1, h0, u, blk0, t0, 8 * ch, 0, mine, x, s_top);
+            continue;
         }
-        const float s = fmaxf(was, pow2_scale<FP8>(sh_dev_h2f((uint16_t)top)));
-        if (off && s != was) {                                      // the page's older tokens: whole words, and the bytes beside the new ones
-            const float ratio = was / s;
-            uint32_t *d32 = (uint32_t *)dst;
-            if (!isv) {
-                for (uint32_t i = tid; i < off * dh / 4; i += NT) d32[i] = rescale4<FP8>(d32[i], ratio);
-            } else {
-                for (uint32_t i = tid; i < blk0 * dh; i += NT) {
-                    uint32_t *p = d32 + (i / blk0) * (c.bs / 4) + i % blk0;
-                    *p = rescale4<FP8>(*p, ratio);
-                }
-                for (uint32_t i = tid; i < (off & 3) * dh; i += NT) {
-                    uint8_t *p = dst + (i % dh) * c.bs + 4 * blk0 + i / dh;
-                    *p = (uint8_t)rescale4<FP8>(*p, ratio);
-                }
-            }
+        uint32_t ca, cb;
+        rope_columns<4>(g.q.p, ch, ca, cb);
+        const bool turned = ch < g.q.p.rot / 8;
+        float cs[4][4], sn[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t t = t0 + j;
+            if (mine && turned && t >= u.off && t < u.end) rope_angles<4>(g.q.p, ch, (uint32_t)g.q.pos[u.r + t - u.off], cs[j], sn[j]);
         }
-        const bool p2 = !(__builtin_amdgcn_readfirstlane(__float_as_uint(s)) & 0x7FFFFFu);      // (only a caller's own scales are not)
-        const float inv = 1.f / s;
-        if (tid < items) {
-            float v[4][8];
+        for (uint32_t h = h0; h < h1; ++h, src += dh) {
+            uint4 x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = sh_dev_h2f((uint16_t)(w[e / 2] >> (16 * (e & 1))));
-            }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                // the product, and what it lacks for the correctly rounded quotient (Markstein, "Computation of elementary functions on
-                // the IBM RISC System/6000 processor", 1990): nothing where s is a power of two
-                const float f = v[j / 8][j % 8], q = f * inv;
-                v[j / 8][j % 8] = p2 ? q : fmaf(fmaf(-q, s, f), inv, q);
-            }
-            if (!isv) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t t = t0 + j;
-                    if (t >= off && t < end)
-                        *(uint2 *)(dst + t * dh + 8 * ch) = make_uint2(codes4<FP8>(v[j][0], v[j][1], v[j][2], v[j][3]), codes4<FP8>(v[j][4], v[j][5], v[j][6], v[j][7]));
+                const uint32_t t = t0 + j;
+                uint32_t w[4] = {0, 0, 0, 0};
+                if (mine && t >= u.off && t < u.end) {
+                    rope_load<4>(src + (uint64_t)(t - u.off) * ld + ca, w);
+                    rope_load<4>(src + (uint64_t)(t - u.off) * ld + cb, w + 2);
+                    if (turned) rope_turn<4>(w, g.q.p.pairs, cs[j], sn[j]);
                 }
-            } else {
-                const bool whole = t0 >= off && t0 + 4 <= end;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    uint8_t *p = dst + (8 * ch + e) * c.bs + t0;
-                    const uint32_t w = codes4<FP8>(v[0][e], v[1][e], v[2][e], v[3][e]);
-                    if (whole) *(uint32_t *)p = w;
-                    else
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (t0 + j >= off && t0 + j < end) p[j] = (uint8_t)(w >> (8 * j));
-                }
+                x[j] = make_uint4(w[0], w[1], w[2], w[3]);
             }
+            append_page<FP8, NT, true>(c, 0, h, u, blk0, t0, ca, cb, mine, x, s_top);
         }
-        if (tid == 0) *sp = s;
     }
 }
 
@@ -349,6 +449,39 @@ void launch_append(const AppendArgs &a, hipStream_t st) {
     else if (items <= 128) launch_append_nt<FP8, 128>(a, st);
     else if (items <= 256) launch_append_nt<FP8, 256>(a, st);
     else launch_append_nt<FP8, 512>(a, st);
+}
+
+template <bool FP8, int NT>
+void launch_append_rope_nt(AppendRopeArgs g, hipStream_t st) {
+    // heads of a workgroup of keys: one while that keeps a step's few rows short, then as many as share a row's angles
+    g.kh = g.a.rows <= 512 ? 1 : std::min(4u, g.a.c.hkv);
+    g.kg = sh_cdiv(g.a.c.hkv, g.kh);
+    const uint32_t heads = g.kg + g.a.c.hkv, chunks = g.a.c.dh / 8, rows = g.a.rows;
+    g.a.dheads = sh_make_div(heads);
+    const uint64_t all = (uint64_t)rows * g.q.heads * chunks;
+    g.q.hs = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(g.q.heads, all >> 18));
+    const uint32_t groups = sh_cdiv(g.q.heads, g.q.hs);
+    g.q.dch = sh_make_div(chunks);
+    g.q.dhg = sh_make_div(std::max(groups, 1u));
+    const uint64_t per = (uint64_t)chunks * groups;                                          // items of a row of queries
+    uint64_t most = std::min<uint64_t>((1u << 30) / (heads * NT) * g.a.rg, (1u << 30) / std::max<uint64_t>(per, 1));
+    most = std::max<uint64_t>(g.a.rg, most / g.a.rg * g.a.rg);                               // rows of a launch, which has fewer than 2^32 threads
+    for (uint64_t r = 0; r < rows; r += most) {
+        const uint32_t n = (uint32_t)std::min<uint64_t>(rows - r, most);
+        g.a.row0 = g.q.row0 = (uint32_t)r;
+        g.q.rows = (uint32_t)r + n;
+        g.blocks = sh_cdiv(n, g.a.rg) * heads;
+        const uint32_t turns = (uint32_t)((n * per + NT - 1) / NT);
+        hipLaunchKernelGGL((k_kv_append_rope<FP8, NT>), dim3(g.blocks + turns), dim3(NT), 0, st, g);
+    }
+}
+template <bool FP8>
+void launch_append_rope(const AppendRopeArgs &g, hipStream_t st) {
+    const uint32_t items = g.a.c.bs * g.a.c.dh / 32;
+    if (items <= 64) launch_append_rope_nt<FP8, 64>(g, st);
+    else if (items <= 128) launch_append_rope_nt<FP8, 128>(g, st);
+    else if (items <= 256) launch_append_rope_nt<FP8, 256>(g, st);
+    else launch_append_rope_nt<FP8, 512>(g, st);
 }
 
 }  // namespace
@@ -393,27 +526,58 @@ int sh_kv_slots(uint64_t table, uint32_t ld, uint64_t lens, uint64_t lens_out, u
     return sh_launch_ok("sh_kv_slots") ? 0 : SH_EHIP;
 }
 
+// The checks that both writes make, and what they share of their arguments.
+static int append_args(const char *name, const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uint32_t ldv, uint64_t slots, uint32_t rows, AppendArgs *a) {
+    if (!k || !v || !slots) { sh_set_error(-1, "[%s] NULL address", name); return -1; }
+    if ((k | v) % 2 || slots % 4) { sh_set_error(-1, "[%s] rows must be 2-byte aligned, slots 4-byte aligned", name); return -1; }
+    if (ldk < c->hkv * c->dh || ldv < c->hkv * c->dh) {
+        sh_set_error(-1, "[%s] leading dim %u or %u < %u", name, ldk, ldv, c->hkv * c->dh);
+        return -1;
+    }
+    if (rows >= (1u << 31)) { sh_set_error(-1, "[%s] %u rows", name, rows); return -1; }
+    a->k = (const uint16_t *)k; a->v = (const uint16_t *)v;
+    a->ldk = ldk; a->ldv = ldv;
+    a->slots = (const int32_t *)slots;
+    a->rows = rows;
+    a->dch = sh_make_div(c->dh / 8);
+    // rows of a workgroup: one while all pages run at once, then few enough that most have a page to do in a prompt
+    a->rg = rows <= 512 ? 1 : rows <= 4096 ? 4 : c->bs;
+    return 0;
+}
+
 int sh_kv_append(const sh_kv_cache *c, uint64_t k, uint64_t v, uint32_t ldk, uint32_t ldv, uint64_t slots, uint32_t rows) {
     AppendArgs a;
     if (int rc = sh_kv_check("sh_kv_append", c, &a.c)) return rc;
     if (!rows) return 0;
-    if (!k || !v || !slots) { sh_set_error(-1, "[sh_kv_append] NULL address"); return -1; }
-    if ((k | v) % 2 || slots % 4) { sh_set_error(-1, "[sh_kv_append] rows must be 2-byte aligned, slots 4-byte aligned"); return -1; }
-    if (ldk < c->hkv * c->dh || ldv < c->hkv * c->dh) {
-        sh_set_error(-1, "[sh_kv_append] leading dim %u or %u < %u", ldk, ldv, c->hkv * c->dh);
-        return -1;
-    }
-    if (rows >= (1u << 31)) { sh_set_error(-1, "[sh_kv_append] %u rows", rows); return -1; }
-    a.k = (const uint16_t *)k; a.v = (const uint16_t *)v;
-    a.ldk = ldk; a.ldv = ldv;
-    a.slots = (const int32_t *)slots;
-    a.rows = rows;
-    a.dch = sh_make_div(c->dh / 8);
-    // rows of a workgroup: one while all pages run at once, then few enough that most have a page to do in a prompt
-    a.rg = rows <= 512 ? 1 : rows <= 4096 ? 4 : c->bs;
+    if (int rc = append_args("sh_kv_append", c, k, v, ldk, ldv, slots, rows, &a)) return rc;
     if (c->fmt == SH_FP8) launch_append<true>(a, sh_stream());
     else launch_append<false>(a, sh_stream());
     return sh_launch_ok("sh_kv_append") ? 0 : SH_EHIP;
+}
+
+int sh_kv_append_rope(const sh_kv_cache *c, const sh_rope_plan *p, uint64_t yq, uint64_t q, uint64_t k, uint64_t v, uint64_t pos, uint64_t slots, uint32_t rows,
+                      uint32_t H, uint32_t ldyq, uint32_t ldq, uint32_t ldk, uint32_t ldv) {
+    AppendRopeArgs g{};
+    if (int rc = sh_kv_check("sh_kv_append_rope", c, &g.a.c)) return rc;
+    if (int rc = sh_rope_check("sh_kv_append_rope", p, c->dh, &g.q.p)) return rc;
+    if (p->rot % 8) { sh_set_error(-1, "[sh_kv_append_rope] %u turned columns (a multiple of 8)", p->rot); return -1; }
+    if (!rows) return 0;
+    if (int rc = append_args("sh_kv_append_rope", c, k, v, ldk, ldv, slots, rows, &g.a)) return rc;
+    if (!pos || (H && (!q || !yq))) { sh_set_error(-1, "[sh_kv_append_rope] NULL address"); return -1; }
+    if (pos % 4 || (q | yq) % 2) { sh_set_error(-1, "[sh_kv_append_rope] rows must be 2-byte aligned, positions 4-byte aligned"); return -1; }
+    const uint64_t wide = (uint64_t)H * c->dh;
+    if (H && (ldyq < wide || ldq < wide)) {
+        sh_set_error(-1, "[sh_kv_append_rope] leading dim %u or %u < %llu", ldyq, ldq, (unsigned long long)wide);
+        return -1;
+    }
+    if (H && q == yq && ldq != ldyq) { sh_set_error(-1, "[sh_kv_append_rope] queries in place with leading dims %u and %u", ldyq, ldq); return -1; }
+    g.q.y = (uint16_t *)yq; g.q.x = (const uint16_t *)q;
+    g.q.pos = (const int32_t *)pos;
+    g.q.ldy = ldyq; g.q.ldx = ldq;
+    g.q.heads = H; g.q.dh = c->dh;
+    if (c->fmt == SH_FP8) launch_append_rope<true>(g, sh_stream());
+    else launch_append_rope<false>(g, sh_stream());
+    return sh_launch_ok("sh_kv_append_rope") ? 0 : SH_EHIP;
 }
 
 }  // extern "C"

@@ -1,0 +1,265 @@
+// Microscaled 4-bit floating point: rows to codes (sh_mx4_quant) and products of codes (sh_gemm_mx4, sh_gemm_mx4_f16).
+//
+// z[m][n] = sum_b 2^(sx[m][b] + sw[n][b]) sum_{k in b} x[m][k] w[n][k] over blocks b of 32 k: v_mfma_scale_f32_*_f8f6f4 takes the e2m1 codes
+// and the scale bytes as they are stored. A lane's operand of a step is one block of one row (16 bytes), and one byte of a scale word
+// that the instruction names, so no code is moved between lanes: of the 16 blocks that four steps of a 16 x 16 x 128 product take, lane (row, g) has the
+// blocks 4 g .. 4 g + 3, in step j block 4 g + j, and their four scales in one aligned word. (Which blocks meet in a step does not
+// matter, as long as both operands have the same.)
+#include "sh_common.h"
+#include <algorithm>
+
+namespace {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+
+constexpr int E2M1 = 4;                    // the instruction's number of the format
+constexpr uint32_t ONES = 0x7F7F7F7Fu;     // four scales of 1
+
+__device__ __forceinline__ v8i operand(uint4 c) { return v8i{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0}; }
+__device__ __forceinline__ us2 bits2(uint32_t w) { return __builtin_bit_cast(us2, w & 0x7FFF7FFFu); }     // a pair of halves without their signs
+
+// The scale byte of a block whose largest |x| is the half `top`: amax = f 2^e with f in [0.5, 1), 6 = 0.75 2^3. 255 where it is not finite.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+    const float amax = sh_dev_h2f((uint16_t)top);
+    const int e = __builtin_amdgcn_frexp_expf(amax), p = top ? max(__builtin_amdgcn_frexp_mantf(amax) <= 0.75f ? e - 3 : e - 2, -32) : -32;
+    return top >= 0x7C00u ? 255u : (uint32_t)(p + 127);
+}
+// Eight halves to eight codes, nearest, ties to even (|x| <= 6 scale).
+__device__ __forceinline__ uint32_t codes8(uint4 v, float scale) {
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(sh_h2, v.x), scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(sh_h2, v.y), scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(sh_h2, v.z), scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(sh_h2, v.w), scale, 3);
+}
+__device__ __forceinline__ us2 top8(uint4 v) {
+    return __builtin_elementwise_max(__builtin_elementwise_max(bits2(v.x), bits2(v.y)), __builtin_elementwise_max(bits2(v.z), bits2(v.w)));
+}
+// Halves [k, k + 8) of a row of K, zeros behind it.
+__device__ __forceinline__ uint4 load8(const uint16_t *row, uint32_t k, uint32_t K) {
+    if (k + 8 <= K) return sh_ld16_any(row + k);
+    if (k >= K) return make_uint4(0, 0, 0, 0);
+    if (K >= 8) return sh_ld8_row(row, k, K);
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (uint32_t i = 0; i < K; ++i) w[i / 2] |= (uint32_t)row[i] << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// ---- sh_mx4_quant -------------------------------------------------------------------------------------------------
+struct QuantArgs {
+    uint8_t *codes, *scales;
+    const uint16_t *x;
+    uint64_t ldc, lds, ldx, items;
+    uint32_t cols, row0;
+    ShDiv dch;                             // by a row's 16-byte pieces
+};
+
+// A lane has 8 columns, four lanes a block.
+__global__ __launch_bounds__(256) void k_mx4_quant(QuantArgs a) {
+    const uint32_t it = blockIdx.x * 256u + threadIdx.x;
+    if (it >= a.items) return;
+    const uint32_t r = sh_div(it, a.dch), c = it - r * a.dch.d;
+    const uint64_t row = a.row0 + (uint64_t)r;
+    const uint4 v = load8(a.x + row * a.ldx, 8 * c, a.cols);
+    const us2 t = top8(v);
+    float top = (float)max(t.x, t.y);                                          // (exact)
+    top = fmaxf(top, sh_dpp<0xb1>(top, top));
+    top = fmaxf(top, sh_dpp<0x4e>(top, top));
+    const uint32_t e = scale_byte((uint32_t)top);
+    const uint32_t w = e < 255u ? codes8(v, __uint_as_float(e << 23)) : 0u;
+    *(uint32_t *)(a.codes + row * a.ldc + 4 * c) = w;
+    if (!(c & 3)) a.scales[row * a.lds + c / 4] = (uint8_t)e;
+}
+
+// ---- products -----------------------------------------------------------------------------------------------------
+struct MxArgs {
+    const uint8_t *xc, *xs, *wc, *ws;
+    const uint16_t *x;                     // fp16 rows in place of xc and xs
+    uint16_t *z;
+    uint32_t M, N, K, nb;
+    uint64_t ldxc, ldxs, ldwc, ldws, ldx, ldz, ldr;
+    const void *bias;
+    const uint16_t *res;
+    uint32_t bias_fp32, act;
+};
+
+__device__ __forceinline__ void store_one(const MxArgs &a, uint32_t m, uint32_t n, float v) {
+    if (a.bias) v += a.bias_fp32 ? ((const float *)a.bias)[n] : sh_dev_h2f(((const uint16_t *)a.bias)[n]);
+    if (a.act == SH_ACT_GELU) v = sh_gelu_f32(v);
+    uint16_t h = sh_dev_f2h_rr(v);
+    if (a.res) h = sh_dev_f2h_rr(sh_dev_h2f(h) + sh_dev_h2f(a.res[m * a.ldr + n]));
+    a.z[m * a.ldz + n] = h;
+}
+
+// One row's blocks b .. b + 3 and their scales; zeros with a scale of 1 behind the last block.
+struct Four { uint4 c[4]; uint32_t s; };
+__device__ __forceinline__ uint32_t scales4(const uint8_t *p, uint32_t b, uint32_t nb) {
+    if (b >= nb) return ONES;
+    const uint32_t s = *(const uint32_t *)(p + b), left = nb - b;
+    if (left >= 4) return s;
+    const uint32_t m = (1u << (8 * left)) - 1;
+    return (s & m) | (ONES & ~m);
+}
+__device__ __forceinline__ void load_four(const uint8_t *codes, const uint8_t *scales, uint32_t b, uint32_t nb, Four &o) {
+    o.s = scales4(scales, b, nb);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.c[j] = b + j < nb ? *(const uint4 *)(codes + 16ull * (b + j)) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void load_four_f16(const uint16_t *row, uint32_t b, uint32_t nb, uint32_t K, Four &o) {
+    o.s = ONES;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        o.c[j] = make_uint4(0, 0, 0, 0);
+        if (b + j < nb) {
+            uint4 v[4];
+            us2 t = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = load8(row, 32 * (b + j) + 8 * i, K);
+                t = __builtin_elementwise_max(t, top8(v[i]));
+            }
+            const uint32_t e = scale_byte(max(t.x, t.y));
+            o.s = (o.s & ~(255u << (8 * j))) | e << (8 * j);
+            if (e < 255u) {
+                const float f = __uint_as_float(e << 23);
+                o.c[j] = make_uint4(codes8(v[0], f), codes8(v[1], f), codes8(v[2], f), codes8(v[3], f));
+            }
+        }
+    }
+}
+
+// Few rows: a workgroup has 16 columns and 16 MT rows of z; its waves take units of 512 k in turn, and their sums are added in LDS in wave order.
+template <int MT, int NW, bool F16>
+__global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
+    __shared__ float s_z[NW][16 * MT][17];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const uint32_t col0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+    const uint64_t wr = min(col0 + n, a.N - 1);
+    const uint32_t units = (a.nb + 15) / 16;
+    sh_f4v acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = sh_f4v{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t u = wave; u < units; u += NW) {
+        const uint32_t b = 16 * u + 4 * g;
+        Four w, x[MT];
+        load_four(a.wc + wr * a.ldwc, a.ws + wr * a.ldws, b, a.nb, w);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const uint64_t xr = min(m0 + 16 * i + n, a.M - 1);
+            if constexpr (F16) load_four_f16(a.x + xr * a.ldx, b, a.nb, a.K, x[i]);
+            else load_four(a.xc + xr * a.ldxc, a.xs + xr * a.ldxs, b, a.nb, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.c[0]), operand(x[i].c[0]), acc[i], E2M1, E2M1, 0, (int)w.s, 0, (int)x[i].s);
+            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.c[1]), operand(x[i].c[1]), acc[i], E2M1, E2M1, 1, (int)w.s, 1, (int)x[i].s);
+            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.c[2]), operand(x[i].c[2]), acc[i], E2M1, E2M1, 2, (int)w.s, 2, (int)x[i].s);
+            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.c[3]), operand(x[i].c[3]), acc[i], E2M1, E2M1, 3, (int)w.s, 3, (int)x[i].s);
+        }
+    }
+    // lane (m, g): the columns 4 g .. 4 g + 3 of row m
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_z[wave][16 * i + n][4 * g + e] = acc[i][e];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < 256 * MT; i += 64 * NW) {
+        const uint32_t r = i / 16, c = i % 16;
+        if (m0 + r >= a.M || col0 + c >= a.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) v += s_z[k][r][c];
+        store_one(a, m0 + r, col0 + c, v);
+    }
+}
+
+template <int MT, int NW, bool F16>
+void launch_rows(const MxArgs &a, hipStream_t st) {
+    hipLaunchKernelGGL((k_mx4_rows<MT, NW, F16>), dim3(sh_cdiv(a.N, 16), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), 0, st, a);
+}
+
+// The checks that both products make of the weight, the result and the epilogue.
+int product_args(const char *name, uint64_t wc, uint64_t ws, uint64_t z, uint32_t M, uint32_t N, uint32_t K, uint32_t ldwc, uint32_t ldws, uint32_t ldz,
+                 const sh_gemm_epi *epi, MxArgs *a) {
+    if (!wc || !ws || !z) { sh_set_error(-1, "[%s] NULL tensor address", name); return -1; }
+    if (!K || K > (1u << 31)) { sh_set_error(-1, "[%s] K %u", name, K); return -1; }
+    if (M > (1u << 26) || N > (1u << 26)) { sh_set_error(-1, "[%s] M=%u N=%u too large", name, M, N); return -1; }
+    const uint32_t nb = (K - 1) / 32 + 1;
+    if (wc % 16 || ldwc % 16 || ldwc < 16 * (uint64_t)nb) { sh_set_error(-1, "[%s] weight codes: 16-byte aligned, leading dim %u for %u blocks", name, ldwc, nb); return -1; }
+    if (ws % 4 || ldws % 4 || ldws < nb) { sh_set_error(-1, "[%s] weight scales: 4-byte aligned, leading dim %u for %u blocks", name, ldws, nb); return -1; }
+    if (z % 2 || ldz < N) { sh_set_error(-1, "[%s] leading dim %u for %u columns, or alignment of z", name, ldz, N); return -1; }
+    *a = MxArgs{};
+    a->wc = (const uint8_t *)wc; a->ws = (const uint8_t *)ws;
+    a->z = (uint16_t *)z;
+    a->M = M; a->N = N; a->K = K; a->nb = nb;
+    a->ldwc = ldwc; a->ldws = ldws; a->ldz = ldz;
+    if (!epi) return 0;
+    if (epi->act > SH_ACT_GELU) { sh_set_error(-1, "[%s] unknown act %u", name, epi->act); return -1; }
+    if (epi->bias && (epi->bias_fmt > SH_BIAS_FP32 || epi->bias % (epi->bias_fmt == SH_BIAS_FP32 ? 4 : 2))) {
+        sh_set_error(-1, "[%s] bias format %u or its alignment", name, epi->bias_fmt);
+        return -1;
+    }
+    if (epi->residual && (epi->ldr < N || epi->residual % 2)) { sh_set_error(-1, "[%s] ldr %u < N %u, or alignment", name, epi->ldr, N); return -1; }
+    if (epi->splits > 1 || epi->ln_stats || epi->ln_c || epi->stats_out || epi->ln_parts) {
+        sh_set_error(-1, "[%s] no K split, LayerNorm fold or row partials", name);
+        return -1;
+    }
+    a->bias = (const void *)epi->bias; a->bias_fp32 = epi->bias_fmt == SH_BIAS_FP32;
+    a->act = epi->act;
+    a->res = (const uint16_t *)epi->residual; a->ldr = epi->ldr;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sh_mx4_quant(uint64_t codes, uint64_t scales, uint64_t x, uint32_t rows, uint32_t cols, uint32_t ldc, uint32_t lds, uint32_t ldx) {
+    if (!rows || !cols) return 0;
+    if (!codes || !scales || !x) { sh_set_error(-1, "[sh_mx4_quant] NULL address"); return -1; }
+    const uint32_t nb = (cols - 1) / 32 + 1;
+    if (codes % 16 || ldc % 16 || ldc < 16 * (uint64_t)nb) { sh_set_error(-1, "[sh_mx4_quant] codes: 16-byte aligned, leading dim %u for %u blocks", ldc, nb); return -1; }
+    if (scales % 4 || lds % 4 || lds < nb) { sh_set_error(-1, "[sh_mx4_quant] scales: 4-byte aligned, leading dim %u for %u blocks", lds, nb); return -1; }
+    if (x % 2 || ldx < cols) { sh_set_error(-1, "[sh_mx4_quant] leading dim %u for %u columns, or alignment of x", ldx, cols); return -1; }
+    if (cols > (1u << 30)) { sh_set_error(-1, "[sh_mx4_quant] %u columns", cols); return -1; }
+    QuantArgs a{(uint8_t *)codes, (uint8_t *)scales, (const uint16_t *)x, ldc, lds, ldx, 0, cols, 0, sh_make_div(4 * nb)};
+    const uint32_t most = std::max(1u, (1u << 30) / (4 * nb));                  // rows of a launch
+    for (uint64_t r = 0; r < rows; r += most) {
+        a.row0 = (uint32_t)r;
+        a.items = std::min<uint64_t>(rows - r, most) * 4 * nb;
+        hipLaunchKernelGGL(k_mx4_quant, dim3((uint32_t)((a.items + 255) / 256)), dim3(256), 0, sh_stream(), a);
+    }
+    return sh_launch_ok("sh_mx4_quant") ? 0 : SH_EHIP;
+}
+
+int sh_gemm_mx4(uint64_t xc, uint64_t xs, uint64_t wc, uint64_t ws, uint64_t z, uint32_t M, uint32_t N, uint32_t K,
+                uint32_t ldxc, uint32_t ldxs, uint32_t ldwc, uint32_t ldws, uint32_t ldz, const sh_gemm_epi *epi) {
+    if (!M || !N) return 0;
+    MxArgs a;
+    if (int rc = product_args("sh_gemm_mx4", wc, ws, z, M, N, K, ldwc, ldws, ldz, epi, &a)) return rc;
+    if (!xc || !xs) { sh_set_error(-1, "[sh_gemm_mx4] NULL tensor address"); return -1; }
+    if (xc % 16 || ldxc % 16 || ldxc < 16 * (uint64_t)a.nb) { sh_set_error(-1, "[sh_gemm_mx4] codes: 16-byte aligned, leading dim %u for %u blocks", ldxc, a.nb); return -1; }
+    if (xs % 4 || ldxs % 4 || ldxs < a.nb) { sh_set_error(-1, "[sh_gemm_mx4] scales: 4-byte aligned, leading dim %u for %u blocks", ldxs, a.nb); return -1; }
+    a.xc = (const uint8_t *)xc; a.xs = (const uint8_t *)xs;
+    a.ldxc = ldxc; a.ldxs = ldxs;
+    const hipStream_t st = sh_stream();
+    if (M <= 16) launch_rows<1, 8, false>(a, st);
+    else launch_rows<4, 8, false>(a, st);
+    return sh_launch_ok("sh_gemm_mx4") ? 0 : SH_EHIP;
+}
+
+int sh_gemm_mx4_f16(uint64_t x, uint64_t wc, uint64_t ws, uint64_t z, uint32_t M, uint32_t N, uint32_t K,
+                    uint32_t ldx, uint32_t ldwc, uint32_t ldws, uint32_t ldz, const sh_gemm_epi *epi) {
+    if (!M || !N) return 0;
+    MxArgs a;
+    if (int rc = product_args("sh_gemm_mx4_f16", wc, ws, z, M, N, K, ldwc, ldws, ldz, epi, &a)) return rc;
+    if (!x || x % 2 || ldx < K) { sh_set_error(-1, "[sh_gemm_mx4_f16] x: NULL, not 2-byte aligned, or leading dim %u < %u", ldx, K); return -1; }
+    if (M > 16) { sh_set_error(-1, "[sh_gemm_mx4_f16] %u rows (up to 16; more by sh_mx4_quant and sh_gemm_mx4)", M); return -1; }
+    a.x = (const uint16_t *)x; a.ldx = ldx;
+    launch_rows<1, 8, true>(a, sh_stream());
+    return sh_launch_ok("sh_gemm_mx4_f16") ? 0 : SH_EHIP;
+}
+
+}  // extern "C"

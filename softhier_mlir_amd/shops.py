@@ -26,6 +26,8 @@ SH_XM_AUTO, SH_XM_PANEL, SH_XM_WHOLE = 0, 1, 2
 SH_LLM_PAD = 0xFFFF
 SH_BIAS_FP16, SH_BIAS_FP32 = 0, 1
 SH_MESH_P = 4
+SH_ROPE_HALF, SH_ROPE_PAIRS = 0, 1
+SH_ROPE_NONE, SH_ROPE_LINEAR, SH_ROPE_BANDS, SH_ROPE_RAMP = 0, 1, 2, 3
 
 
 class sh_gemm_cfg(C.Structure):
@@ -46,6 +48,11 @@ class sh_kv_cache(C.Structure):
     """The 8-bit paged key / value cache of sh_kv_append and sh_attention_kv (additive)."""
     _fields_ = [("k", C.c_uint64), ("v", C.c_uint64), ("ks", C.c_uint64), ("vs", C.c_uint64), ("pgk", C.c_uint64), ("pgv", C.c_uint64),
                 ("pgs", C.c_uint32), ("pages", C.c_uint32), ("hkv", C.c_uint32), ("dh", C.c_uint32), ("bs", C.c_uint32), ("fmt", C.c_uint32)]
+
+
+class sh_rope_plan(C.Structure):
+    """Rotary positions of sh_rope_pos and sh_kv_append_rope (additive): `step` holds turns per position x 2^64."""
+    _fields_ = [("step", C.c_uint64), ("rot", C.c_uint32), ("layout", C.c_uint32), ("mscale", C.c_float), ("reserved", C.c_uint32)]
 
 
 u32, u64, i32, f32, i16 = C.c_uint32, C.c_uint64, C.c_int, C.c_float, C.c_uint16
@@ -104,6 +111,13 @@ _SIGS: dict[str, tuple] = {
     "sh_attention_kv": (i32, [u64, u64, C.POINTER(sh_kv_cache), u64, u32, u64, u64, u32, u32, u32, u32, u32, u32, f32, u32, u64, u64]),
     "sh_attention_kv_ws_bytes": (u64, [C.POINTER(sh_kv_cache), u32, u32, u32, u32, u32]),
     "sh_gemm_w4": (i32, [u64, u64, u64, u64, u64, u32, u32, u32, u32, u32, u32, u32, u32, C.POINTER(sh_gemm_epi)]),
+    # rotary positions, microscaled 4-bit products
+    "sh_rope_steps": (i32, [u64, u32, C.c_double, u32, C.c_double, C.c_double, C.c_double, u32]),
+    "sh_rope_pos": (i32, [u64, u64, u64, C.POINTER(sh_rope_plan), u32, u32, u32, u32, u32]),
+    "sh_kv_append_rope": (i32, [C.POINTER(sh_kv_cache), C.POINTER(sh_rope_plan), u64, u64, u64, u64, u64, u64, u32, u32, u32, u32, u32, u32]),
+    "sh_mx4_quant": (i32, [u64, u64, u64, u32, u32, u32, u32, u32]),
+    "sh_gemm_mx4": (i32, [u64, u64, u64, u64, u64, u32, u32, u32, u32, u32, u32, u32, u32, C.POINTER(sh_gemm_epi)]),
+    "sh_gemm_mx4_f16": (i32, [u64, u64, u64, u64, u32, u32, u32, u32, u32, u32, u32, C.POINTER(sh_gemm_epi)]),
     # test helpers
     "sh_test_fill_int_fp16": (None, [u64, u32, u32, u32, u32, i32, i32]),
     "sh_test_fill_fp16": (None, [u64, u32, u32, u32, u32, i32, i32, f32]),
@@ -168,6 +182,10 @@ def epi(bias: int = 0, bias_fmt: int = SH_BIAS_FP16, act: int = SH_ACT_NONE, res
 def kv_cache(k: int, v: int, ks: int, vs: int, pages: int, hkv: int, dh: int, bs: int, fmt: int = SH_INT8, pgk: int = 0,
              pgv: int = 0, pgs: int = 0) -> sh_kv_cache:
     return sh_kv_cache(k, v, ks, vs, pgk, pgv, pgs, pages, hkv, dh, bs, fmt)
+
+
+def rope_plan(step: int, rot: int, layout: int = SH_ROPE_HALF, mscale: float = 1.0) -> sh_rope_plan:
+    return sh_rope_plan(step, rot, layout, mscale, 0)
 
 
 def addr(t, elem_offset: int = 0) -> int:
