@@ -7,10 +7,10 @@
 // matter, as long as both operands have the same.)
 #include "sh_common.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
-typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 
@@ -175,6 +175,231 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
     }
 }
 
+// Many rows. A workgroup has a BM x BN tile of z, a wave TM x TN blocks of 32 x 32 of it (W's rows are the instruction's rows, so a lane has one row
+// of z and groups of four columns). Slices of 128 k (four blocks of a row: 64 bytes) go by DMA into a ring of four stages, three slices ahead; the scales of four
+// slices (16 bytes of a row) into a ring of three. A slice is two steps of 64 k; a step's operands are read while the last step multiplies, and the barrier that frees
+// a stage lies between the two, so that no wave meets it without products to issue. Chunk c of a row lies at c ^ (row / 2 % 4) of its 64 bytes: eight lanes'
+// reads then touch every bank once. Behind the last block the codes are those of the last one again and both scales 2^-127: their product is 0 in fp32.
+__device__ __forceinline__ void dma4_s(const void *base, uint32_t off, uint32_t lds_wave_base) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_wave_base), "v"(off), "s"(base) : "memory", "m0");
+#pragma clang diagnostic pop
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    return __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) sh_u4v *)(uintptr_t)addr);
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t addr) { return *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)addr; }
+
+template <int BM, int BN, int WGM, int WGN>
+struct Tile {
+    static constexpr int NW = WGM * WGN, TM = BM / WGM / 32, TN = BN / WGN / 32, NST = 4, ROWS = BM + BN;
+    static constexpr int CPW = ROWS / 16 / NW, SCI = ROWS / 16, SPW = (SCI + 4 * NW - 1) / (4 * NW);       // DMAs of a wave for a slice: codes, scales
+    static constexpr uint32_t CODE = ROWS * 64, SC = ROWS * 16, RING = NST * CODE, PITCH = BN * 2 + 16, STAGED = BM * PITCH;
+    static constexpr uint32_t LDS = RING + 3 * SC > STAGED ? RING + 3 * SC : STAGED;
+    static_assert(ROWS % (16 * NW) == 0 && BM % (32 * WGM) == 0 && BN % (32 * WGN) == 0 && LDS <= 163840, "tile");
+};
+
+template <int BM, int BN, int WGM, int WGN, int PER>
+__global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
+    using T = Tile<BM, BN, WGM, WGN>;
+    constexpr int NW = T::NW, TM = T::TM, TN = T::TN, NST = T::NST, CPW = T::CPW, SPW = T::SPW;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const uint32_t lds0 = sh_lds_addr(smem), sc0 = lds0 + T::RING;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WGM, wn = wave / WGM;
+    const uint32_t g = lane >> 5, r32 = lane & 31;
+    // tiles in bands of eight of a column, a contiguous range of them for each XCD
+    const uint32_t tm_all = (a.M + BM - 1) / BM, tn_all = (a.N + BN - 1) / BN, tiles = tm_all * tn_all;
+    uint32_t id = blockIdx.x;
+    {
+        const uint32_t x = id & 7, per = tiles / 8, more = tiles % 8;
+        id = x * per + min(x, more) + (id >> 3);
+    }
+    const uint32_t band = id / (8 * tn_all), in = id - band * 8 * tn_all, high = min(8u, tm_all - band * 8);
+    const uint32_t m0 = (band * 8 + in % high) * BM, n0 = in / high * BN;
+    const uint32_t nb = a.nb, nd = (nb + 3) / 4, n = nd;                               // slices
+    const uint8_t *wc = a.wc + (uint64_t)n0 * a.ldwc, *xc = a.xc + (uint64_t)m0 * a.ldxc, *ws = a.ws + (uint64_t)n0 * a.ldws, *xs = a.xs + (uint64_t)m0 * a.ldxs;
+    const uint32_t wlim = a.N - 1 - n0, xlim = a.M - 1 - m0;
+    const uint32_t ldwc = (uint32_t)a.ldwc, ldxc = (uint32_t)a.ldxc, ldws = (uint32_t)a.ldws, ldxs = (uint32_t)a.ldxs;
+    const uint32_t chunk = (lane & 3) ^ ((lane >> 3) & 3);
+    uint32_t off[CPW];
+#pragma unroll
+    for (int i = 0; i < CPW; ++i) {
+        const uint32_t first = (wave * CPW + i) * 16, row = first + (lane >> 2);
+        off[i] = 16 * chunk + (first < BN ? min(row, wlim) * ldwc : min(row - BN, xlim) * ldxc);
+    }
+    // `part` of `parts` of a wave's DMAs
+    const auto load_codes = [&](uint32_t u, int part = 0, int parts = 1) {
+        const uint32_t slot = lds0 + (u % NST) * T::CODE;
+        uint32_t back = 0;
+        if (4 * u + 4 > nb && 4 * u + chunk >= nb) back = 16 * (4 * u + chunk + 1 - nb);
+#pragma unroll
+        for (int i = CPW * part / parts; i < CPW * (part + 1) / parts; ++i) {
+            const uint32_t ins = wave * CPW + i;
+            sh_lds_dma16_s((ins * 16 < BN ? wc : xc) + 64ull * u, off[i] - back, slot + ins * 1024);
+        }
+    };
+    // part `q` of the scales of slices 4 gr .. 4 gr + 3
+    const auto load_scales = [&](uint32_t gr, uint32_t q) {
+#pragma unroll
+        for (int i = 0; i < SPW; ++i) {
+            const uint32_t ins = ((q * NW + wave) * SPW + i) % T::SCI, row = ins * 16 + (lane >> 2), d = 4 * min(4 * gr + (lane & 3), nd - 1);
+            const bool isw = ins * 16 < BN;
+            dma4_s(isw ? ws : xs, d + (isw ? min(row, wlim) * ldws : min(row - BN, xlim) * ldxs), sc0 + gr % 3 * T::SC + ins * 256);
+        }
+    };
+    const uint32_t lane_at = r32 * 64 + ((2 * g) ^ ((lane >> 1) & 3)) * 16;
+    struct Ops { uint4 w[TN], x[TM]; };
+    const auto read = [&](uint32_t t, int j, Ops &o) {
+        const uint32_t at = lds0 + (t % NST) * T::CODE + (lane_at ^ (16 * j));
+#pragma unroll
+        for (int i = 0; i < TN; ++i) o.w[i] = lds16(at + (wn * TN + i) * 2048);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) o.x[i] = lds16(at + BN * 64 + (wm * TM + i) * 2048);
+    };
+    struct Scales { uint32_t w[TN], x[TM]; };
+    const auto read_scales = [&](uint32_t t, Scales &s) {
+        const uint32_t at = sc0 + t / 4 % 3 * T::SC + r32 * 16 + 4 * (t & 3);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) s.w[i] = lds4(at + (wn * TN + i) * 512);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) s.x[i] = lds4(at + BN * 16 + (wm * TM + i) * 512);
+    };
+    const auto own_scales = [&](uint32_t t, Scales &s) {
+        const uint32_t sh = 16 * g, keep = 4 * t + 4 > nb ? (1u << (8 * (nb - 4 * t))) - 1 : ~0u;
+#pragma unroll
+        for (int i = 0; i < TN; ++i) s.w[i] = (s.w[i] & keep) >> sh;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) s.x[i] = (s.x[i] & keep) >> sh;
+    };
+    sh_f16v acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int k = 0; k < TM; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
+    const auto multiply = [&](auto j, const Ops &o, const Scales &s, auto between) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            between(i);
+#pragma unroll
+            for (int k = 0; k < TM; ++k)
+                acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(o.w[i]), operand(o.x[k]), acc[i][k], E2M1, E2M1, decltype(j)::value, (int)s.w[i],
+                                                                           decltype(j)::value, (int)s.x[k]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (uint32_t q = 0; q < 4; ++q) load_scales(0, q);
+#pragma unroll
+    for (uint32_t u = 0; u < NST; ++u)
+        if (u < n) {
+            load_codes(u);
+            load_scales(1, u);
+        }
+    if (n >= NST) sh_wait_vmcnt<3 * (CPW + SPW)>();
+    else sh_wait_vmcnt<0>();
+    __syncthreads();
+    Ops o0, o1;
+    Scales s0, s1;
+    read(0, 0, o0);
+    read_scales(0, s0);
+    own_scales(0, s0);
+    // (no branch in a slice: the compiler would move products past the barrier)
+    const auto slice = [&](uint32_t t, auto more) {
+        read(t, 1, o1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(std::integral_constant<int, 0>{}, o0, s0, [](int) {});
+        // the next slice has come, and this one's operands are all in registers
+        sh_wait_vmcnt<decltype(more)::value ? 2 * (CPW + SPW) : 0>();
+        sh_wait_lgkm0();
+        asm volatile("" ::: "memory");                      // (the barrier alone does not keep the compiler's loads on their side)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const uint32_t nx = decltype(more)::value ? t + 1 : min(t + 1, n - 1);
+        read(nx, 0, o0);
+        read_scales(nx, s1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(std::integral_constant<int, 1>{}, o1, s0, [&](int i) {
+            if constexpr (decltype(more)::value) {
+                load_codes(t + NST, i, TN);
+                if (i == TN - 1) load_scales(t / 4 + 2, t & 3);
+            }
+        });
+        s0 = s1;
+        own_scales(nx, s0);
+    };
+    uint32_t t = 0;
+    for (; t + NST < n; ++t) slice(t, std::true_type{});
+    for (; t < n; ++t) slice(t, std::false_type{});
+    // The tile through LDS: bias and GELU in fp32, then whole rows of fp16 with the residual.
+    __syncthreads();
+    const uint32_t epi_lds = lds0;
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t nl = (wn * TN + i) * 32 + 8 * q + 4 * g;
+            float b[4] = {0.f, 0.f, 0.f, 0.f};
+            if (a.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t nn = min(n0 + nl + e, a.N - 1);
+                    b[e] = a.bias_fp32 ? ((const float *)a.bias)[nn] : sh_dev_h2f(((const uint16_t *)a.bias)[nn]);
+                }
+#pragma unroll
+            for (int k = 0; k < TM; ++k) {
+                uint16_t h[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = acc[i][k][4 * q + e] + b[e];
+                    if (a.act == SH_ACT_GELU) v = sh_gelu_f32(v);
+                    h[e] = sh_dev_f2h_rr(v);
+                }
+                const uint32_t ml = (wm * TM + k) * 32 + r32;
+                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                *(__attribute__((address_space(3))) u2 *)(uintptr_t)(epi_lds + ml * T::PITCH + nl * 2) = u2{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
+            }
+        }
+    __syncthreads();
+    constexpr uint32_t CH = BN / 8;
+    for (uint32_t i = threadIdx.x; i < BM * CH; i += 64 * NW) {
+        const uint32_t r = i / CH, c = 8 * (i % CH), m = m0 + r, nn = n0 + c;
+        if (m >= a.M || nn >= a.N) continue;
+        uint4 v = lds16(epi_lds + r * T::PITCH + c * 2);
+        const uint32_t left = min(a.N - nn, 8u);
+        if (a.res) {
+            const uint16_t *p = a.res + m * a.ldr + nn;
+            uint4 q;
+            if (left == 8) q = sh_ld16_any(p);
+            else {
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    if (e < left) w[e / 2] |= (uint32_t)p[e] << (16 * (e & 1));
+                q = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            v = make_uint4(sh_hadd2(v.x, q.x), sh_hadd2(v.y, q.y), sh_hadd2(v.z, q.z), sh_hadd2(v.w, q.w));
+        }
+        sh_st8_any(a.z + m * a.ldz + nn, v, left);
+    }
+}
+
+template <int BM, int BN, int WGM, int WGN, int PER>
+bool launch_tile(const MxArgs &a, hipStream_t st) {
+    using T = Tile<BM, BN, WGM, WGN>;
+    static bool set = false;
+    if (!set && T::LDS > 65536) {
+        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_mx4_tile<BM, BN, WGM, WGN, PER>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS),
+                       "sh_gemm_mx4 hipFuncSetAttribute")) return false;
+        set = true;
+    }
+    const uint64_t tiles = (uint64_t)sh_cdiv(a.M, BM) * sh_cdiv(a.N, BN);
+    hipLaunchKernelGGL((k_mx4_tile<BM, BN, WGM, WGN, PER>), dim3((uint32_t)tiles), dim3(64 * T::NW), T::LDS, st, a);
+    return true;
+}
+
 template <int MT, int NW, bool F16>
 void launch_rows(const MxArgs &a, hipStream_t st) {
     hipLaunchKernelGGL((k_mx4_rows<MT, NW, F16>), dim3(sh_cdiv(a.N, 16), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), 0, st, a);
@@ -245,8 +470,12 @@ int sh_gemm_mx4(uint64_t xc, uint64_t xs, uint64_t wc, uint64_t ws, uint64_t z, 
     a.xc = (const uint8_t *)xc; a.xs = (const uint8_t *)xs;
     a.ldxc = ldxc; a.ldxs = ldxs;
     const hipStream_t st = sh_stream();
+    const bool near = ldxc <= (1u << 24) && ldwc <= (1u << 24) && ldxs <= (1u << 24) && ldws <= (1u << 24);       // a tile's rows within 32-bit offsets
+    const uint64_t big = (uint64_t)sh_cdiv(M, 256) * sh_cdiv(N, 256), mid = (uint64_t)sh_cdiv(M, 128) * sh_cdiv(N, 128);
     if (M <= 16) launch_rows<1, 8, false>(a, st);
-    else launch_rows<4, 8, false>(a, st);
+    else if (M <= 64 || !near || mid > (1u << 22)) launch_rows<4, 8, false>(a, st);
+    else if (big >= 256) { if (!launch_tile<256, 256, 2, 2, 1>(a, st)) return SH_EHIP; }
+    else if (!launch_tile<128, 128, 2, 2, 2>(a, st)) return SH_EHIP;
     return sh_launch_ok("sh_gemm_mx4") ? 0 : SH_EHIP;
 }
 

@@ -138,7 +138,7 @@ def _check(got, x, w, bias=None, gelu=False, residual=None):
 
 SHAPES = [(1, 1, 1), (1, 16, 32), (1, 17, 33), (1, 64, 128), (1, 2048, 720), (1, 100, 4096), (2, 33, 200), (5, 68, 1032), (16, 256, 512), (17, 132, 968), (31, 960, 960),
           (33, 40, 136), (50, 720, 2048), (64, 260, 1608), (65, 48, 320), (200, 72, 264), (3, 5000, 64), (64, 64, 16384), (128, 128, 256), (129, 127, 255), (256, 256, 512),
-          (257, 300, 700), (300, 1000, 1000), (511, 513, 96), (700, 640, 2880), (1000, 260, 4100), (70, 2100, 31), (2048, 512, 512)]
+          (257, 300, 700), (300, 1000, 1000), (511, 513, 96), (700, 640, 2880), (1000, 260, 4100), (70, 2100, 31), (2048, 512, 512), (4100, 4200, 200), (4097, 4096, 33), (2500, 8200, 1200)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
