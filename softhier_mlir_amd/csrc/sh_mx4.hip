@@ -17,7 +17,7 @@ typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 constexpr int E2M1 = 4;                    // the instruction's number of the format
 constexpr uint32_t ONES = 0x7F7F7F7Fu;     // four scales of 1
 
-__device__ __forceinline__ v8i operand(uint4 c) { return v8i{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0}; }
+__device__ __forceinline__ v8i operand(sh_u4v c) { return v8i{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0}; }
 __device__ __forceinline__ us2 bits2(uint32_t w) { return __builtin_bit_cast(us2, w & 0x7FFF7FFFu); }     // a pair of halves without their signs
 
 // The scale byte of a block whose largest |x| is the half `top`: amax = f 2^e with f in [0.5, 1), 6 = 0.75 2^3. 255 where it is not finite.
@@ -94,7 +94,7 @@ __device__ __forceinline__ void store_one(const MxArgs &a, uint32_t m, uint32_t 
 }
 
 // One row's blocks b .. b + 3 and their scales; zeros with a scale of 1 behind the last block.
-struct Four { uint4 c[4]; uint32_t s; };
+struct Four { sh_u4v c[4]; uint32_t s; };
 __device__ __forceinline__ uint32_t scales4(const uint8_t *p, uint32_t b, uint32_t nb) {
     if (b >= nb) return ONES;
     const uint32_t s = *(const uint32_t *)(p + b), left = nb - b;
@@ -105,13 +105,13 @@ __device__ __forceinline__ uint32_t scales4(const uint8_t *p, uint32_t b, uint32
 __device__ __forceinline__ void load_four(const uint8_t *codes, const uint8_t *scales, uint32_t b, uint32_t nb, Four &o) {
     o.s = scales4(scales, b, nb);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o.c[j] = b + j < nb ? *(const uint4 *)(codes + 16ull * (b + j)) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) o.c[j] = b + j < nb ? *(const sh_u4v *)(codes + 16ull * (b + j)) : sh_u4v{0, 0, 0, 0};
 }
 __device__ __forceinline__ void load_four_f16(const uint16_t *row, uint32_t b, uint32_t nb, uint32_t K, Four &o) {
     o.s = ONES;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        o.c[j] = make_uint4(0, 0, 0, 0);
+        o.c[j] = sh_u4v{0, 0, 0, 0};
         if (b + j < nb) {
             uint4 v[4];
             us2 t = {0, 0};
@@ -124,7 +124,7 @@ __device__ __forceinline__ void load_four_f16(const uint16_t *row, uint32_t b, u
             o.s = (o.s & ~(255u << (8 * j))) | e << (8 * j);
             if (e < 255u) {
                 const float f = __uint_as_float(e << 23);
-                o.c[j] = make_uint4(codes8(v[0], f), codes8(v[1], f), codes8(v[2], f), codes8(v[3], f));
+                o.c[j] = sh_u4v{codes8(v[0], f), codes8(v[1], f), codes8(v[2], f), codes8(v[3], f)};
             }
         }
     }
@@ -186,24 +186,37 @@ __device__ __forceinline__ void dma4_s(const void *base, uint32_t off, uint32_t 
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_wave_base), "v"(off), "s"(base) : "memory", "m0");
 #pragma clang diagnostic pop
 }
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-    return __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) sh_u4v *)(uintptr_t)addr);
-}
+__device__ __forceinline__ sh_u4v lds16(uint32_t addr) { return *(const __attribute__((address_space(3))) sh_u4v *)(uintptr_t)addr; }
 __device__ __forceinline__ uint32_t lds4(uint32_t addr) { return *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)addr; }
+
+// f(0), f(1), ..., f(N - 1) as compile-time numbers; and the part of them that falls to place E of P when they are spread evenly.
+template <int N, int B = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+    if constexpr (B < N) {
+        f(std::integral_constant<int, B>{});
+        each<N, B + 1>(f);
+    }
+}
+template <int N, int P, typename E, typename F>
+__device__ __forceinline__ void some(E, F f) {
+    if constexpr (E::value < P) each<N * (E::value + 1) / P, N * E::value / P>(f);
+}
 
 template <int BM, int BN, int WGM, int WGN>
 struct Tile {
     static constexpr int NW = WGM * WGN, TM = BM / WGM / 32, TN = BN / WGN / 32, NST = 4, ROWS = BM + BN;
-    static constexpr int CPW = ROWS / 16 / NW, SCI = ROWS / 16, SPW = (SCI + 4 * NW - 1) / (4 * NW);       // DMAs of a wave for a slice: codes, scales
-    static constexpr uint32_t CODE = ROWS * 64, SC = ROWS * 16, RING = NST * CODE, PITCH = BN * 2 + 16, STAGED = BM * PITCH;
-    static constexpr uint32_t LDS = RING + 3 * SC > STAGED ? RING + 3 * SC : STAGED;
-    static_assert(ROWS % (16 * NW) == 0 && BM % (32 * WGM) == 0 && BN % (32 * WGN) == 0 && LDS <= 163840, "tile");
+    static constexpr int CPW = ROWS / 16 / NW;                                        // DMAs of a wave: a slice's codes (16 rows each),
+    static constexpr int SPG = ROWS / 64 / NW, SPW = ROWS / 64 / NW;                  // the scales of four slices (64 rows), or a quarter of them by words (16 rows)
+    static constexpr uint32_t CODE = ROWS * 64, SC = ROWS * 16, RING = NST * CODE, PITCH = BN * 4 + 16;
+    static constexpr int PASSES = BM * PITCH <= 81920 ? 1 : 2;                        // of the sums through LDS
+    static constexpr uint32_t STAGED = BM / PASSES * PITCH, LDS = RING + 3 * SC > STAGED ? RING + 3 * SC : STAGED;
+    static_assert(ROWS % (64 * NW) == 0 && SPG <= 2 && BN % 64 == 0 && BM % (32 * WGM) == 0 && BN % (32 * WGN) == 0 && LDS <= 163840, "tile");
 };
 
-template <int BM, int BN, int WGM, int WGN, int PER>
+template <int BM, int BN, int WGM, int WGN, int PER, bool A16>
 __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
     using T = Tile<BM, BN, WGM, WGN>;
-    constexpr int NW = T::NW, TM = T::TM, TN = T::TN, NST = T::NST, CPW = T::CPW, SPW = T::SPW;
+    constexpr int NW = T::NW, TM = T::TM, TN = T::TN, NST = T::NST, CPW = T::CPW, SPG = T::SPG, SPW = T::SPW;
     extern __shared__ __align__(16) uint8_t smem[];
     const uint32_t lds0 = sh_lds_addr(smem), sc0 = lds0 + T::RING;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WGM, wn = wave / WGM;
@@ -221,7 +234,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
     const uint8_t *wc = a.wc + (uint64_t)n0 * a.ldwc, *xc = a.xc + (uint64_t)m0 * a.ldxc, *ws = a.ws + (uint64_t)n0 * a.ldws, *xs = a.xs + (uint64_t)m0 * a.ldxs;
     const uint32_t wlim = a.N - 1 - n0, xlim = a.M - 1 - m0;
     const uint32_t ldwc = (uint32_t)a.ldwc, ldxc = (uint32_t)a.ldxc, ldws = (uint32_t)a.ldws, ldxs = (uint32_t)a.ldxs;
-    const uint32_t chunk = (lane & 3) ^ ((lane >> 3) & 3);
+    const uint32_t chunk = (lane & 3) ^ ((lane >> 3 ^ lane >> 5) & 3);
     uint32_t off[CPW];
 #pragma unroll
     for (int i = 0; i < CPW; ++i) {
@@ -239,38 +252,66 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
             sh_lds_dma16_s((ins * 16 < BN ? wc : xc) + 64ull * u, off[i] - back, slot + ins * 1024);
         }
     };
-    // part `q` of the scales of slices 4 gr .. 4 gr + 3
-    const auto load_scales = [&](uint32_t gr, uint32_t q) {
+    // Part `q` of the scales of slices 4 gr .. 4 gr + 3, of the last ones where there are none: rows of 16 bytes where these are aligned (A16), else words.
+    uint32_t soff[A16 ? SPG : 4 * SPW];
 #pragma unroll
-        for (int i = 0; i < SPW; ++i) {
-            const uint32_t ins = ((q * NW + wave) * SPW + i) % T::SCI, row = ins * 16 + (lane >> 2), d = 4 * min(4 * gr + (lane & 3), nd - 1);
-            const bool isw = ins * 16 < BN;
-            dma4_s(isw ? ws : xs, d + (isw ? min(row, wlim) * ldws : min(row - BN, xlim) * ldxs), sc0 + gr % 3 * T::SC + ins * 256);
+    for (int i = 0; i < (A16 ? SPG : 4 * SPW); ++i) {
+        const uint32_t ins = A16 ? wave * SPG + i : (i / SPW * NW + wave) * SPW + i % SPW, row = A16 ? ins * 64 + lane : ins * 16 + (lane >> 2);
+        soff[i] = row < BN ? min(row, wlim) * ldws : min(row - BN, xlim) * ldxs;
+    }
+    const auto load_scales = [&](uint32_t gr, auto part) {
+        constexpr int Q = decltype(part)::value;
+        const uint32_t at = sc0 + gr % 3 * T::SC;
+        if constexpr (A16) {
+            if constexpr (Q % 2 == 0 && Q / 2 < SPG) {
+                const uint32_t ins = wave * SPG + Q / 2;
+                sh_lds_dma16_s((ins * 64 < BN ? ws : xs) + 16 * min(gr, (nd - 1) / 4), soff[Q / 2], at + ins * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < SPW; ++i) {
+                const uint32_t ins = (Q * NW + wave) * SPW + i;
+                dma4_s(ins * 16 < BN ? ws : xs, soff[Q * SPW + i] + 4 * min(4 * gr + (lane & 3), nd - 1), at + ins * 256);
+            }
         }
     };
-    const uint32_t lane_at = r32 * 64 + ((2 * g) ^ ((lane >> 1) & 3)) * 16;
-    struct Ops { uint4 w[TN], x[TM]; };
-    const auto read = [&](uint32_t t, int j, Ops &o) {
-        const uint32_t at = lds0 + (t % NST) * T::CODE + (lane_at ^ (16 * j));
-#pragma unroll
-        for (int i = 0; i < TN; ++i) o.w[i] = lds16(at + (wn * TN + i) * 2048);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) o.x[i] = lds16(at + BN * 64 + (wm * TM + i) * 2048);
-    };
+    constexpr int W2 = 2 * CPW + (A16 ? SPG / 2 : 2 * SPW), W3 = 3 * CPW + (A16 ? SPG / 2 : 3 * SPW);      // DMAs of two and of three slices in a row, at least
+    const uint32_t lane_at = r32 * 64 + ((2 * g) ^ ((r32 >> 1 ^ (r32 >> 3 & 1)) & 3)) * 16;
+    struct Ops { sh_u4v w[TN], x[TM]; };
     struct Scales { uint32_t w[TN], x[TM]; };
-    const auto read_scales = [&](uint32_t t, Scales &s) {
-        const uint32_t at = sc0 + t / 4 % 3 * T::SC + r32 * 16 + 4 * (t & 3);
-#pragma unroll
-        for (int i = 0; i < TN; ++i) s.w[i] = lds4(at + (wn * TN + i) * 512);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) s.x[i] = lds4(at + BN * 16 + (wm * TM + i) * 512);
+    // read i of a step's operands (w0, the x, the other w), and of a slice's scales
+    const auto read = [&](uint32_t at, auto i, Ops &o) {
+        constexpr int I = decltype(i)::value;
+        if constexpr (I > 0 && I <= TM) o.x[I - 1] = lds16(at + BN * 64 + (wm * TM + I - 1) * 2048);
+        else { constexpr int W = I ? I - TM : 0; o.w[W] = lds16(at + (wn * TN + W) * 2048); }
     };
+    const auto read_scale = [&](uint32_t at, auto i, Scales &s) {
+        constexpr int I = decltype(i)::value;
+        if constexpr (I < TN) s.w[I] = lds4(at + (wn * TN + I) * 512);
+        else s.x[I - TN] = lds4(at + BN * 16 + (wm * TM + I - TN) * 512);
+    };
+    const auto ops_at = [&](uint32_t t, int j) { return lds0 + (t % NST) * T::CODE + (lane_at ^ (16 * j)); };
+    const auto scales_at = [&](uint32_t t) { return sc0 + t / 4 % 3 * T::SC + r32 * 16 + 4 * (t & 3); };
     const auto own_scales = [&](uint32_t t, Scales &s) {
-        const uint32_t sh = 16 * g, keep = 4 * t + 4 > nb ? (1u << (8 * (nb - 4 * t))) - 1 : ~0u;
+        const uint32_t keep = 4 * t + 4 > nb ? (1u << (8 * (nb - 4 * t))) - 1 : ~0u;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) s.w[i] = (s.w[i] & keep) >> sh;
+        for (int i = 0; i < TN; ++i) s.w[i] = (s.w[i] & keep) >> (16 * g);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) s.x[i] = (s.x[i] & keep) >> sh;
+        for (int i = 0; i < TM; ++i) s.x[i] = (s.x[i] & keep) >> (16 * g);
+    };
+    struct Group { sh_u4v w[TN], x[TM]; };
+    const auto read_group = [&](uint32_t at, auto i, Group &s) {
+        constexpr int I = decltype(i)::value;
+        if constexpr (I < TN) s.w[I] = lds16(at + (wn * TN + I) * 512);
+        else s.x[I - TN] = lds16(at + BN * 16 + (wm * TM + I - TN) * 512);
+    };
+    const auto pick = [&](auto part, const Group &v, Scales &s) {
+        constexpr int Q = decltype(part)::value;
+        const auto word = [&](const sh_u4v &u) { return u[Q] >> (16 * g); };
+#pragma unroll
+        for (int i = 0; i < TN; ++i) s.w[i] = word(v.w[i]);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) s.x[i] = word(v.x[i]);
     };
     sh_f16v acc[TN][TM];
 #pragma unroll
@@ -279,125 +320,170 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
         for (int k = 0; k < TM; ++k)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
+    // A step's products, with `between(e)` before each: what it issues stays there (the compiler would put all reads first, and no product
+    // is issued while LDS takes them).
+    constexpr int P = TN * TM;
     const auto multiply = [&](auto j, const Ops &o, const Scales &s, auto between) {
-#pragma unroll
-        for (int i = 0; i < TN; ++i) {
-            between(i);
-#pragma unroll
-            for (int k = 0; k < TM; ++k)
-                acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(o.w[i]), operand(o.x[k]), acc[i][k], E2M1, E2M1, decltype(j)::value, (int)s.w[i],
-                                                                           decltype(j)::value, (int)s.x[k]);
+        each<P>([&](auto e) {
+            constexpr int E = decltype(e)::value, I = E / TM, K = E % TM;
+            between(e);
+            acc[I][K] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(o.w[I]), operand(o.x[K]), acc[I][K], E2M1, E2M1, decltype(j)::value, (int)s.w[I],
+                                                                       decltype(j)::value, (int)s.x[K]);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
     };
-#pragma unroll
-    for (uint32_t q = 0; q < 4; ++q) load_scales(0, q);
-#pragma unroll
-    for (uint32_t u = 0; u < NST; ++u)
-        if (u < n) {
-            load_codes(u);
+    each<4>([&](auto q) { load_scales(0, q); });
+    each<NST>([&](auto u) {
+        if (decltype(u)::value < n) {
+            load_codes(decltype(u)::value);
             load_scales(1, u);
         }
-    if (n >= NST) sh_wait_vmcnt<3 * (CPW + SPW)>();
+    });
+    if (n >= NST) sh_wait_vmcnt<W3>();
     else sh_wait_vmcnt<0>();
     __syncthreads();
+    constexpr int R = TN + TM, SPREAD = P * 3 / 4;           // reads of a step, and the products that they are spread over
     Ops o0, o1;
     Scales s0, s1;
-    read(0, 0, o0);
-    read_scales(0, s0);
-    own_scales(0, s0);
-    // (no branch in a slice: the compiler would move products past the barrier)
-    const auto slice = [&](uint32_t t, auto more) {
-        read(t, 1, o1);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(std::integral_constant<int, 0>{}, o0, s0, [](int) {});
-        // the next slice has come, and this one's operands are all in registers
-        sh_wait_vmcnt<decltype(more)::value ? 2 * (CPW + SPW) : 0>();
+    {
+        const uint32_t at = ops_at(0, 0);
+        each<R>([&](auto i) { read(at, i, o0); });
+    }
+    // Between a slice's steps: the next slice has come, this one's operands are all in registers. (The barrier alone does not keep the compiler's
+    // loads on their side; and a branch within a slice lets it move products past the barrier.)
+    const auto turn = [&](auto waiting) {
+        sh_wait_vmcnt<decltype(waiting)::value>();
         sh_wait_lgkm0();
-        asm volatile("" ::: "memory");                      // (the barrier alone does not keep the compiler's loads on their side)
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const uint32_t nx = decltype(more)::value ? t + 1 : min(t + 1, n - 1);
-        read(nx, 0, o0);
-        read_scales(nx, s1);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(std::integral_constant<int, 1>{}, o1, s0, [&](int i) {
-            if constexpr (decltype(more)::value) {
-                load_codes(t + NST, i, TN);
-                if (i == TN - 1) load_scales(t / 4 + 2, t & 3);
-            }
+    };
+    uint32_t t = 0;
+    if (n >= 8) {                                            // four slices at a time, their scales in registers
+        Group ga, gb;
+        {
+            const uint32_t at = sc0 + r32 * 16;
+            each<R>([&](auto i) { read_group(at, i, ga); });
+        }
+        for (; t + 8 <= n; t += 4) {
+            const uint32_t gat = sc0 + (t / 4 + 1) % 3 * T::SC + r32 * 16;
+            each<4>([&](auto q) {
+                constexpr int Q = decltype(q)::value;
+                const uint32_t at1 = ops_at(Q, 1), at0 = ops_at(Q + 1, 0);
+                pick(q, ga, s0);
+                multiply(std::integral_constant<int, 0>{}, o0, s0, [&](auto e) {
+                    some<R, SPREAD>(e, [&](auto i) {
+                        read(at1, i, o1);
+                        if constexpr (Q == 3) read_group(gat, i, gb);
+                    });
+                });
+                turn(std::integral_constant<int, W2>{});
+                multiply(std::integral_constant<int, 1>{}, o1, s0, [&](auto e) {
+                    some<R, SPREAD>(e, [&](auto i) { read(at0, i, o0); });
+                    load_codes(t + Q + NST, decltype(e)::value, P);
+                    if constexpr (decltype(e)::value == P - 1) load_scales(t / 4 + 2, q);
+                });
+            });
+            ga = gb;
+        }
+    }
+    {
+        const uint32_t at = scales_at(t);
+        each<R>([&](auto i) { read_scale(at, i, s0); });
+        own_scales(t, s0);
+    }
+    const auto slice = [&](auto more) {
+        constexpr bool MORE = decltype(more)::value;
+        const uint32_t at1 = ops_at(t, 1), nx = min(t + 1, n - 1), at0 = ops_at(nx, 0), sat = scales_at(nx);
+        multiply(std::integral_constant<int, 0>{}, o0, s0, [&](auto e) { some<R, SPREAD>(e, [&](auto i) { read(at1, i, o1); }); });
+        turn(std::integral_constant<int, MORE ? W2 : 0>{});
+        multiply(std::integral_constant<int, 1>{}, o1, s0, [&](auto e) {
+            some<R, SPREAD>(e, [&](auto i) { read(at0, i, o0); read_scale(sat, i, s1); });
+            if constexpr (MORE) load_codes(t + NST, decltype(e)::value, P);
         });
         s0 = s1;
         own_scales(nx, s0);
     };
-    uint32_t t = 0;
-    for (; t + NST < n; ++t) slice(t, std::true_type{});
-    for (; t < n; ++t) slice(t, std::false_type{});
-    // The tile through LDS: bias and GELU in fp32, then whole rows of fp16 with the residual.
-    __syncthreads();
-    const uint32_t epi_lds = lds0;
+    for (; t + NST < n; ++t) slice(std::true_type{});        // (up to three, whose loads need no further scales)
+    for (; t < n; ++t) slice(std::false_type{});
+    // The sums through LDS, in as many passes as they need room, to whole rows: a thread has the same eight columns of every row that it
+    // finishes. (Finished where they are, 256 values a thread, they took 18 us of a tile's 85 in code that is run once.)
+    constexpr int PASSES = T::PASSES, KP = TM / PASSES;
+    constexpr uint32_t CH = BN / 8, RS = 64 * NW / CH, RP = 32 * KP;
+    const uint32_t c8 = threadIdx.x % CH * 8, nn = n0 + c8, left = nn < a.N ? min(a.N - nn, 8u) : 0u;
+    float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (a.bias)
+        for (uint32_t e = 0; e < left; ++e) {
+            const float b = a.bias_fp32 ? ((const float *)a.bias)[nn + e] : sh_dev_h2f(((const uint16_t *)a.bias)[nn + e]);
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint32_t nl = (wn * TN + i) * 32 + 8 * q + 4 * g;
-            float b[4] = {0.f, 0.f, 0.f, 0.f};
-            if (a.bias)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t nn = min(n0 + nl + e, a.N - 1);
-                    b[e] = a.bias_fp32 ? ((const float *)a.bias)[nn] : sh_dev_h2f(((const uint16_t *)a.bias)[nn]);
-                }
-#pragma unroll
-            for (int k = 0; k < TM; ++k) {
-                uint16_t h[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = acc[i][k][4 * q + e] + b[e];
-                    if (a.act == SH_ACT_GELU) v = sh_gelu_f32(v);
-                    h[e] = sh_dev_f2h_rr(v);
-                }
-                const uint32_t ml = (wm * TM + k) * 32 + r32;
-                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-                *(__attribute__((address_space(3))) u2 *)(uintptr_t)(epi_lds + ml * T::PITCH + nl * 2) = u2{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
-            }
+            for (uint32_t i = 0; i < 8; ++i) bias[i] = i == e ? b : bias[i];
         }
-    __syncthreads();
-    constexpr uint32_t CH = BN / 8;
-    for (uint32_t i = threadIdx.x; i < BM * CH; i += 64 * NW) {
-        const uint32_t r = i / CH, c = 8 * (i % CH), m = m0 + r, nn = n0 + c;
-        if (m >= a.M || nn >= a.N) continue;
-        uint4 v = lds16(epi_lds + r * T::PITCH + c * 2);
-        const uint32_t left = min(a.N - nn, 8u);
-        if (a.res) {
-            const uint16_t *p = a.res + m * a.ldr + nn;
-            uint4 q;
-            if (left == 8) q = sh_ld16_any(p);
-            else {
-                uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e)
-                    if (e < left) w[e / 2] |= (uint32_t)p[e] << (16 * (e & 1));
-                q = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int p = 0; p < PASSES; ++p) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < KP; ++k)
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const sh_f16v &v = acc[i][p * KP + k];
+                    *(__attribute__((address_space(3))) sh_f4v *)(uintptr_t)(lds0 + ((wm * KP + k) * 32 + r32) * T::PITCH + ((wn * TN + i) * 32 + 8 * q + 4 * g) * 4) =
+                        sh_f4v{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                }
+        __syncthreads();
+        const auto finish = [&](auto gelu) {
+            constexpr uint32_t U = 4;                            // rows at a time
+            static_assert(BM / PASSES % (U * RS) == 0, "rows");
+            for (uint32_t r0 = threadIdx.x / CH; r0 < BM / PASSES; r0 += U * RS) {
+                sh_f4v f[U][2];
+#pragma unroll
+                for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) f[u][e] = __builtin_bit_cast(sh_f4v, lds16(lds0 + (r0 + u * RS) * T::PITCH + c8 * 4 + 16 * e));
+#pragma unroll
+                for (uint32_t u = 0; u < U; ++u) {
+                    const uint32_t r = r0 + u * RS, m = m0 + r / RP * (32 * TM) + p * RP + r % RP;
+                    sh_u4v v;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        float x = f[u][e / 4][e % 4] + bias[e], y = f[u][e / 4][e % 4 + 1] + bias[e + 1];
+                        if constexpr (decltype(gelu)::value) { x = sh_gelu_f32(x); y = sh_gelu_f32(y); }
+                        asm("" : "+v"(x), "+v"(y));              // (rounded to fp32 before fp16, as sh_dev_f2h_rr)
+                        v[e / 2] = __builtin_bit_cast(uint32_t, sh_h2{(_Float16)x, (_Float16)y});
+                    }
+                    if (m >= a.M) continue;
+                    if (a.res) {
+                        const uint4 q = load8(a.res + m * a.ldr, nn, a.N);
+                        v = sh_u4v{sh_hadd2(v[0], q.x), sh_hadd2(v[1], q.y), sh_hadd2(v[2], q.z), sh_hadd2(v[3], q.w)};
+                    }
+                    sh_st8_any(a.z + m * a.ldz + nn, make_uint4(v[0], v[1], v[2], v[3]), left);
+                }
             }
-            v = make_uint4(sh_hadd2(v.x, q.x), sh_hadd2(v.y, q.y), sh_hadd2(v.z, q.z), sh_hadd2(v.w, q.w));
-        }
-        sh_st8_any(a.z + m * a.ldz + nn, v, left);
+        };
+        if (!left) continue;
+        if (a.act == SH_ACT_GELU) finish(std::true_type{});
+        else finish(std::false_type{});
     }
 }
 
-template <int BM, int BN, int WGM, int WGN, int PER>
-bool launch_tile(const MxArgs &a, hipStream_t st) {
+template <int BM, int BN, int WGM, int WGN, int PER, bool A16>
+bool launch_tile_as(const MxArgs &a, hipStream_t st) {
     using T = Tile<BM, BN, WGM, WGN>;
     static bool set = false;
     if (!set && T::LDS > 65536) {
-        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_mx4_tile<BM, BN, WGM, WGN, PER>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS),
+        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_mx4_tile<BM, BN, WGM, WGN, PER, A16>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS),
                        "sh_gemm_mx4 hipFuncSetAttribute")) return false;
         set = true;
     }
     const uint64_t tiles = (uint64_t)sh_cdiv(a.M, BM) * sh_cdiv(a.N, BN);
-    hipLaunchKernelGGL((k_mx4_tile<BM, BN, WGM, WGN, PER>), dim3((uint32_t)tiles), dim3(64 * T::NW), T::LDS, st, a);
+    hipLaunchKernelGGL((k_mx4_tile<BM, BN, WGM, WGN, PER, A16>), dim3((uint32_t)tiles), dim3(64 * T::NW), T::LDS, st, a);
     return true;
+}
+template <int BM, int BN, int WGM, int WGN, int PER>
+bool launch_tile(const MxArgs &a, hipStream_t st) {
+    const bool a16 = !(((uint64_t)a.xs | (uint64_t)a.ws | a.ldxs | a.ldws) % 16);
+    return a16 ? launch_tile_as<BM, BN, WGM, WGN, PER, true>(a, st) : launch_tile_as<BM, BN, WGM, WGN, PER, false>(a, st);
 }
 
 template <int MT, int NW, bool F16>
