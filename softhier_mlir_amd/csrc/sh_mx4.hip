@@ -93,84 +93,149 @@ __device__ __forceinline__ void store_one(const MxArgs &a, uint32_t m, uint32_t 
     a.z[m * a.ldz + n] = h;
 }
 
-// One row's blocks b .. b + 3 and their scales; zeros with a scale of 1 behind the last block.
-struct Four { sh_u4v c[4]; uint32_t s; };
-__device__ __forceinline__ uint32_t scales4(const uint8_t *p, uint32_t b, uint32_t nb) {
-    if (b >= nb) return ONES;
-    const uint32_t s = *(const uint32_t *)(p + b), left = nb - b;
-    if (left >= 4) return s;
-    const uint32_t m = (1u << (8 * left)) - 1;
-    return (s & m) | (ONES & ~m);
-}
-__device__ __forceinline__ void load_four(const uint8_t *codes, const uint8_t *scales, uint32_t b, uint32_t nb, Four &o) {
-    o.s = scales4(scales, b, nb);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o.c[j] = b + j < nb ? *(const sh_u4v *)(codes + 16ull * (b + j)) : sh_u4v{0, 0, 0, 0};
-}
-__device__ __forceinline__ void load_four_f16(const uint16_t *row, uint32_t b, uint32_t nb, uint32_t K, Four &o) {
-    o.s = ONES;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        o.c[j] = sh_u4v{0, 0, 0, 0};
-        if (b + j < nb) {
-            uint4 v[4];
-            us2 t = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = load8(row, 32 * (b + j) + 8 * i, K);
-                t = __builtin_elementwise_max(t, top8(v[i]));
-            }
-            const uint32_t e = scale_byte(max(t.x, t.y));
-            o.s = (o.s & ~(255u << (8 * j))) | e << (8 * j);
-            if (e < 255u) {
-                const float f = __uint_as_float(e << 23);
-                o.c[j] = sh_u4v{codes8(v[0], f), codes8(v[1], f), codes8(v[2], f), codes8(v[3], f)};
-            }
-        }
+// f(0), f(1), ..., f(N - 1) as compile-time numbers; and the part of them that falls to place E of P when they are spread evenly.
+template <int N, int B = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+    if constexpr (B < N) {
+        f(std::integral_constant<int, B>{});
+        each<N, B + 1>(f);
     }
+}
+template <int N, int P, typename E, typename F>
+__device__ __forceinline__ void some(E, F f) {
+    if constexpr (E::value < P) each<N * (E::value + 1) / P, N * E::value / P>(f);
 }
 
-// Few rows: a workgroup has 16 columns and 16 MT rows of z; its waves take units of 512 k in turn, and their sums are added in LDS in wave order.
-template <int MT, int NW, bool F16>
-__global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
-    __shared__ float s_z[NW][16 * MT][17];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const uint32_t col0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
-    const uint64_t wr = min(col0 + n, a.N - 1);
-    const uint32_t units = (a.nb + 15) / 16;
-    sh_f4v acc[MT];
+// What a lane has of a row's 16 blocks from b0: in step j block b0 + 4 j + g (the four lanes of a row read 64 bytes side by side; with four blocks side by
+// side for each lane a load touches 64 lines, and one row of 4096 x 14336 takes 14.5 us for 12.7), and the row's four words of scales. WHOLE: all
+// blocks are there; else zeros with a scale of 1 behind the last.
+constexpr int SU = 4;                      // steps of a unit
+struct Part { sh_u4v c[SU], s; };
+template <bool WHOLE>
+__device__ __forceinline__ void load_part(const uint8_t *codes, const uint8_t *scales, uint32_t b0, uint32_t g, uint32_t nb, Part &o) {
+    if constexpr (WHOLE) {
+        typedef sh_u4v words __attribute__((aligned(4)));
+        o.s = *(const words *)(scales + b0);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = sh_f4v{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t u = wave; u < units; u += NW) {
-        const uint32_t b = 16 * u + 4 * g;
-        Four w, x[MT];
-        load_four(a.wc + wr * a.ldwc, a.ws + wr * a.ldws, b, a.nb, w);
+        for (int j = 0; j < SU; ++j) o.c[j] = *(const sh_u4v *)(codes + 16ull * (b0 + 4 * j + g));
+    } else {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const uint64_t xr = min(m0 + 16 * i + n, a.M - 1);
-            if constexpr (F16) load_four_f16(a.x + xr * a.ldx, b, a.nb, a.K, x[i]);
-            else load_four(a.xc + xr * a.ldxc, a.xs + xr * a.ldxs, b, a.nb, x[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.c[0]), operand(x[i].c[0]), acc[i], E2M1, E2M1, 0, (int)w.s, 0, (int)x[i].s);
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.c[1]), operand(x[i].c[1]), acc[i], E2M1, E2M1, 1, (int)w.s, 1, (int)x[i].s);
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.c[2]), operand(x[i].c[2]), acc[i], E2M1, E2M1, 2, (int)w.s, 2, (int)x[i].s);
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w.c[3]), operand(x[i].c[3]), acc[i], E2M1, E2M1, 3, (int)w.s, 3, (int)x[i].s);
+        for (int j = 0; j < SU; ++j) {
+            const uint32_t b = b0 + 4 * j;
+            o.s[j] = b < nb ? *(const uint32_t *)(scales + b) : ONES;
+            o.c[j] = b + g < nb ? *(const sh_u4v *)(codes + 16ull * (b + g)) : sh_u4v{0, 0, 0, 0};
         }
     }
+}
+// The scales of the lane's own four blocks in a word.
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t gather(const Part &o, uint32_t b0, uint32_t g, uint32_t nb) {
+    const uint32_t sel = 0x0C0C0400u + 0x0101u * g;
+    uint32_t s = __builtin_amdgcn_perm(__builtin_amdgcn_perm(o.s[3], o.s[2], sel), __builtin_amdgcn_perm(o.s[1], o.s[0], sel), 0x05040100u);
+    if constexpr (!WHOLE)
+#pragma unroll
+        for (int j = 0; j < SU; ++j)
+            if (b0 + 4 * j + g >= nb) s = (s & ~(255u << (8 * j))) | 127u << (8 * j);
+    return s;
+}
+// The same of a row of halves: the scales' word, and the codes.
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t load_part_f16(const uint16_t *row, uint32_t b0, uint32_t g, uint32_t nb, uint32_t K, Part &o) {
+    uint32_t s = WHOLE ? 0u : ONES;
+    uint4 v[SU][4];
+#pragma unroll
+    for (int j = 0; j < SU; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t k = 32 * (b0 + 4 * j + g) + 8 * i;
+            v[j][i] = WHOLE ? sh_ld16_any(row + k) : load8(row, k, K);
+        }
+#pragma unroll
+    for (int j = 0; j < SU; ++j) {
+        if (!WHOLE && b0 + 4 * j + g >= nb) {
+            o.c[j] = sh_u4v{0, 0, 0, 0};
+            continue;
+        }
+        const us2 t = __builtin_elementwise_max(__builtin_elementwise_max(top8(v[j][0]), top8(v[j][1])), __builtin_elementwise_max(top8(v[j][2]), top8(v[j][3])));
+        const uint32_t e = scale_byte(max(t.x, t.y));
+        s = WHOLE ? s | e << (8 * j) : (s & ~(255u << (8 * j))) | e << (8 * j);
+        const float f = __uint_as_float(e << 23);            // (255: infinity, whose codes are put right)
+        o.c[j] = sh_u4v{codes8(v[j][0], f), codes8(v[j][1], f), codes8(v[j][2], f), codes8(v[j][3], f)};
+        if (e == 255u) o.c[j] = sh_u4v{0, 0, 0, 0};
+    }
+    return s;
+}
+
+// Few rows: a workgroup has 16 CW columns and 16 MT rows of z; its waves take units of 512 k in turn, and their sums are added in LDS in wave order.
+template <int MT, int CW, int NW, bool F16>
+__global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
+    constexpr uint32_t LC = 16 * CW + 1;
+    extern __shared__ float s_z[];                                             // [NW][rows][LC]
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const uint32_t col0 = blockIdx.x * 16 * CW, m0 = blockIdx.y * 16 * MT, nrow = min(a.M - m0, 16u * MT);
+    const uint32_t units = (a.nb + 4 * SU - 1) / (4 * SU);
+    const uint8_t *wc[CW], *ws[CW], *xc[MT], *xs[MT];
+    const uint16_t *xh[MT];
+#pragma unroll
+    for (int k = 0; k < CW; ++k) {
+        const uint64_t r = min(col0 + 16 * k + n, a.N - 1);
+        wc[k] = a.wc + r * a.ldwc; ws[k] = a.ws + r * a.ldws;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const uint64_t r = min(m0 + 16 * i + n, a.M - 1);
+        xc[i] = a.xc + r * a.ldxc; xs[i] = a.xs + r * a.ldxs; xh[i] = a.x + r * a.ldx;
+    }
+    sh_f4v acc[CW][MT];
+#pragma unroll
+    for (int k = 0; k < CW; ++k)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[k][i] = sh_f4v{0.f, 0.f, 0.f, 0.f};
+    const auto unit = [&](uint32_t u, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        const uint32_t b0 = 4 * SU * u;
+        Part w[CW], x[MT];
+        int sx[MT];
+#pragma unroll
+        for (int k = 0; k < CW; ++k) load_part<WHOLE>(wc[k], ws[k], b0, g, a.nb, w[k]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if constexpr (F16) sx[i] = (int)load_part_f16<WHOLE>(xh[i], b0, g, a.nb, a.K, x[i]);
+            else load_part<WHOLE>(xc[i], xs[i], b0, g, a.nb, x[i]);
+        }
+        if constexpr (!F16)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) sx[i] = (int)gather<WHOLE>(x[i], b0, g, a.nb);
+#pragma unroll
+        for (int k = 0; k < CW; ++k) {
+            const int sw = (int)gather<WHOLE>(w[k], b0, g, a.nb);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                each<SU>([&](auto j) {
+                    constexpr int J = decltype(j)::value;
+                    acc[k][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w[k].c[J]), operand(x[i].c[J]), acc[k][i], E2M1, E2M1, J, sw, J, sx[i]);
+                });
+        }
+    };
+    const uint32_t full = F16 ? a.K / (128 * SU) : a.nb / (4 * SU);            // units with all of their blocks (halves)
+    uint32_t u = wave;
+    for (; u < full; u += NW) unit(u, std::true_type{});
+    if (u < units) unit(u, std::false_type{});
     // lane (m, g): the columns 4 g .. 4 g + 3 of row m
 #pragma unroll
     for (int i = 0; i < MT; ++i)
+        if (16 * i + n < nrow)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s_z[wave][16 * i + n][4 * g + e] = acc[i][e];
+            for (int k = 0; k < CW; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s_z[(wave * nrow + 16 * i + n) * LC + 16 * k + 4 * g + e] = acc[k][i][e];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 256 * MT; i += 64 * NW) {
-        const uint32_t r = i / 16, c = i % 16;
-        if (m0 + r >= a.M || col0 + c >= a.N) continue;
+    for (uint32_t i = threadIdx.x; i < nrow * 16 * CW; i += 64 * NW) {
+        const uint32_t r = i / (16 * CW), c = i % (16 * CW);
+        if (col0 + c >= a.N) continue;
         float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < NW; ++k) v += s_z[k][r][c];
+        for (int k = 0; k < NW; ++k) v += s_z[(k * nrow + r) * LC + c];
         store_one(a, m0 + r, col0 + c, v);
     }
 }
@@ -189,28 +254,16 @@ __device__ __forceinline__ void dma4_s(const void *base, uint32_t off, uint32_t 
 __device__ __forceinline__ sh_u4v lds16(uint32_t addr) { return *(const __attribute__((address_space(3))) sh_u4v *)(uintptr_t)addr; }
 __device__ __forceinline__ uint32_t lds4(uint32_t addr) { return *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)addr; }
 
-// f(0), f(1), ..., f(N - 1) as compile-time numbers; and the part of them that falls to place E of P when they are spread evenly.
-template <int N, int B = 0, typename F>
-__device__ __forceinline__ void each(F f) {
-    if constexpr (B < N) {
-        f(std::integral_constant<int, B>{});
-        each<N, B + 1>(f);
-    }
-}
-template <int N, int P, typename E, typename F>
-__device__ __forceinline__ void some(E, F f) {
-    if constexpr (E::value < P) each<N * (E::value + 1) / P, N * E::value / P>(f);
-}
-
 template <int BM, int BN, int WGM, int WGN>
 struct Tile {
     static constexpr int NW = WGM * WGN, TM = BM / WGM / 32, TN = BN / WGN / 32, NST = 4, ROWS = BM + BN;
     static constexpr int CPW = ROWS / 16 / NW;                                        // DMAs of a wave: a slice's codes (16 rows each),
-    static constexpr int SPG = ROWS / 64 / NW, SPW = ROWS / 64 / NW;                  // the scales of four slices (64 rows), or a quarter of them by words (16 rows)
+    static constexpr int SPG = (ROWS / 64 + NW - 1) / NW, SPW = SPG;                  // the scales of four slices (64 rows), or a quarter of them by words (16 rows);
+                                                                                      // where there are fewer than waves, some are loaded twice
     static constexpr uint32_t CODE = ROWS * 64, SC = ROWS * 16, RING = NST * CODE, PITCH = BN * 4 + 16;
     static constexpr int PASSES = BM * PITCH <= 81920 ? 1 : 2;                        // of the sums through LDS
     static constexpr uint32_t STAGED = BM / PASSES * PITCH, LDS = RING + 3 * SC > STAGED ? RING + 3 * SC : STAGED;
-    static_assert(ROWS % (64 * NW) == 0 && SPG <= 2 && BN % 64 == 0 && BM % (32 * WGM) == 0 && BN % (32 * WGN) == 0 && LDS <= 163840, "tile");
+    static_assert(ROWS % (16 * NW) == 0 && SPG <= 2 && BN % 64 == 0 && TM % PASSES == 0 && BM % (32 * WGM) == 0 && BN % (32 * WGN) == 0 && LDS <= 163840, "tile");
 };
 
 template <int BM, int BN, int WGM, int WGN, int PER, bool A16>
@@ -256,7 +309,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
     uint32_t soff[A16 ? SPG : 4 * SPW];
 #pragma unroll
     for (int i = 0; i < (A16 ? SPG : 4 * SPW); ++i) {
-        const uint32_t ins = A16 ? wave * SPG + i : (i / SPW * NW + wave) * SPW + i % SPW, row = A16 ? ins * 64 + lane : ins * 16 + (lane >> 2);
+        const uint32_t ins = A16 ? (wave * SPG + i) % (T::ROWS / 64) : ((i / SPW * NW + wave) * SPW + i % SPW) % (T::ROWS / 16), row = A16 ? ins * 64 + lane : ins * 16 + (lane >> 2);
         soff[i] = row < BN ? min(row, wlim) * ldws : min(row - BN, xlim) * ldxs;
     }
     const auto load_scales = [&](uint32_t gr, auto part) {
@@ -264,13 +317,13 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
         const uint32_t at = sc0 + gr % 3 * T::SC;
         if constexpr (A16) {
             if constexpr (Q % 2 == 0 && Q / 2 < SPG) {
-                const uint32_t ins = wave * SPG + Q / 2;
+                const uint32_t ins = (wave * SPG + Q / 2) % (T::ROWS / 64);
                 sh_lds_dma16_s((ins * 64 < BN ? ws : xs) + 16 * min(gr, (nd - 1) / 4), soff[Q / 2], at + ins * 1024);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < SPW; ++i) {
-                const uint32_t ins = (Q * NW + wave) * SPW + i;
+                const uint32_t ins = ((Q * NW + wave) * SPW + i) % (T::ROWS / 16);
                 dma4_s(ins * 16 < BN ? ws : xs, soff[Q * SPW + i] + 4 * min(4 * gr + (lane & 3), nd - 1), at + ins * 256);
             }
         }
@@ -342,7 +395,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
     if (n >= NST) sh_wait_vmcnt<W3>();
     else sh_wait_vmcnt<0>();
     __syncthreads();
-    constexpr int R = TN + TM, SPREAD = P * 3 / 4;           // reads of a step, and the products that they are spread over
+    constexpr int R = TN + TM, SPREAD = P > 1 ? P * 3 / 4 : 1;           // reads of a step, and the products that they are spread over
     Ops o0, o1;
     Scales s0, s1;
     {
@@ -396,7 +449,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
         constexpr bool MORE = decltype(more)::value;
         const uint32_t at1 = ops_at(t, 1), nx = min(t + 1, n - 1), at0 = ops_at(nx, 0), sat = scales_at(nx);
         multiply(std::integral_constant<int, 0>{}, o0, s0, [&](auto e) { some<R, SPREAD>(e, [&](auto i) { read(at1, i, o1); }); });
-        turn(std::integral_constant<int, MORE ? W2 : 0>{});
+        turn(std::integral_constant<int, MORE ? 2 * CPW : 0>{});      // (these load no scales)
         multiply(std::integral_constant<int, 1>{}, o1, s0, [&](auto e) {
             some<R, SPREAD>(e, [&](auto i) { read(at0, i, o0); read_scale(sat, i, s1); });
             if constexpr (MORE) load_codes(t + NST, decltype(e)::value, P);
@@ -433,7 +486,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
                 }
         __syncthreads();
         const auto finish = [&](auto gelu) {
-            constexpr uint32_t U = 4;                            // rows at a time
+            constexpr uint32_t U = BM / PASSES / RS < 4 ? BM / PASSES / RS : 4;      // rows at a time
             static_assert(BM / PASSES % (U * RS) == 0, "rows");
             for (uint32_t r0 = threadIdx.x / CH; r0 < BM / PASSES; r0 += U * RS) {
                 sh_f4v f[U][2];
@@ -486,9 +539,32 @@ bool launch_tile(const MxArgs &a, hipStream_t st) {
     return a16 ? launch_tile_as<BM, BN, WGM, WGN, PER, true>(a, st) : launch_tile_as<BM, BN, WGM, WGN, PER, false>(a, st);
 }
 
-template <int MT, int NW, bool F16>
-void launch_rows(const MxArgs &a, hipStream_t st) {
-    hipLaunchKernelGGL((k_mx4_rows<MT, NW, F16>), dim3(sh_cdiv(a.N, 16), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), 0, st, a);
+template <int MT, int CW, int NW, bool F16>
+bool launch_rows_as(const MxArgs &a, hipStream_t st) {
+    constexpr uint32_t most = NW * 16 * MT * (16 * CW + 1) * 4;
+    static bool set = false;
+    if (!set && most > 65536) {
+        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_mx4_rows<MT, CW, NW, F16>, hipFuncAttributeMaxDynamicSharedMemorySize, most),
+                       "sh_gemm_mx4 hipFuncSetAttribute")) return false;
+        set = true;
+    }
+    const uint32_t lds = NW * std::min(a.M, 16u * MT) * (16 * CW + 1) * 4;
+    hipLaunchKernelGGL((k_mx4_rows<MT, CW, NW, F16>), dim3(sh_cdiv(a.N, 16 * CW), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), lds, st, a);
+    return true;
+}
+// Columns and waves of a workgroup, by N and K. Many columns: wider workgroups, which read x (and bring it into codes) less often: 4096 x 14336, one row 8.6 us with
+// 16 columns, 7.9 with 32, 8.4 with 64; of halves 12.8 / 9.8 / 9.3, 16 rows of halves 22.1 / 14.9 / 12.2; 30 rows of 4096 x 8192 9.2 / 7.5. Fewer columns need every
+// workgroup: 4096 x 4096 5.1 / 6.0 / 8.6. A long chain over them is shared by sixteen waves: halves, 14336 x 4096 15.1 us with eight, 12.6 with sixteen,
+// 16384 x 1024 11.5 / 10.5; at K = 8192 and below they are level.
+template <int MT, bool F16>
+bool launch_rows(const MxArgs &a, hipStream_t st) {
+    if constexpr (F16)
+        if (a.N > 8192) return launch_rows_as<MT, 4, 8, F16>(a, st);
+    if constexpr (!F16 && MT < 4)
+        if (a.N >= 8192) return launch_rows_as<MT, 2, 8, F16>(a, st);
+    if constexpr (MT == 1)
+        if (a.K > 8192) return launch_rows_as<MT, 1, 16, F16>(a, st);
+    return launch_rows_as<MT, 1, 8, F16>(a, st);
 }
 
 // The checks that both products make of the weight, the result and the epilogue.
@@ -556,12 +632,31 @@ int sh_gemm_mx4(uint64_t xc, uint64_t xs, uint64_t wc, uint64_t ws, uint64_t z, 
     a.xc = (const uint8_t *)xc; a.xs = (const uint8_t *)xs;
     a.ldxc = ldxc; a.ldxs = ldxs;
     const hipStream_t st = sh_stream();
+    // Tiles by the rounds of workgroups that they take on 256 CUs. Times (us, K = 4096, epilogue without residual) of the first round and of a further one: small
+    // tiles' workgroups share a CU. 2048 x 4096: 47 / 40 / 30 / 27.5 / 31.5; 1000 x 2048: 14.4 / 13.6 / 15.0 / 21 / 29; 300 x 4096: 12.0 / 11.8 / 13.7 / 20 / 27;
+    // 100 x 4096: 8.0 / 10.3 / 12.0 / 17 / 24; 700 x 5000 (K = 2880): 22 / 18.5 / 15.3 / 19.7 / 26; 4096 x 4096: 87 / 70 / 55 / 51 / 41.
+    struct Shape { uint32_t bm, bn; double first, more; };
+    static const Shape shapes[] = {{64, 64, 8, 6}, {64, 128, 11.5, 9.5}, {128, 128, 14.5, 14.5}, {128, 256, 26, 26}, {256, 256, 39, 39}};
+    int pick = 0;
+    double least = 0;
+    for (int i = 0; i < 5; ++i) {
+        const uint64_t tiles = (uint64_t)sh_cdiv(M, shapes[i].bm) * sh_cdiv(N, shapes[i].bn);
+        const double c = shapes[i].first + shapes[i].more * (double)((tiles - 1) / 256);
+        if (!i || c < least) { pick = i; least = c; }
+    }
     const bool near = ldxc <= (1u << 24) && ldwc <= (1u << 24) && ldxs <= (1u << 24) && ldws <= (1u << 24);       // a tile's rows within 32-bit offsets
-    const uint64_t big = (uint64_t)sh_cdiv(M, 256) * sh_cdiv(N, 256), mid = (uint64_t)sh_cdiv(M, 128) * sh_cdiv(N, 128);
-    if (M <= 16) launch_rows<1, 8, false>(a, st);
-    else if (M <= 64 || !near || mid > (1u << 22)) launch_rows<4, 8, false>(a, st);
-    else if (big >= 256) { if (!launch_tile<256, 256, 2, 2, 1>(a, st)) return SH_EHIP; }
-    else if (!launch_tile<128, 128, 2, 2, 2>(a, st)) return SH_EHIP;
+    bool ok = true;
+    // Up to 64 rows the chain is shared by a workgroup's waves; more than 32 of many columns fill the GPU as tiles (64 rows of 4096 x 14336: 10.9 us, 29.6 so; 50
+    // of 8192 x 4096 15.5 against 13.9).
+    if (M <= 16) ok = launch_rows<1, false>(a, st);
+    else if (M <= 32) ok = launch_rows<2, false>(a, st);
+    else if ((M <= 64 && N <= 4096) || !near) ok = launch_rows<4, false>(a, st);
+    else if (pick == 0) ok = launch_tile<64, 64, 2, 2, 2>(a, st);
+    else if (pick == 1) ok = launch_tile<64, 128, 2, 2, 2>(a, st);
+    else if (pick == 2) ok = launch_tile<128, 128, 2, 2, 2>(a, st);
+    else if (pick == 3) ok = launch_tile<128, 256, 2, 4, 2>(a, st);
+    else ok = launch_tile<256, 256, 4, 2, 2>(a, st);
+    if (!ok) return SH_EHIP;
     return sh_launch_ok("sh_gemm_mx4") ? 0 : SH_EHIP;
 }
 
@@ -573,7 +668,7 @@ int sh_gemm_mx4_f16(uint64_t x, uint64_t wc, uint64_t ws, uint64_t z, uint32_t M
     if (!x || x % 2 || ldx < K) { sh_set_error(-1, "[sh_gemm_mx4_f16] x: NULL, not 2-byte aligned, or leading dim %u < %u", ldx, K); return -1; }
     if (M > 16) { sh_set_error(-1, "[sh_gemm_mx4_f16] %u rows (up to 16; more by sh_mx4_quant and sh_gemm_mx4)", M); return -1; }
     a.x = (const uint16_t *)x; a.ldx = ldx;
-    launch_rows<1, 8, true>(a, sh_stream());
+    if (!launch_rows<1, true>(a, sh_stream())) return SH_EHIP;
     return sh_launch_ok("sh_gemm_mx4_f16") ? 0 : SH_EHIP;
 }
 
