@@ -360,8 +360,10 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
 
 // ---- sh_kv_append_rope ----------------------------------------------------------------------------------------------
 // The same with keys turned by their rows' positions before they are codes, and the queries' heads turned in the launch's last
-// workgroups. A thread's eight columns of a key are four pairs of each of its four tokens, and it keeps their cosines and sines for `kh` heads:
-// they cost more than all else here (fp64, about 180 cycles a wave each).
+// workgroups. A thread's eight columns of a key are four pairs of each of its four tokens, and it keeps their cosines and sines (fp64, about 180
+// cycles a wave each) for `kh` heads, the next head's halves on their way while one is stored: of 17 thousand rows of 32 + 8 heads of 128, 78.6 us (4.1 TB/s) with
+// four heads, 82.2 with two, 126 with one. Three waves a SIMD hold too little in flight for more: queries spread among the workgroups that append, so that both
+// run at once, made it slower (88.5). 64 single rows 5.6 us, one launch: slots and positions, then rows and scales, then codes.
 struct AppendRopeArgs {
     AppendArgs a;
     RopeArgs q;                            // rows turned for themselves
@@ -408,24 +410,35 @@ __global__ __launch_bounds__(NT) void k_kv_append_rope(AppendRopeArgs g) {
         uint32_t ca, cb;
         rope_columns<4>(g.q.p, ch, ca, cb);
         const bool turned = ch < g.q.p.rot / 8;
-        float cs[4][4], sn[4][4];
+        uint32_t w[4][4];                                            // a head's halves, on their way while the last one is stored
+        const auto load = [&]() {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t t = t0 + j;
+                w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;
+                if (mine && t >= u.off && t < u.end) {
+                    rope_load<4>(src + (uint64_t)(t - u.off) * ld + ca, w[j]);
+                    rope_load<4>(src + (uint64_t)(t - u.off) * ld + cb, w[j] + 2);
+                }
+            }
+        };
+        load();
+        float cs[4][4] = {}, sn[4][4] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t t = t0 + j;
             if (mine && turned && t >= u.off && t < u.end) rope_angles<4>(g.q.p, ch, (uint32_t)g.q.pos[u.r + t - u.off], cs[j], sn[j]);
         }
-        for (uint32_t h = h0; h < h1; ++h, src += dh) {
+        for (uint32_t h = h0; h < h1; ++h) {
             uint4 x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t t = t0 + j;
-                uint32_t w[4] = {0, 0, 0, 0};
-                if (mine && t >= u.off && t < u.end) {
-                    rope_load<4>(src + (uint64_t)(t - u.off) * ld + ca, w);
-                    rope_load<4>(src + (uint64_t)(t - u.off) * ld + cb, w + 2);
-                    if (turned) rope_turn<4>(w, g.q.p.pairs, cs[j], sn[j]);
-                }
-                x[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                if (turned) rope_turn<4>(w[j], g.q.p.pairs, cs[j], sn[j]);      // (zeros stay zeros where no row is)
+                x[j] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+            }
+            if (h + 1 < h1) {
+                src += dh;
+                load();
             }
             append_page<FP8, NT, true>(c, 0, h, u, blk0, t0, ca, cb, mine, x, s_top);
         }
@@ -459,7 +472,7 @@ void launch_append_rope_nt(AppendRopeArgs g, hipStream_t st) {
     const uint32_t heads = g.kg + g.a.c.hkv, chunks = g.a.c.dh / 8, rows = g.a.rows;
     g.a.dheads = sh_make_div(heads);
     const uint64_t all = (uint64_t)rows * g.q.heads * chunks;
-    g.q.hs = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(g.q.heads, all >> 18));
+    g.q.hs = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(g.q.heads, all >> 19));
     const uint32_t groups = sh_cdiv(g.q.heads, g.q.hs);
     g.q.dch = sh_make_div(chunks);
     g.q.dhg = sh_make_div(std::max(groups, 1u));

@@ -1,6 +1,7 @@
 // Rotary positions: what sh_rope_pos and sh_kv_append_rope share (not part of the C ABI).
 #pragma once
 #include "sh_common.h"
+#include <type_traits>
 
 // A checked sh_rope_plan.
 struct RopePlan {
@@ -127,14 +128,25 @@ __device__ __forceinline__ void rope_rows(const RopeArgs &a, uint32_t item) {
             y[cb] = v;
         }
     } else {
-#pragma unroll 2
-        for (uint32_t h = h0; h < h1; ++h, x += a.dh, y += a.dh) {
-            uint32_t w[P];
-            rope_load<P>(x + ca, w);
-            rope_load<P>(x + cb, w + P / 2);
-            if (turned) rope_turn<P>(w, a.p.pairs, c, s);
-            rope_store<P>(y + ca, w);
-            rope_store<P>(y + cb, w + P / 2);
-        }
+        const auto heads = [&](auto count) {                         // some heads at once: their loads are on their way together
+            constexpr int N = decltype(count)::value;
+            uint32_t w[N][P];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                rope_load<P>(x + i * a.dh + ca, w[i]);
+                rope_load<P>(x + i * a.dh + cb, w[i] + P / 2);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (turned) rope_turn<P>(w[i], a.p.pairs, c, s);
+                rope_store<P>(y + i * a.dh + ca, w[i]);
+                rope_store<P>(y + i * a.dh + cb, w[i] + P / 2);
+            }
+            x += N * a.dh;
+            y += N * a.dh;
+        };
+        uint32_t h = h0;
+        for (; h + 4 <= h1; h += 4) heads(std::integral_constant<int, 4>{});
+        for (; h < h1; ++h) heads(std::integral_constant<int, 1>{});
     }
 }
