@@ -213,15 +213,22 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
 // One page's new rows: first row, page, offsets [off, end).
 struct AppendRun { uint32_t r, page, off, end; };
 
+// A head's part of a page: its codes and its scale, read before the rows are.
+struct AppendTo { uint8_t *dst; float *sp, was; };
+__device__ __forceinline__ AppendTo append_to(const KvCache &c, uint32_t isv, uint32_t h, const AppendRun &u) {
+    float *sp = (isv ? c.vs : c.ks) + (uint64_t)u.page * c.pgs + h;
+    return AppendTo{(isv ? c.v + u.page * c.pgv : c.k + u.page * c.pgk) + (uint64_t)h * c.bs * c.dh, sp, u.off ? *sp : 0.f};
+}
+
 // What a thread holds of a page: four tokens from t0 by eight columns, four of them from ca and four from cb (SPLIT), or all from ca. `items`
 // threads hold something. Finds the scale, rounds older tokens again where it grew, and stores the codes.
 template <bool FP8, int NT, bool SPLIT>
-__device__ __forceinline__ void append_page(const KvCache &c, uint32_t isv, uint32_t h, const AppendRun &u, uint32_t blk0, uint32_t t0, uint32_t ca, uint32_t cb,
+__device__ __forceinline__ void append_page(const KvCache &c, uint32_t isv, const AppendTo &to, const AppendRun &u, uint32_t blk0, uint32_t t0, uint32_t ca, uint32_t cb,
                                             bool mine, uint4 (&x)[4], uint32_t *s_top) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, dh = c.dh, off = u.off, end = u.end;
-    uint8_t *dst = (isv ? c.v + u.page * c.pgv : c.k + u.page * c.pgk) + (uint64_t)h * c.bs * dh;
-    float *sp = (isv ? c.vs : c.ks) + (uint64_t)u.page * c.pgs + h;
-    const float was = off ? *sp : 0.f;
+    uint8_t *dst = to.dst;
+    float *sp = to.sp;
+    const float was = to.was;
     // the largest |x| as an integer (halves without their sign are ordered like their bits); only if a NaN or an infinity is
     // among them are these put right, and it is taken again
     uint32_t top;
@@ -345,6 +352,7 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
         lead &= lead - 1;
         const AppendRun u = append_run(c, a.rows, r0, f, sl, [&](uint32_t r) { return (uint32_t)a.slots[r]; });
         const uint16_t *src = (isv ? a.v : a.k) + (uint64_t)u.r * ld + (uint64_t)h * dh;
+        const AppendTo to = append_to(c, isv, h, u);
         uint4 x[4];
         const uint32_t blk0 = u.off / 4, items = ((u.end + 3) / 4 - blk0) * nch;
         const uint32_t bl = sh_div(tid, a.dch), ch = tid - bl * nch, t0 = 4 * (blk0 + bl);
@@ -352,9 +360,9 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
         for (int j = 0; j < 4; ++j) {
             const uint32_t t = t0 + j;
             x[j] = make_uint4(0, 0, 0, 0);
-            if (tid < items && t >= u.off && t < u.end) x[j] = sh_ld16_any(src + (uint64_t)(t - u.off) * ld + 8 * ch);
+            if ((tid < items) & (t >= u.off) & (t < u.end)) x[j] = sh_ld16_any(src + (uint64_t)(t - u.off) * ld + 8 * ch);
         }
-        append_page<FP8, NT, false>(c, isv, h, u, blk0, t0, 8 * ch, 0, tid < items, x, s_top);
+        append_page<FP8, NT, false>(c, isv, to, u, blk0, t0, 8 * ch, 0, tid < items, x, s_top);
     }
 }
 
@@ -396,15 +404,16 @@ __global__ __launch_bounds__(NT) void k_kv_append_rope(AppendRopeArgs g) {
         const uint32_t blk0 = u.off / 4, items = ((u.end + 3) / 4 - blk0) * nch;
         const uint32_t bl = sh_div(tid, a.dch), ch = tid - bl * nch, t0 = 4 * (blk0 + bl);
         const bool mine = tid < items;
+        AppendTo to = append_to(c, isv, h0, u);
         if (isv) {
             uint4 x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t t = t0 + j;
                 x[j] = make_uint4(0, 0, 0, 0);
-                if (mine && t >= u.off && t < u.end) x[j] = sh_ld16_any(src + (uint64_t)(t - u.off) * ld + 8 * ch);
+                if (mine & (t >= u.off) & (t < u.end)) x[j] = sh_ld16_any(src + (uint64_t)(t - u.off) * ld + 8 * ch);
             }
-            append_page<FP8, NT, false>(c, 1, h0, u, blk0, t0, 8 * ch, 0, mine, x, s_top);
+            append_page<FP8, NT, false>(c, 1, to, u, blk0, t0, 8 * ch, 0, mine, x, s_top);
             continue;
         }
         uint32_t ca, cb;
@@ -416,7 +425,7 @@ __global__ __launch_bounds__(NT) void k_kv_append_rope(AppendRopeArgs g) {
             for (int j = 0; j < 4; ++j) {
                 const uint32_t t = t0 + j;
                 w[j][0] = w[j][1] = w[j][2] = w[j][3] = 0;
-                if (mine && t >= u.off && t < u.end) {
+                if (mine & (t >= u.off) & (t < u.end)) {
                     rope_load<4>(src + (uint64_t)(t - u.off) * ld + ca, w[j]);
                     rope_load<4>(src + (uint64_t)(t - u.off) * ld + cb, w[j] + 2);
                 }
@@ -436,11 +445,13 @@ __global__ __launch_bounds__(NT) void k_kv_append_rope(AppendRopeArgs g) {
                 if (turned) rope_turn<4>(w[j], g.q.p.pairs, cs[j], sn[j]);      // (zeros stay zeros where no row is)
                 x[j] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
             }
+            const AppendTo here = to;
             if (h + 1 < h1) {
                 src += dh;
+                to = append_to(c, 0, h + 1, u);
                 load();
             }
-            append_page<FP8, NT, true>(c, 0, h, u, blk0, t0, ca, cb, mine, x, s_top);
+            append_page<FP8, NT, true>(c, 0, here, u, blk0, t0, ca, cb, mine, x, s_top);
         }
     }
 }

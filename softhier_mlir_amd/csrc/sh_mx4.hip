@@ -56,7 +56,7 @@ struct QuantArgs {
     ShDiv dch;                             // by a row's 16-byte pieces
 };
 
-// A lane has 8 columns, four lanes a block.
+// A lane has 8 columns, four lanes a block. Bound by HBM (8192 x 14336: 52 us, 5.7 TB/s), for a few rows by the launch (50 x 4096 4.8 us).
 __global__ __launch_bounds__(256) void k_mx4_quant(QuantArgs a) {
     const uint32_t it = blockIdx.x * 256u + threadIdx.x;
     if (it >= a.items) return;
@@ -106,9 +106,9 @@ __device__ __forceinline__ void some(E, F f) {
     if constexpr (E::value < P) each<N * (E::value + 1) / P, N * E::value / P>(f);
 }
 
-// What a lane has of a row's 16 blocks from b0: in step j block b0 + 4 j + g (the four lanes of a row read 64 bytes side by side; with four blocks side by
-// side for each lane a load touches 64 lines, and one row of 4096 x 14336 takes 14.5 us for 12.7), and the row's four words of scales. WHOLE: all
-// blocks are there; else zeros with a scale of 1 behind the last.
+// What a lane has of a row's 16 blocks from b0: in step j block b0 + 4 j + g (the four lanes of a row read 64 bytes side by side), and the
+// row's four words of scales. WHOLE: all blocks are there, no conditions (one fp16 row of 4096 x 14336 14.5 -> 12.7 us with both, 50 rows of 8192 x 4096 15.8 -> 13.7,
+// from blocks side by side for a lane, each under its condition); else zeros with a scale of 1 behind the last.
 constexpr int SU = 4;                      // steps of a unit
 struct Part { sh_u4v c[SU], s; };
 template <bool WHOLE>
@@ -243,8 +243,12 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
 // Many rows. A workgroup has a BM x BN tile of z, a wave TM x TN blocks of 32 x 32 of it (W's rows are the instruction's rows, so a lane has one row
 // of z and groups of four columns). Slices of 128 k (four blocks of a row: 64 bytes) go by DMA into a ring of four stages, three slices ahead; the scales of four
 // slices (16 bytes of a row) into a ring of three. A slice is two steps of 64 k; a step's operands are read while the last step multiplies, and the barrier that frees
-// a stage lies between the two, so that no wave meets it without products to issue. Chunk c of a row lies at c ^ (row / 2 % 4) of its 64 bytes: eight lanes'
-// reads then touch every bank once. Behind the last block the codes are those of the last one again and both scales 2^-127: their product is 0 in fp32.
+// a stage lies between the two, so that no wave meets it without products to issue. Chunk c of a row lies at c ^ ((row / 2 ^ row / 8 % 2) % 4) of its 64 bytes, so
+// that neither eight nor sixteen lanes in a row meet in a bank (row / 2 % 4 alone: twice the conflicts). Behind the last block the codes are those of the last one again and both scales 2^-127: their product is 0 in fp32.
+// Bound by what L2 gives the CUs (12 TB/s at most was seen here, in lines or halves of them alike: 256 columns a slice in two stages, or a line of 128 bytes a row in four,
+// were no faster) and, in large problems, by power: 8192^3, 298 us, 3.7 PFLOP/s at 1.78 GHz, matrix pipe busy 47 %; the pipe alone, fed from registers, gives 6.3 PFLOP/s
+// of random codes and 9.7 of zeros. Eight waves share a 256 x 256 tile (four, with twice the registers each: 302 us); of the 73 us that a round of tiles takes
+// there, 10 are its start and its end.
 __device__ __forceinline__ void dma4_s(const void *base, uint32_t off, uint32_t lds_wave_base) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -460,7 +464,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
     for (; t + NST < n; ++t) slice(std::true_type{});        // (up to three, whose loads need no further scales)
     for (; t < n; ++t) slice(std::false_type{});
     // The sums through LDS, in as many passes as they need room, to whole rows: a thread has the same eight columns of every row that it
-    // finishes. (Finished where they are, 256 values a thread, they took 18 us of a tile's 85 in code that is run once.)
+    // finishes, in a short loop. (Finished where they are, 256 values a thread, 8192 x 8192 x 512 took 84.8 us, this way 70.8; both with four waves.)
     constexpr int PASSES = T::PASSES, KP = TM / PASSES;
     constexpr uint32_t CH = BN / 8, RS = 64 * NW / CH, RP = 32 * KP;
     const uint32_t c8 = threadIdx.x % CH * 8, nn = n0 + c8, left = nn < a.N ? min(a.N - nn, 8u) : 0u;
@@ -548,8 +552,17 @@ bool launch_rows_as(const MxArgs &a, hipStream_t st) {
                        "sh_gemm_mx4 hipFuncSetAttribute")) return false;
         set = true;
     }
-    const uint32_t lds = NW * std::min(a.M, 16u * MT) * (16 * CW + 1) * 4;
-    hipLaunchKernelGGL((k_mx4_rows<MT, CW, NW, F16>), dim3(sh_cdiv(a.N, 16 * CW), sh_cdiv(a.M, 16 * MT)), dim3(64 * NW), lds, st, a);
+    const uint32_t lds = NW * std::min(a.M, 16u * MT) * (16 * CW + 1) * 4, most_rows = 65535 * 16 * MT;        // (workgroups in y)
+    const uint32_t M = a.M;
+    for (uint32_t m = 0; m < M; m += most_rows) {
+        MxArgs b = a;
+        b.M = std::min(M - m, most_rows);
+        if (m) {
+            b.xc += m * a.ldxc; b.xs += m * a.ldxs; b.z += m * a.ldz;
+            if (b.res) b.res += m * a.ldr;
+        }
+        hipLaunchKernelGGL((k_mx4_rows<MT, CW, NW, F16>), dim3(sh_cdiv(a.N, 16 * CW), sh_cdiv(b.M, 16 * MT)), dim3(64 * NW), lds, st, b);
+    }
     return true;
 }
 // Columns and waves of a workgroup, by N and K. Many columns: wider workgroups, which read x (and bring it into codes) less often: 4096 x 14336, one row 8.6 us with
