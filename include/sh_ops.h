@@ -310,7 +310,8 @@ int sh_attention_batched_prefetch(uint64_t q, uint64_t k, uint64_t v, uint64_t o
  * value = code x scale. A request's tokens 0, 1, ... lie in the pages its row of the block table names, bs to a page.
  * SH_INT8: two's complement, -127 .. 127. SH_FP8: OCP e4m3 (finite, largest 448). Values are stored with the tokens of a
  * page consecutive, as the product with the probabilities reads them.
- * A serving step: sh_kv_slots (where the new tokens go), the projections, sh_rope, sh_kv_append, sh_attention_kv. (sh_rope takes a
+ * A serving step: sh_kv_slots (where the new tokens go), the projections, sh_kv_append_rope (queries and keys turned by their positions), sh_attention_kv;
+ * or, with a table of the caller's own, sh_rope and sh_kv_append. (sh_rope takes a
  * cos / sin row for each row and no positions: the caller gathers its table's rows at `pos`, any row where that is -1.) The
  * calls need no device memory of the library's own and no host synchronisation, so a step captures into a HIP graph whose replays
  * read the lengths of that moment. */
@@ -430,7 +431,7 @@ int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero, uint64_t z
  * A row of K numbers as codes and scales, both operands of a product alike (a weight W [K, N] as the N rows of W^T): codes of e2m1 (sign,
  * 2 bits of exponent, 1 of fraction: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two to a byte, the lower k in the low four bits, 16 bytes for each
  * block of 32 k; a scale byte e for each block, 2^(e - 127), 255: NaN. Codes: 16-byte aligned, leading dim in bytes a multiple of 16, at least 16
- * ceil(K / 32). Scales: 4-byte aligned, leading dim in bytes a multiple of 4, at least ceil(K / 32). */
+ * ceil(K / 32) (multiples of 128 are read fastest). Scales: 4-byte aligned, leading dim in bytes a multiple of 4, at least ceil(K / 32) (of 16: fastest). */
 
 /* Rows x (fp16 [rows][cols], leading dim ldx) as codes and scales. The scale of a block is the smallest power of two s >= 2^-32 with |x| <= 6 s; codes
  * are nearest, ties to even; a block with a NaN or an infinity has scale 255 and codes of 0. Codes behind `cols` in the last block are 0; bytes
