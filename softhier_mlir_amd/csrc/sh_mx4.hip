@@ -106,42 +106,24 @@ __device__ __forceinline__ void some(E, F f) {
     if constexpr (E::value < P) each<N * (E::value + 1) / P, N * E::value / P>(f);
 }
 
-// What a lane has of a row's 16 blocks from b0: in step j block b0 + 4 j + g (the four lanes of a row read 64 bytes side by side), and the
-// row's four words of scales. WHOLE: all blocks are there, no conditions (one fp16 row of 4096 x 14336 14.5 -> 12.7 us with both, 50 rows of 8192 x 4096 15.8 -> 13.7,
-// from blocks side by side for a lane, each under its condition); else zeros with a scale of 1 behind the last.
-constexpr int SU = 4;                      // steps of a unit
-struct Part { sh_u4v c[SU], s; };
-template <bool WHOLE>
-__device__ __forceinline__ void load_part(const uint8_t *codes, const uint8_t *scales, uint32_t b0, uint32_t g, uint32_t nb, Part &o) {
-    if constexpr (WHOLE) {
-        typedef sh_u4v words __attribute__((aligned(4)));
-        o.s = *(const words *)(scales + b0);
-#pragma unroll
-        for (int j = 0; j < SU; ++j) o.c[j] = *(const sh_u4v *)(codes + 16ull * (b0 + 4 * j + g));
-    } else {
-#pragma unroll
-        for (int j = 0; j < SU; ++j) {
-            const uint32_t b = b0 + 4 * j;
-            o.s[j] = b < nb ? *(const uint32_t *)(scales + b) : ONES;
-            o.c[j] = b + g < nb ? *(const sh_u4v *)(codes + 16ull * (b + g)) : sh_u4v{0, 0, 0, 0};
-        }
-    }
+__device__ __forceinline__ sh_u4v lds16(uint32_t addr) { return *(const __attribute__((address_space(3))) sh_u4v *)(uintptr_t)addr; }
+__device__ __forceinline__ uint32_t lds4(uint32_t addr) { return *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)addr; }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// One global_load_lds_dword: each lane's word lands at lds_wave_base + 4 lane.
+__device__ __forceinline__ void dma4(const void *src, uint32_t lds_wave_base) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_wave_base), "v"(src) : "memory", "m0");
 }
-// The scales of the lane's own four blocks in a word.
-template <bool WHOLE>
-__device__ __forceinline__ uint32_t gather(const Part &o, uint32_t b0, uint32_t g, uint32_t nb) {
-    const uint32_t sel = 0x0C0C0400u + 0x0101u * g;
-    uint32_t s = __builtin_amdgcn_perm(__builtin_amdgcn_perm(o.s[3], o.s[2], sel), __builtin_amdgcn_perm(o.s[1], o.s[0], sel), 0x05040100u);
-    if constexpr (!WHOLE)
-#pragma unroll
-        for (int j = 0; j < SU; ++j)
-            if (b0 + 4 * j + g >= nb) s = (s & ~(255u << (8 * j))) | 127u << (8 * j);
-    return s;
+__device__ __forceinline__ void dma4_s(const void *base, uint32_t off, uint32_t lds_wave_base) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_wave_base), "v"(off), "s"(base) : "memory", "m0");
 }
-// The same of a row of halves: the scales' word, and the codes.
+#pragma clang diagnostic pop
+
+constexpr int SU = 4;                      // steps of a unit of 512 k
+// A row of halves as a lane's operands: block b0 + 4 j + g in step j, and the scales' word. WHOLE: all blocks of the unit are there.
 template <bool WHOLE>
-__device__ __forceinline__ uint32_t load_part_f16(const uint16_t *row, uint32_t b0, uint32_t g, uint32_t nb, uint32_t K, Part &o) {
-    uint32_t s = WHOLE ? 0u : ONES;
+__device__ __forceinline__ uint32_t load_halves(const uint16_t *row, uint32_t b0, uint32_t g, uint32_t nb, uint32_t K, sh_u4v (&c)[SU]) {
+    uint32_t s = 0;
     uint4 v[SU][4];
 #pragma unroll
     for (int j = 0; j < SU; ++j)
@@ -153,74 +135,118 @@ __device__ __forceinline__ uint32_t load_part_f16(const uint16_t *row, uint32_t 
 #pragma unroll
     for (int j = 0; j < SU; ++j) {
         if (!WHOLE && b0 + 4 * j + g >= nb) {
-            o.c[j] = sh_u4v{0, 0, 0, 0};
+            c[j] = sh_u4v{0, 0, 0, 0};
             continue;
         }
         const us2 t = __builtin_elementwise_max(__builtin_elementwise_max(top8(v[j][0]), top8(v[j][1])), __builtin_elementwise_max(top8(v[j][2]), top8(v[j][3])));
         const uint32_t e = scale_byte(max(t.x, t.y));
-        s = WHOLE ? s | e << (8 * j) : (s & ~(255u << (8 * j))) | e << (8 * j);
+        s |= e << (8 * j);
         const float f = __uint_as_float(e << 23);            // (255: infinity, whose codes are put right)
-        o.c[j] = sh_u4v{codes8(v[j][0], f), codes8(v[j][1], f), codes8(v[j][2], f), codes8(v[j][3], f)};
-        if (e == 255u) o.c[j] = sh_u4v{0, 0, 0, 0};
+        c[j] = sh_u4v{codes8(v[j][0], f), codes8(v[j][1], f), codes8(v[j][2], f), codes8(v[j][3], f)};
+        if (e == 255u) c[j] = sh_u4v{0, 0, 0, 0};
     }
     return s;
 }
 
-// Few rows: a workgroup has 16 CW columns and 16 MT rows of z; its waves take units of 512 k in turn, and their sums are added in LDS in wave order.
+// Few rows: a workgroup has 16 CW columns and 16 MT rows of z; its waves take units of 512 k in turn, and their sums are added in LDS in wave order. A wave
+// brings a unit's codes and scales into LDS of its own by DMA, without a barrier: four lanes side by side read 64 bytes of a row. (Read straight into the
+// operands' lanes, where neighbours are rows, each lane is an access of its own: 50 rows of 8192 x 4096 13.3 us, this way 11.5; 64 of 16384 x 4096 25.5 and 15.0; one
+// fp16 row of 4096 x 14336 9.1 and 8.7.) In step j a lane has block 4 j + g. Behind the last block the codes are those of the last one again and both scales 2^-127.
+template <int MT, int CW, int NW, bool F16>
+struct Rows {
+    static constexpr int GROUPS = CW + (F16 ? 0 : MT);                         // of 16 rows, of W and of x
+    static constexpr uint32_t CODES = SU * 1024, GROUP = CODES + SU * 64, WAVE = GROUPS * GROUP, LC = 16 * CW + 1;
+    static uint32_t lds(uint32_t nrow) { return std::max(NW * WAVE, NW * nrow * LC * 4); }
+    static_assert(NW * WAVE <= 163840, "rows");
+};
 template <int MT, int CW, int NW, bool F16>
 __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
-    constexpr uint32_t LC = 16 * CW + 1;
-    extern __shared__ float s_z[];                                             // [NW][rows][LC]
+    using T = Rows<MT, CW, NW, F16>;
+    constexpr uint32_t LC = T::LC;
+    extern __shared__ __align__(128) uint8_t smem[];
+    float *s_z = (float *)smem;                                                // [NW][rows][LC], after the products
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const uint32_t col0 = blockIdx.x * 16 * CW, m0 = blockIdx.y * 16 * MT, nrow = min(a.M - m0, 16u * MT);
-    const uint32_t units = (a.nb + 4 * SU - 1) / (4 * SU);
-    const uint8_t *wc[CW], *ws[CW], *xc[MT], *xs[MT];
-    const uint16_t *xh[MT];
+    const uint32_t nb = a.nb, nd = (nb + 3) / 4, units = (nb + 4 * SU - 1) / (4 * SU);
+    const uint32_t mine = sh_lds_addr(smem) + wave * T::WAVE;
+    // DMAs: lane -> row, 16-byte chunk of a segment of 64; lane -> row, word of the unit's scales
+    const uint32_t chunk = (lane & 3) ^ ((lane >> 3 ^ lane >> 5) & 3), word = lane & 3;
+    const uint8_t *pc[T::GROUPS], *ps[T::GROUPS];
 #pragma unroll
-    for (int k = 0; k < CW; ++k) {
-        const uint64_t r = min(col0 + 16 * k + n, a.N - 1);
-        wc[k] = a.wc + r * a.ldwc; ws[k] = a.ws + r * a.ldws;
+    for (int k = 0; k < T::GROUPS; ++k) {
+        const uint32_t r = lane >> 2;
+        if (k < CW) {
+            pc[k] = a.wc + min(col0 + 16 * k + r, a.N - 1) * a.ldwc;
+            ps[k] = a.ws + min(col0 + 16 * k + r, a.N - 1) * a.ldws;
+        } else {
+            pc[k] = a.xc + min(m0 + 16 * (k - CW) + r, a.M - 1) * a.ldxc;
+            ps[k] = a.xs + min(m0 + 16 * (k - CW) + r, a.M - 1) * a.ldxs;
+        }
     }
+    const auto load = [&](uint32_t u) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const uint64_t r = min(m0 + 16 * i + n, a.M - 1);
-        xc[i] = a.xc + r * a.ldxc; xs[i] = a.xs + r * a.ldxs; xh[i] = a.x + r * a.ldx;
-    }
+        for (int k = 0; k < T::GROUPS; ++k) {
+#pragma unroll
+            for (int j = 0; j < SU; ++j) sh_lds_dma16(pc[k] + 16ull * min(4 * (SU * u + j) + chunk, nb - 1), mine + k * T::GROUP + j * 1024);
+            dma4(ps[k] + 4ull * min(SU * u + word, nd - 1), mine + k * T::GROUP + T::CODES);
+        }
+    };
+    const uint32_t code_at = n * 64 + (g ^ ((n >> 1 ^ n >> 3) & 3)) * 16;
     sh_f4v acc[CW][MT];
 #pragma unroll
     for (int k = 0; k < CW; ++k)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[k][i] = sh_f4v{0.f, 0.f, 0.f, 0.f};
-    const auto unit = [&](uint32_t u, auto whole) {
-        constexpr bool WHOLE = decltype(whole)::value;
+    const auto codes = [&](int k, sh_u4v (&c)[SU]) {
+#pragma unroll
+        for (int j = 0; j < SU; ++j) c[j] = lds16(mine + k * T::GROUP + j * 1024 + code_at);
+    };
+    // a row's four words of scales to the lane's own blocks' bytes
+    const auto scales = [&](int k, uint32_t b0) {
+        const sh_u4v v = lds16(mine + k * T::GROUP + T::CODES + n * 16);
+        const uint32_t sel = 0x0C0C0400u + 0x0101u * g;
+        uint32_t s = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], sel), __builtin_amdgcn_perm(v[1], v[0], sel), 0x05040100u);
+        if (b0 + 4 * SU > nb)
+#pragma unroll
+            for (int j = 0; j < SU; ++j)
+                if (b0 + 4 * j + g >= nb) s &= ~(255u << (8 * j));
+        return (int)s;
+    };
+    for (uint32_t u = wave; u < units; u += NW) {
         const uint32_t b0 = 4 * SU * u;
-        Part w[CW], x[MT];
+        sh_u4v x[MT][SU];
         int sx[MT];
+        load(u);
+        if constexpr (F16)                                                     // (loads and work of their own, while the codes are on their way)
 #pragma unroll
-        for (int k = 0; k < CW; ++k) load_part<WHOLE>(wc[k], ws[k], b0, g, a.nb, w[k]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            if constexpr (F16) sx[i] = (int)load_part_f16<WHOLE>(xh[i], b0, g, a.nb, a.K, x[i]);
-            else load_part<WHOLE>(xc[i], xs[i], b0, g, a.nb, x[i]);
-        }
+            for (int i = 0; i < MT; ++i) {
+                const uint16_t *row = a.x + min(m0 + 16 * i + n, a.M - 1) * a.ldx;
+                sx[i] = (int)(128 * SU * (u + 1) <= a.K ? load_halves<true>(row, b0, g, nb, a.K, x[i]) : load_halves<false>(row, b0, g, nb, a.K, x[i]));
+            }
+        sh_wait_vmcnt<0>();
+        asm volatile("" ::: "memory");
         if constexpr (!F16)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) sx[i] = (int)gather<WHOLE>(x[i], b0, g, a.nb);
+            for (int i = 0; i < MT; ++i) {
+                codes(CW + i, x[i]);
+                sx[i] = scales(CW + i, b0);
+            }
 #pragma unroll
         for (int k = 0; k < CW; ++k) {
-            const int sw = (int)gather<WHOLE>(w[k], b0, g, a.nb);
+            sh_u4v w[SU];
+            codes(k, w);
+            const int sw = scales(k, b0);
 #pragma unroll
             for (int i = 0; i < MT; ++i)
                 each<SU>([&](auto j) {
                     constexpr int J = decltype(j)::value;
-                    acc[k][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w[k].c[J]), operand(x[i].c[J]), acc[k][i], E2M1, E2M1, J, sw, J, sx[i]);
+                    acc[k][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w[J]), operand(x[i][J]), acc[k][i], E2M1, E2M1, J, sw, J, sx[i]);
                 });
         }
-    };
-    const uint32_t full = F16 ? a.K / (128 * SU) : a.nb / (4 * SU);            // units with all of their blocks (halves)
-    uint32_t u = wave;
-    for (; u < full; u += NW) unit(u, std::true_type{});
-    if (u < units) unit(u, std::false_type{});
+        sh_wait_lgkm0();                                                       // (the next unit's codes come into the same place)
+        asm volatile("" ::: "memory");
+    }
+    __syncthreads();
     // lane (m, g): the columns 4 g .. 4 g + 3 of row m
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -249,15 +275,6 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
 // were no faster) and, in large problems, by power: 8192^3, 298 us, 3.7 PFLOP/s at 1.78 GHz, matrix pipe busy 47 %; the pipe alone, fed from registers, gives 6.3 PFLOP/s
 // of random codes and 9.7 of zeros. Eight waves share a 256 x 256 tile (four, with twice the registers each: 302 us); of the 73 us that a round of tiles takes
 // there, 10 are its start and its end.
-__device__ __forceinline__ void dma4_s(const void *base, uint32_t off, uint32_t lds_wave_base) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_wave_base), "v"(off), "s"(base) : "memory", "m0");
-#pragma clang diagnostic pop
-}
-__device__ __forceinline__ sh_u4v lds16(uint32_t addr) { return *(const __attribute__((address_space(3))) sh_u4v *)(uintptr_t)addr; }
-__device__ __forceinline__ uint32_t lds4(uint32_t addr) { return *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)addr; }
-
 template <int BM, int BN, int WGM, int WGN>
 struct Tile {
     static constexpr int NW = WGM * WGN, TM = BM / WGM / 32, TN = BN / WGN / 32, NST = 4, ROWS = BM + BN;
@@ -545,14 +562,14 @@ bool launch_tile(const MxArgs &a, hipStream_t st) {
 
 template <int MT, int CW, int NW, bool F16>
 bool launch_rows_as(const MxArgs &a, hipStream_t st) {
-    constexpr uint32_t most = NW * 16 * MT * (16 * CW + 1) * 4;
+    using T = Rows<MT, CW, NW, F16>;
     static bool set = false;
-    if (!set && most > 65536) {
-        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_mx4_rows<MT, CW, NW, F16>, hipFuncAttributeMaxDynamicSharedMemorySize, most),
+    const uint32_t lds = T::lds(std::min(a.M, 16u * MT)), most_rows = 65535 * 16 * MT;                         // (workgroups in y)
+    if (!set && T::lds(16 * MT) > 65536) {
+        if (!sh_hip_ok(hipFuncSetAttribute((const void *)k_mx4_rows<MT, CW, NW, F16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::lds(16 * MT)),
                        "sh_gemm_mx4 hipFuncSetAttribute")) return false;
         set = true;
     }
-    const uint32_t lds = NW * std::min(a.M, 16u * MT) * (16 * CW + 1) * 4, most_rows = 65535 * 16 * MT;        // (workgroups in y)
     const uint32_t M = a.M;
     for (uint32_t m = 0; m < M; m += most_rows) {
         MxArgs b = a;
@@ -565,19 +582,16 @@ bool launch_rows_as(const MxArgs &a, hipStream_t st) {
     }
     return true;
 }
-// Columns and waves of a workgroup, by N and K. Many columns: wider workgroups, which read x (and bring it into codes) less often: 4096 x 14336, one row 8.6 us with
-// 16 columns, 7.9 with 32, 8.4 with 64; of halves 12.8 / 9.8 / 9.3, 16 rows of halves 22.1 / 14.9 / 12.2; 30 rows of 4096 x 8192 9.2 / 7.5. Fewer columns need every
-// workgroup: 4096 x 4096 5.1 / 6.0 / 8.6. A long chain over them is shared by sixteen waves: halves, 14336 x 4096 15.1 us with eight, 12.6 with sixteen,
-// 16384 x 1024 11.5 / 10.5; at K = 8192 and below they are level.
+// Columns and waves of a workgroup, by N alone. Many columns: wider workgroups, which read x (and bring it into codes) less often: 4096 x 14336, one fp16 row 11.6 us with 16
+// columns, 9.2 with 32, 8.7 with 64, 16 rows 20.0 / 13.1 / 11.3; 30 rows of codes, 4096 x 6144 7.3 / 5.9, 4096 x 8192 8.1 / 6.6. Fewer columns need every workgroup
+// (4096 x 4096, one fp16 row 4.8 / 5.3 / 6.5; 30 rows, 2048 x 2048 level), and one row of codes is level (7.8 / 8.2). 64 rows: what LDS holds, seven waves.
 template <int MT, bool F16>
 bool launch_rows(const MxArgs &a, hipStream_t st) {
     if constexpr (F16)
         if (a.N > 8192) return launch_rows_as<MT, 4, 8, F16>(a, st);
-    if constexpr (!F16 && MT < 4)
-        if (a.N >= 8192) return launch_rows_as<MT, 2, 8, F16>(a, st);
-    if constexpr (MT == 1)
-        if (a.K > 8192) return launch_rows_as<MT, 1, 16, F16>(a, st);
-    return launch_rows_as<MT, 1, 8, F16>(a, st);
+    if constexpr (MT == 2)
+        if (a.N > 4096) return launch_rows_as<MT, 2, 8, F16>(a, st);
+    return launch_rows_as<MT, 1, MT == 4 ? 7 : 8, F16>(a, st);
 }
 
 // The checks that both products make of the weight, the result and the epilogue.
@@ -659,8 +673,8 @@ int sh_gemm_mx4(uint64_t xc, uint64_t xs, uint64_t wc, uint64_t ws, uint64_t z, 
     }
     const bool near = ldxc <= (1u << 24) && ldwc <= (1u << 24) && ldxs <= (1u << 24) && ldws <= (1u << 24);       // a tile's rows within 32-bit offsets
     bool ok = true;
-    // Up to 64 rows the chain is shared by a workgroup's waves; more than 32 of many columns fill the GPU as tiles (64 rows of 4096 x 14336: 10.9 us, 29.6 so; 50
-    // of 8192 x 4096 15.5 against 13.9).
+    // Up to 64 rows the chain is shared by a workgroup's waves; more than 32 of many columns fill the GPU as tiles (64 rows of 4096 x 6144: 9.4 us, 10.7 so; 48 of
+    // 2880 x 5000 7.1 and 8.6; but 64 of 4096 x 4096 9.1 and 5.9, of 8192 x 2048 13.8 and 7.9).
     if (M <= 16) ok = launch_rows<1, false>(a, st);
     else if (M <= 32) ok = launch_rows<2, false>(a, st);
     else if ((M <= 64 && N <= 4096) || !near) ok = launch_rows<4, false>(a, st);
