@@ -138,7 +138,8 @@ def _check(got, x, w, bias=None, gelu=False, residual=None):
 
 SHAPES = [(1, 1, 1), (1, 16, 32), (1, 17, 33), (1, 64, 128), (1, 2048, 720), (1, 100, 4096), (2, 33, 200), (5, 68, 1032), (16, 256, 512), (17, 132, 968), (31, 960, 960),
           (33, 40, 136), (50, 720, 2048), (64, 260, 1608), (65, 48, 320), (200, 72, 264), (3, 5000, 64), (64, 64, 16384), (128, 128, 256), (129, 127, 255), (256, 256, 512),
-          (257, 300, 700), (300, 1000, 1000), (511, 513, 96), (700, 640, 2880), (1000, 260, 4100), (70, 2100, 31), (2048, 512, 512), (4100, 4200, 200), (4097, 4096, 33), (2500, 8200, 1200)]
+          (257, 300, 700), (300, 1000, 1000), (511, 513, 96), (700, 640, 2880), (1000, 260, 4100), (70, 2100, 31), (2048, 512, 512), (4100, 4200, 200), (4097, 4096, 33), (2500, 8200, 1200),
+          (20, 5000, 600), (32, 8300, 1100), (40, 5000, 300), (64, 4096, 4128), (1000, 2048, 300), (2048, 4096, 288), (700, 5000, 1000), (9, 9000, 520)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -209,7 +210,7 @@ def test_nan_scales(lib, gpu, M, N):
     assert np.array_equal(np.isnan(z), bad)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 64, 1), (1, 2048, 720), (1, 200, 4096), (2, 33, 5), (7, 100, 1000), (16, 300, 2080), (5, 40, 31), (16, 50, 9000), (3, 1024, 260)])
+@pytest.mark.parametrize("M,N,K", [(1, 64, 1), (1, 2048, 720), (1, 200, 4096), (2, 33, 5), (7, 100, 1000), (16, 300, 2080), (5, 40, 31), (16, 50, 9000), (3, 1024, 260), (1, 8300, 700), (13, 8193, 1100)])
 @pytest.mark.parametrize("pad,off", [(0, 0), (1, 1), (8, 3)])
 def test_f16_rows(lib, gpu, M, N, K, pad, off):
     """The bits of sh_mx4_quant and sh_gemm_mx4, and the product within its bound."""
@@ -303,3 +304,42 @@ def test_calls_give_the_same_bits_again(lib, gpu):
         first = _run(lib, x, w, M, N, K)
         for _ in range(3):
             assert np.array_equal(_run(lib, x, w, M, N, K), first)
+
+
+@pytest.mark.parametrize("M,N", [(70, 90), (40, 200), (300, 40)])
+def test_rows_far_apart(lib, gpu, M, N):
+    """Leading dims so large that offsets pass 32 bits, of x, of W and of z."""
+    import torch
+    rng = np.random.default_rng(M)
+    K, far = 700, (1 << 32) // 30 // 128 * 128
+    x, w = _operand(rng, M, K), _operand(rng, N, K, -9, -5)
+    nb = x[1].shape[1]
+    want = _run(lib, x, w, M, N, K)
+    ops, lds = [], []
+    for (c, s), n, big in ((x, M, M > 60), (w, N, N > 60)):
+        ldc = far if big else 16 * nb
+        buf = torch.zeros((n, ldc), dtype=torch.uint8, device="cuda")
+        buf[:, : 16 * nb] = dev(R.pack(c))
+        ops += [buf, _put(c, s)[1]]
+        lds += [ldc, ops[-1].shape[1]]
+    z = torch.zeros((M, far // 2), dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    assert lib.sh_gemm_mx4(*(A(t) for t in ops), A(z), M, N, K, *lds, far // 2, None) == 0, shops.last_error()
+    got = to_np(z[:, :N]).astype(np.float64)
+    if M <= 64:                                              # (the same kernel: for more rows it is the one whose offsets hold)
+        assert np.array_equal(got, want)
+    _check(got, x, w)
+
+
+def test_quant_rows_far_apart(lib, gpu):
+    import torch
+    rng = np.random.default_rng(6)
+    rows, cols, far = 40, 300, (1 << 32) // 36 // 16 * 16
+    x = rng.standard_normal((rows, cols)).astype(np.float16)
+    X = torch.zeros((rows, far), dtype=torch.float16, device="cuda")
+    X[:, :cols] = to_dev(x)
+    c, s = torch.zeros((rows, far), dtype=torch.uint8, device="cuda"), torch.zeros((rows, 12), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    assert lib.sh_mx4_quant(A(c), A(s), A(X), rows, cols, far, 12, far) == 0, shops.last_error()
+    wc, ws = R.quant(x)
+    assert np.array_equal(to_np(s[:, :10]), ws) and np.array_equal(R.unpack(to_np(c[:, :160].contiguous())), wc)

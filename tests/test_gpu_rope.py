@@ -143,6 +143,21 @@ def test_steps(lib, gpu, rot, base, scaling, factor, lo, hi, ctx):
     assert (np.abs(got[:-1].view(np.uint64).astype(np.float64) * 2.0 ** -64 - w) <= 2.0 ** -45 * w + 2.0 ** -65).all()
 
 
+def test_rows_far_apart(lib, gpu):
+    """A leading dim with which offsets pass 32 bits, in the builds for few and for many columns."""
+    import torch
+    rng = np.random.default_rng(8)
+    far = (1 << 32) // 50
+    for heads, dh, rot in ((3, 64, 64), (2, 20, 14)):
+        x = rng.standard_normal((60, heads * dh)).astype(np.float16)
+        step, pos = R.steps(R.frequencies(rot, 1e4)), np.arange(60, dtype=np.int32) * 1000
+        X, Y = (torch.zeros((60, far), dtype=torch.float16, device="cuda") for _ in "xy")
+        X[:, : heads * dh] = to_dev(x)
+        torch.cuda.synchronize()
+        assert lib.sh_rope_pos(A(Y), A(X), A(dev(pos)), _plan(step, R.PAIRS), 60, heads, dh, far, far) == 0, shops.last_error()
+        _check(to_np(Y[:, : heads * dh].contiguous()), x, step, pos, heads, dh, R.PAIRS)
+
+
 # ---- sh_kv_append_rope ----------------------------------------------------------------------------------------------
 class Cache:
     def __init__(self, rng, pages, hkv, dh, bs, fmt, pad=0):
@@ -305,3 +320,25 @@ def test_append_in_a_graph(lib, gpu):
         assert np.array_equal(codes(q[0]), codes(q[1]))
         for a, b in zip(one.bits(), two.bits()):
             assert np.array_equal(a, b), i
+
+
+def test_append_into_a_cache_of_gigabytes(lib, gpu):
+    """Pages whose bytes lie past 32 bits: the bits that the same rows have in the first pages."""
+    import torch
+    rng = np.random.default_rng(31)
+    H, hkv, dh, bs, pages = 2, 8, 128, 64, 70000
+    nq, nk, wide = H * dh, hkv * dh, (H + 2 * hkv) * dh
+    step = R.steps(R.frequencies(128, 1e4))
+    plan = _plan(step, R.HALF)
+    X, P = to_dev(rng.standard_normal((70, wide)).astype(np.float16)), dev(np.arange(5, 75, dtype=np.int32))
+    k, v = (torch.zeros((pages, hkv * bs * dh), dtype=torch.uint8, device="cuda") for _ in "kv")
+    ks, vs = (torch.zeros((pages, hkv), device="cuda") for _ in "kv")
+    q = torch.zeros((70, nq), dtype=torch.float16, device="cuda")
+    c = shops.kv_cache(A(k), A(v), A(ks), A(vs), pages, hkv, dh, bs, shops.SH_INT8)
+    torch.cuda.synchronize()
+    for first in (0, pages - 2):
+        S = dev((first * bs + np.arange(70)).astype(np.int32))
+        assert lib.sh_kv_append_rope(C.byref(c), plan, A(q), A(X), A(X, nq), A(X, nq + nk), A(P), A(S), 70, H, nq, wide, wide, wide) == 0, shops.last_error()
+    for t in (k, v, ks, vs):
+        assert torch.equal(t[:2], t[pages - 2:]) and bool((t[:2] != 0).any())
+        assert not bool((t[2: pages - 2: 997] != 0).any())
