@@ -111,16 +111,13 @@ __device__ __forceinline__ uint32_t lds4(uint32_t addr) { return *(const __attri
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // One global_load_lds_dword: each lane's word lands at lds_wave_base + 4 lane.
-__device__ __forceinline__ void dma4(const void *src, uint32_t lds_wave_base) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_wave_base), "v"(src) : "memory", "m0");
-}
 __device__ __forceinline__ void dma4_s(const void *base, uint32_t off, uint32_t lds_wave_base) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_wave_base), "v"(off), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
-constexpr int SU = 4;                      // steps of a unit of 512 k
-// A row of halves as a lane's operands: block b0 + 4 j + g in step j, and the scales' word. WHOLE: all blocks of the unit are there.
+constexpr int SU = 4;                      // steps of a unit of 512 k: four segments of 64 bytes of a row, four words of scales
+// A row of halves as a lane's operands: block b0 + 4 g + j in step j, and the scales' word. WHOLE: all blocks of the unit are there.
 template <bool WHOLE>
 __device__ __forceinline__ uint32_t load_halves(const uint16_t *row, uint32_t b0, uint32_t g, uint32_t nb, uint32_t K, sh_u4v (&c)[SU]) {
     uint32_t s = 0;
@@ -129,12 +126,12 @@ __device__ __forceinline__ uint32_t load_halves(const uint16_t *row, uint32_t b0
     for (int j = 0; j < SU; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t k = 32 * (b0 + 4 * j + g) + 8 * i;
+            const uint32_t k = 32 * (b0 + 4 * g + j) + 8 * i;
             v[j][i] = WHOLE ? sh_ld16_any(row + k) : load8(row, k, K);
         }
 #pragma unroll
     for (int j = 0; j < SU; ++j) {
-        if (!WHOLE && b0 + 4 * j + g >= nb) {
+        if (!WHOLE && b0 + 4 * g + j >= nb) {
             c[j] = sh_u4v{0, 0, 0, 0};
             continue;
         }
@@ -149,13 +146,15 @@ __device__ __forceinline__ uint32_t load_halves(const uint16_t *row, uint32_t b0
 }
 
 // Few rows: a workgroup has 16 CW columns and 16 MT rows of z; its waves take units of 512 k in turn, and their sums are added in LDS in wave order. A wave
-// brings a unit's codes and scales into LDS of its own by DMA, without a barrier: four lanes side by side read 64 bytes of a row. (Read straight into the
-// operands' lanes, where neighbours are rows, each lane is an access of its own: 50 rows of 8192 x 4096 13.3 us, this way 11.5; 64 of 16384 x 4096 25.5 and 15.0; one
-// fp16 row of 4096 x 14336 9.1 and 8.7.) In step j a lane has block 4 j + g. Behind the last block the codes are those of the last one again and both scales 2^-127.
+// brings a unit's codes into LDS of its own by DMA, without a barrier: four lanes side by side read 64 bytes of a row, or its four words of scales, which
+// change lanes afterwards. (Read straight into the operands' lanes, where neighbours are rows, each lane is an access of its own: 50 rows of 8192 x 4096 13.3 us, with
+// DMAs 11.3; 64 of 16384 x 4096 25.5 and 15.2. The scales alone read so: one row of 720 x 2048 5.1 us, 4.7 this way.) A workgroup begins at a unit of its own: where all begin
+// with the same lines of x, they wait for each other's (50 rows 12.0 us, 9.2 so; 16 rows of 8192 x 4096 6.9 and 5.3). Seven waves would leave LDS for the scales too, and take
+// a round more. In step j a lane has block 4 g + j. Behind the last block the codes are those of the last one again and both scales 2^-127.
 template <int MT, int CW, int NW, bool F16>
 struct Rows {
     static constexpr int GROUPS = CW + (F16 ? 0 : MT);                         // of 16 rows, of W and of x
-    static constexpr uint32_t CODES = SU * 1024, GROUP = CODES + SU * 64, WAVE = GROUPS * GROUP, LC = 16 * CW + 1;
+    static constexpr uint32_t GROUP = SU * 1024, WAVE = GROUPS * GROUP, LC = 16 * CW + 1;
     static uint32_t lds(uint32_t nrow) { return std::max(NW * WAVE, NW * nrow * LC * 4); }
     static_assert(NW * WAVE <= 163840, "rows");
 };
@@ -169,8 +168,8 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
     const uint32_t col0 = blockIdx.x * 16 * CW, m0 = blockIdx.y * 16 * MT, nrow = min(a.M - m0, 16u * MT);
     const uint32_t nb = a.nb, nd = (nb + 3) / 4, units = (nb + 4 * SU - 1) / (4 * SU);
     const uint32_t mine = sh_lds_addr(smem) + wave * T::WAVE;
-    // DMAs: lane -> row, 16-byte chunk of a segment of 64; lane -> row, word of the unit's scales
-    const uint32_t chunk = (lane & 3) ^ ((lane >> 3 ^ lane >> 5) & 3), word = lane & 3;
+    // DMAs: lane -> row, 16-byte chunk of a segment of 64; scales: lane -> row, word of the unit
+    const uint32_t chunk = (lane & 3) ^ ((lane >> 3 ^ lane >> 5) & 3);
     const uint8_t *pc[T::GROUPS], *ps[T::GROUPS];
 #pragma unroll
     for (int k = 0; k < T::GROUPS; ++k) {
@@ -183,15 +182,19 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
             ps[k] = a.xs + min(m0 + 16 * (k - CW) + r, a.M - 1) * a.ldxs;
         }
     }
+    uint32_t sc[T::GROUPS];
     const auto load = [&](uint32_t u) {
+        const uint32_t b = 4 * (SU * u + g), left = b < nb ? nb - b : 0u, keep = left < 4 ? (1u << (8 * left)) - 1 : ~0u;
 #pragma unroll
-        for (int k = 0; k < T::GROUPS; ++k) {
+        for (int k = 0; k < T::GROUPS; ++k) sc[k] = *(const uint32_t *)(ps[k] + 4ull * min(SU * u + (lane & 3), nd - 1));
+#pragma unroll
+        for (int k = 0; k < T::GROUPS; ++k)
 #pragma unroll
             for (int j = 0; j < SU; ++j) sh_lds_dma16(pc[k] + 16ull * min(4 * (SU * u + j) + chunk, nb - 1), mine + k * T::GROUP + j * 1024);
-            dma4(ps[k] + 4ull * min(SU * u + word, nd - 1), mine + k * T::GROUP + T::CODES);
-        }
+        return keep;
     };
-    const uint32_t code_at = n * 64 + (g ^ ((n >> 1 ^ n >> 3) & 3)) * 16;
+    const auto scale = [&](int k, uint32_t keep) { return (int)(__builtin_amdgcn_ds_bpermute((int)(4 * n + g) * 4, (int)sc[k]) & keep); };
+    const uint32_t code_at = g * 1024 + n * 64, swap = (n >> 1 ^ n >> 3) & 3;
     sh_f4v acc[CW][MT];
 #pragma unroll
     for (int k = 0; k < CW; ++k)
@@ -199,24 +202,14 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
         for (int i = 0; i < MT; ++i) acc[k][i] = sh_f4v{0.f, 0.f, 0.f, 0.f};
     const auto codes = [&](int k, sh_u4v (&c)[SU]) {
 #pragma unroll
-        for (int j = 0; j < SU; ++j) c[j] = lds16(mine + k * T::GROUP + j * 1024 + code_at);
+        for (int j = 0; j < SU; ++j) c[j] = lds16(mine + k * T::GROUP + code_at + 16 * (j ^ swap));
     };
-    // a row's four words of scales to the lane's own blocks' bytes
-    const auto scales = [&](int k, uint32_t b0) {
-        const sh_u4v v = lds16(mine + k * T::GROUP + T::CODES + n * 16);
-        const uint32_t sel = 0x0C0C0400u + 0x0101u * g;
-        uint32_t s = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], sel), __builtin_amdgcn_perm(v[1], v[0], sel), 0x05040100u);
-        if (b0 + 4 * SU > nb)
-#pragma unroll
-            for (int j = 0; j < SU; ++j)
-                if (b0 + 4 * j + g >= nb) s &= ~(255u << (8 * j));
-        return (int)s;
-    };
-    for (uint32_t u = wave; u < units; u += NW) {
-        const uint32_t b0 = 4 * SU * u;
+    const uint32_t first = col0 / 64 % units;                                  // (by the column alone, whatever CW: a column's sums keep their order)
+    for (uint32_t i = wave; i < units; i += NW) {
+        const uint32_t u = i + first < units ? i + first : i + first - units, b0 = 4 * SU * u;
         sh_u4v x[MT][SU];
         int sx[MT];
-        load(u);
+        const uint32_t keep = load(u);
         if constexpr (F16)                                                     // (loads and work of their own, while the codes are on their way)
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -229,13 +222,13 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 codes(CW + i, x[i]);
-                sx[i] = scales(CW + i, b0);
+                sx[i] = scale(CW + i, keep);
             }
 #pragma unroll
         for (int k = 0; k < CW; ++k) {
             sh_u4v w[SU];
             codes(k, w);
-            const int sw = scales(k, b0);
+            const int sw = scale(k, keep);
 #pragma unroll
             for (int i = 0; i < MT; ++i)
                 each<SU>([&](auto j) {
@@ -582,16 +575,17 @@ bool launch_rows_as(const MxArgs &a, hipStream_t st) {
     }
     return true;
 }
-// Columns and waves of a workgroup, by N alone. Many columns: wider workgroups, which read x (and bring it into codes) less often: 4096 x 14336, one fp16 row 11.6 us with 16
-// columns, 9.2 with 32, 8.7 with 64, 16 rows 20.0 / 13.1 / 11.3; 30 rows of codes, 4096 x 6144 7.3 / 5.9, 4096 x 8192 8.1 / 6.6. Fewer columns need every workgroup
-// (4096 x 4096, one fp16 row 4.8 / 5.3 / 6.5; 30 rows, 2048 x 2048 level), and one row of codes is level (7.8 / 8.2). 64 rows: what LDS holds, seven waves.
+// Columns of a workgroup, by N alone. Wider ones read x (and bring it into codes) less often, but there have to be enough for 256 CUs. us with 16 / 32 / 64
+// columns, K = 4096, fp16 rows: 1 x 4096 5.3 / 5.8 / 6.5, 1 x 5000 6.4 / 5.9 / 6.6, 1 x 10240 9.4 / 8.5 / 7.7, 1 x 28000 18.4 / 14.6 / 15.1, 16 x 4096 7.4 / 8.0 / 9.2,
+// 16 x 5000 11.7 / 8.3 / 9.4, 16 x 10240 17.2 / 14.0 / 10.6; K = 2048, 16 x 20000 15.3 / 11.8 / 13.0. Rows of codes: 20 x 14336 12.4 / 10.5, 32 x 5000 6.9 / 5.6,
+// 32 x 2048 level; up to 16 of them 16 columns (16 x 28000 12.9 / 15.7 / 14.9, 1 x 14336 7.9 / 8.3 / 7.8).
 template <int MT, bool F16>
 bool launch_rows(const MxArgs &a, hipStream_t st) {
     if constexpr (F16)
-        if (a.N > 8192) return launch_rows_as<MT, 4, 8, F16>(a, st);
-    if constexpr (MT == 2)
+        if (a.N > 8192 && a.N <= 16384) return launch_rows_as<MT, 4, 8, F16>(a, st);
+    if constexpr (MT == 2 || F16)
         if (a.N > 4096) return launch_rows_as<MT, 2, 8, F16>(a, st);
-    return launch_rows_as<MT, 1, MT == 4 ? 7 : 8, F16>(a, st);
+    return launch_rows_as<MT, 1, 8, F16>(a, st);
 }
 
 // The checks that both products make of the weight, the result and the epilogue.
