@@ -122,15 +122,29 @@ template <bool WHOLE>
 __device__ __forceinline__ uint32_t load_halves(const uint16_t *row, uint32_t b0, uint32_t g, uint32_t nb, uint32_t K, sh_u4v (&c)[SU]) {
     uint32_t s = 0;
     uint4 v[SU][4];
+    const uint32_t k0 = 32 * (b0 + 4 * g), end = K - min(K, 8u);
+    if (WHOLE || K >= 8)                                     // (no branch between the loads, what lies behind the row is put right below)
 #pragma unroll
-    for (int j = 0; j < SU; ++j)
+        for (int j = 0; j < SU; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t k = 32 * (b0 + 4 * g + j) + 8 * i;
-            v[j][i] = WHOLE ? sh_ld16_any(row + k) : load8(row, k, K);
-        }
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t k = k0 + 32 * j + 8 * i;
+                v[j][i] = sh_ld16_any(row + (WHOLE ? k : min(k, end)));
+            }
+    else
+#pragma unroll
+        for (int j = 0; j < SU; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j][i] = load8(row, k0 + 32 * j + 8 * i, K);
 #pragma unroll
     for (int j = 0; j < SU; ++j) {
+        if (!WHOLE && K >= 8 && k0 + 32 * j + 32 > K)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t k = k0 + 32 * j + 8 * i;
+                if (k >= K) v[j][i] = make_uint4(0, 0, 0, 0);
+                else if (k > end) v[j][i] = sh_fix8(v[j][i], k - end, 8 - (k - end));
+            }
         if (!WHOLE && b0 + 4 * g + j >= nb) {
             c[j] = sh_u4v{0, 0, 0, 0};
             continue;
@@ -148,7 +162,7 @@ __device__ __forceinline__ uint32_t load_halves(const uint16_t *row, uint32_t b0
 // Few rows: a workgroup has 16 CW columns and 16 MT rows of z; its waves take units of 512 k in turn, and their sums are added in LDS in wave order. A wave
 // brings a unit's codes into LDS of its own by DMA, without a barrier: four lanes side by side read 64 bytes of a row, or its four words of scales, which
 // change lanes afterwards. (Read straight into the operands' lanes, where neighbours are rows, each lane is an access of its own: 50 rows of 8192 x 4096 13.3 us, with
-// DMAs 11.3; 64 of 16384 x 4096 25.5 and 15.2. The scales alone read so: one row of 720 x 2048 5.1 us, 4.7 this way.) A workgroup begins at a unit of its own: where all begin
+// DMAs 11.3; 64 of 16384 x 4096 25.5 and 15.2. With the scales alone read so, 20 of 16384 x 1024 9.2 us, 7.8 this way.) A workgroup begins at a unit of its own: where all begin
 // with the same lines of x, they wait for each other's (50 rows 12.0 us, 9.2 so; 16 rows of 8192 x 4096 6.9 and 5.3). Seven waves would leave LDS for the scales too, and take
 // a round more. In step j a lane has block 4 g + j. Behind the last block the codes are those of the last one again and both scales 2^-127.
 template <int MT, int CW, int NW, bool F16>
