@@ -431,7 +431,8 @@ int sh_gemm_w4(uint64_t x, uint64_t w, uint64_t scale, uint64_t zero, uint64_t z
  * A row of K numbers as codes and scales, both operands of a product alike (a weight W [K, N] as the N rows of W^T): codes of e2m1 (sign,
  * 2 bits of exponent, 1 of fraction: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two to a byte, the lower k in the low four bits, 16 bytes for each
  * block of 32 k; a scale byte e for each block, 2^(e - 127), 255: NaN. Codes: 16-byte aligned, leading dim in bytes a multiple of 16, at least 16
- * ceil(K / 32) (multiples of 128 are read fastest). Scales: 4-byte aligned, leading dim in bytes a multiple of 4, at least ceil(K / 32) (of 16: fastest). */
+ * ceil(K / 32) (multiples of 64 are read fastest). Scales: 4-byte aligned, leading dim in bytes a multiple of 4, at least ceil(K / 32) (of 16: fastest).
+ * All rows have their leading dim in memory, the last one too. */
 
 /* Rows x (fp16 [rows][cols], leading dim ldx) as codes and scales. The scale of a block is the smallest power of two s >= 2^-32 with |x| <= 6 s; codes
  * are nearest, ties to even; a block with a NaN or an infinity has scale 255 and codes of 0. Codes behind `cols` in the last block are 0; bytes
