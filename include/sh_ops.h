@@ -442,7 +442,8 @@ int sh_mx4_quant(uint64_t codes, uint64_t scales, uint64_t x, uint32_t rows, uin
 /* z = act(x . W + bias) rounded to fp16, then [+ residual, rounded again], of rows in 4 bits: xc, xs [M], wc, ws [N] (the rows of W^T). fp32
  * sums of exact products. Codes behind K in the last block count where both operands' are not 0 (sh_mx4_quant's are 0); scale bytes behind the last block are
  * not used. A row of x or W with a scale of 255 gives NaN. epi: bias, act, residual as sh_gemm_ex (splits 0 or 1, no LayerNorm
- * fold, no row partials). M, N <= 2^26. 0, -1 for bad arguments, SH_EHIP. Deterministic; which kernel runs depends on M, so a row's low bits may. */
+ * fold, no row partials). M, N <= 2^26. 0, -1 for bad arguments, SH_EHIP. Deterministic; which kernel runs depends on M, N and
+ * the leading dims, so a row's low bits may. */
 int sh_gemm_mx4(uint64_t xc, uint64_t xs, uint64_t wc, uint64_t ws, uint64_t z, uint32_t M, uint32_t N, uint32_t K,
                 uint32_t ldxc, uint32_t ldxs, uint32_t ldwc, uint32_t ldws, uint32_t ldz, const sh_gemm_epi *epi);
 

@@ -493,12 +493,12 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
     constexpr uint32_t CH = BN / 8, RS = 64 * NW / CH, RP = 32 * KP;
     const uint32_t c8 = threadIdx.x % CH * 8, nn = n0 + c8, left = nn < a.N ? min(a.N - nn, 8u) : 0u;
     float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (a.bias)
-        for (uint32_t e = 0; e < left; ++e) {
-            const float b = a.bias_fp32 ? ((const float *)a.bias)[nn + e] : sh_dev_h2f(((const uint16_t *)a.bias)[nn + e]);
+    if (a.bias && a.bias_fp32)                                       // (loads at once; columns behind the last one are not stored)
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) bias[i] = i == e ? b : bias[i];
-        }
+        for (uint32_t e = 0; e < 8; ++e) bias[e] = ((const float *)a.bias)[min(nn + e, a.N - 1)];
+    else if (a.bias)
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) bias[e] = sh_dev_h2f(((const uint16_t *)a.bias)[min(nn + e, a.N - 1)]);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
         __syncthreads();

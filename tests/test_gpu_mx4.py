@@ -210,7 +210,7 @@ def test_nan_scales(lib, gpu, M, N):
     assert np.array_equal(np.isnan(z), bad)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 64, 1), (1, 2048, 720), (1, 200, 4096), (2, 33, 5), (7, 100, 1000), (16, 300, 2080), (5, 40, 31), (16, 50, 9000), (3, 1024, 260), (1, 8300, 700), (13, 8193, 1100)])
+@pytest.mark.parametrize("M,N,K", [(1, 64, 1), (1, 2048, 720), (1, 200, 4096), (2, 33, 5), (7, 100, 1000), (16, 300, 2080), (5, 40, 31), (16, 50, 9000), (3, 1024, 260), (1, 8300, 700), (13, 8193, 1100), (7, 5000, 600), (2, 17000, 300)])
 @pytest.mark.parametrize("pad,off", [(0, 0), (1, 1), (8, 3)])
 def test_f16_rows(lib, gpu, M, N, K, pad, off):
     """The bits of sh_mx4_quant and sh_gemm_mx4, and the product within its bound."""
