@@ -285,19 +285,19 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
 template <int BM, int BN, int WGM, int WGN>
 struct Tile {
     static constexpr int NW = WGM * WGN, TM = BM / WGM / 32, TN = BN / WGN / 32, NST = 4, ROWS = BM + BN;
-    static constexpr int CPW = ROWS / 16 / NW;                                        // DMAs of a wave: a slice's codes (16 rows each),
-    static constexpr int SPG = (ROWS / 64 + NW - 1) / NW, SPW = SPG;                  // the scales of four slices (64 rows), or a quarter of them by words (16 rows);
-                                                                                      // where there are fewer than waves, some are loaded twice
+    static constexpr int CPW = ROWS / 16 / NW;                                        // a wave's DMAs of a slice's codes (16 rows each)
+    static constexpr int SG = ROWS / 64, SW = ROWS / 16;                              // DMAs of four slices' scales: one a wave (64 rows), or by words four (16 rows),
+                                                                                      // one a slice; where there are fewer than waves, some are loaded twice
     static constexpr uint32_t CODE = ROWS * 64, SC = ROWS * 16, RING = NST * CODE, PITCH = BN * 4 + 16;
     static constexpr int PASSES = BM * PITCH <= 81920 ? 1 : 2;                        // of the sums through LDS
     static constexpr uint32_t STAGED = BM / PASSES * PITCH, LDS = RING + 3 * SC > STAGED ? RING + 3 * SC : STAGED;
-    static_assert(ROWS % (16 * NW) == 0 && SPG <= 2 && BN % 64 == 0 && TM % PASSES == 0 && BM % (32 * WGM) == 0 && BN % (32 * WGN) == 0 && LDS <= 163840, "tile");
+    static_assert(ROWS % (16 * NW) == 0 && SG <= NW && SW <= 4 * NW && BN % 64 == 0 && TM % PASSES == 0 && BM % (32 * WGM) == 0 && BN % (32 * WGN) == 0 && LDS <= 163840, "tile");
 };
 
 template <int BM, int BN, int WGM, int WGN, int PER, bool A16>
 __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
     using T = Tile<BM, BN, WGM, WGN>;
-    constexpr int NW = T::NW, TM = T::TM, TN = T::TN, NST = T::NST, CPW = T::CPW, SPG = T::SPG, SPW = T::SPW;
+    constexpr int NW = T::NW, TM = T::TM, TN = T::TN, NST = T::NST, CPW = T::CPW;
     extern __shared__ __align__(16) uint8_t smem[];
     const uint32_t lds0 = sh_lds_addr(smem), sc0 = lds0 + T::RING;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WGM, wn = wave / WGM;
@@ -334,29 +334,26 @@ __global__ __launch_bounds__(64 * WGM * WGN, PER) void k_mx4_tile(MxArgs a) {
         }
     };
     // Part `q` of the scales of slices 4 gr .. 4 gr + 3, of the last ones where there are none: rows of 16 bytes where these are aligned (A16), else words.
-    uint32_t soff[A16 ? SPG : 4 * SPW];
+    uint32_t soff[A16 ? 1 : 4];
 #pragma unroll
-    for (int i = 0; i < (A16 ? SPG : 4 * SPW); ++i) {
-        const uint32_t ins = A16 ? (wave * SPG + i) % (T::ROWS / 64) : ((i / SPW * NW + wave) * SPW + i % SPW) % (T::ROWS / 16), row = A16 ? ins * 64 + lane : ins * 16 + (lane >> 2);
-        soff[i] = row < BN ? min(row, wlim) * ldws : min(row - BN, xlim) * ldxs;
+    for (int q = 0; q < (A16 ? 1 : 4); ++q) {
+        const uint32_t row = A16 ? wave % T::SG * 64 + lane : (q * NW + wave) % T::SW * 16 + (lane >> 2);
+        soff[q] = row < BN ? min(row, wlim) * ldws : min(row - BN, xlim) * ldxs;
     }
     const auto load_scales = [&](uint32_t gr, auto part) {
         constexpr int Q = decltype(part)::value;
         const uint32_t at = sc0 + gr % 3 * T::SC;
-        if constexpr (A16) {
-            if constexpr (Q % 2 == 0 && Q / 2 < SPG) {
-                const uint32_t ins = (wave * SPG + Q / 2) % (T::ROWS / 64);
-                sh_lds_dma16_s((ins * 64 < BN ? ws : xs) + 16 * min(gr, (nd - 1) / 4), soff[Q / 2], at + ins * 1024);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < SPW; ++i) {
-                const uint32_t ins = ((Q * NW + wave) * SPW + i) % (T::ROWS / 16);
-                dma4_s(ins * 16 < BN ? ws : xs, soff[Q * SPW + i] + 4 * min(4 * gr + (lane & 3), nd - 1), at + ins * 256);
-            }
+        if constexpr (!A16) {
+            const uint32_t ins = (Q * NW + wave) % T::SW;
+            dma4_s(ins * 16 < BN ? ws : xs, soff[Q] + 4 * min(4 * gr + (lane & 3), nd - 1), at + ins * 256);
+        } else if constexpr (Q == 0) {
+            const uint32_t ins = wave % T::SG;
+            sh_lds_dma16_s((ins * 64 < BN ? ws : xs) + 16 * min(gr, (nd - 1) / 4), soff[0], at + ins * 1024);
         }
     };
-    constexpr int W2 = 2 * CPW + (A16 ? SPG / 2 : 2 * SPW), W3 = 3 * CPW + (A16 ? SPG / 2 : 3 * SPW);      // DMAs of two and of three slices in a row, at least
+    // What may be outstanding behind a slice that is waited for: two or three slices' codes, and by words the part of the scales that each slice brings behind
+    // its codes (its own, still, is waited for). By 16 bytes a group's scales go behind one slice's codes in four, and none are counted.
+    constexpr int W2 = 2 * CPW + (A16 ? 0 : 2), W3 = 3 * CPW + (A16 ? 0 : 3);
     const uint32_t lane_at = r32 * 64 + ((2 * g) ^ ((r32 >> 1 ^ (r32 >> 3 & 1)) & 3)) * 16;
     struct Ops { sh_u4v w[TN], x[TM]; };
     struct Scales { uint32_t w[TN], x[TM]; };
