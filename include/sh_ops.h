@@ -381,7 +381,8 @@ uint64_t sh_attention_kv_ws_bytes(const sh_kv_cache *c, uint32_t B, uint32_t row
 /* ---- rotary positions (no counterpart in the reference but sh_rope's formula) ---------------------------------------
  * The first `rot` columns of a head are turned in pairs by an angle that grows with the row's position: pair i by a =
  * 2 pi position step[i] / 2^64 (whole turns fall off), (x1, x2) -> (x1 c - x2 s, x2 c + x1 s) with c, s = mscale (cos a, sin a); the other
- * columns stay. Cosine and sine are rounded to fp32 from 64 bits, products and sums to fp32, the result to fp16, so no position is too far. */
+ * columns stay. Cosine and sine are rounded to fp32 from 64 bits, products and sums to fp32, the result to fp16: by given steps the farthest position is turned
+ * as exactly as the first. What a step is off counts once for each position (sh_rope_steps: 1.5e-16 turns, below). */
 enum { SH_ROPE_HALF = 0,      /* pair i: columns i and i + rot / 2 */
        SH_ROPE_PAIRS = 1 };   /* pair i: columns 2 i and 2 i + 1 */
 enum { SH_ROPE_NONE = 0, SH_ROPE_LINEAR = 1, SH_ROPE_BANDS = 2, SH_ROPE_RAMP = 3 };
@@ -400,6 +401,8 @@ typedef struct {
  *   SH_ROPE_BANDS   by the pair's turns n = ctx w_i / (2 pi) in the first context: 0 for n <= lo, 1 for n >= hi, linear in n between
  *   SH_ROPE_RAMP    by its index: 1 up to the index (rounded down, at least 0) whose pair turns hi times in it, 0 from that (rounded up, at most
  *                   rot - 1) of lo turns, linear in the index between
+ * Frequencies are computed in fp64: of w_i up to 1 a step is within 1.5e-16 turns of the formula's (for bands while hi^2 / (hi - lo) is far below ctx), a position's
+ * angle within that many times the position: 1e-9 rad at 2^20, 2e-6 at 2^31 - 1. A caller with exacter frequencies writes the steps.
  * 0, -1 for bad arguments (0 < lo < hi), SH_EHIP. */
 int sh_rope_steps(uint64_t step, uint32_t rot, double base, uint32_t scaling, double factor, double lo, double hi, uint32_t ctx);
 

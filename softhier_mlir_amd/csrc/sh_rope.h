@@ -12,8 +12,8 @@ struct RopePlan {
 // 0 and *out, or -1 with the message set. dh: the head's width.
 int sh_rope_check(const char *name, const sh_rope_plan *p, uint32_t dh, RopePlan *out);
 
-// (c, s) = m (cos, sin) of 2 pi phase / 2^64, phase = pos step mod 2^64: the whole turns fall off the product, so far positions lose
-// nothing. The phase is taken to the nearest quarter turn, the rest |a| <= pi / 4 goes through Taylor's series (sine to a^11,
+// (c, s) = m (cos, sin) of 2 pi phase / 2^64, phase = pos step mod 2^64: the whole turns fall off the product, so by a given step far positions
+// lose nothing (the step's own error counts pos times). The phase is taken to the nearest quarter turn, the rest |a| <= pi / 4 goes through Taylor's series (sine to a^11,
 // cosine to a^12: 7e-12 off at most), in fp64, whose rate is that of fp32 here. Rounded to fp32 once: other programs' 64-bit angles
 // give the same cosine and sine, but for one in thousands of far positions.
 __device__ __forceinline__ void rope_angle(uint32_t pos, uint64_t step, double m, float &c, float &s) {

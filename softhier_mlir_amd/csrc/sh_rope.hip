@@ -18,7 +18,8 @@ namespace {
 
 struct StepArgs { uint64_t *step; uint32_t pairs, scaling, ctx; double base, factor, lo, hi; };
 
-// One thread a pair, in fp64; once for a model.
+// One thread a pair, in fp64; once for a model (3.4 us). w is off by (|ln w| + 8) 2^-53 of itself at most: its exponent's rounding, two steps of the power, three
+// more operations; turns by 1.5e-16 at most, where w is 1.
 __global__ void k_rope_steps(StepArgs a) {
     const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= a.pairs) return;
