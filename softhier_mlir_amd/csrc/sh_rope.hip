@@ -70,7 +70,7 @@ int sh_rope_steps(uint64_t step, uint32_t rot, double base, uint32_t scaling, do
     if (rot < 2 || rot % 2 || rot > 65536) { sh_set_error(-1, "[sh_rope_steps] %u turned columns (even, 2 .. 65536)", rot); return -1; }
     if (!std::isfinite(base) || base <= 1.0) { sh_set_error(-1, "[sh_rope_steps] base %g (greater than 1)", base); return -1; }
     if (scaling > SH_ROPE_RAMP) { sh_set_error(-1, "[sh_rope_steps] unknown scaling %u", scaling); return -1; }
-    if (scaling != SH_ROPE_NONE && !(std::isfinite(factor) && factor > 0.0)) { sh_set_error(-1, "[sh_rope_steps] factor %g", factor); return -1; }
+    if (scaling != SH_ROPE_NONE && !(std::isfinite(factor) && factor > 0.0 && std::isfinite(1.0 / factor))) { sh_set_error(-1, "[sh_rope_steps] factor %g", factor); return -1; }
     if (scaling >= SH_ROPE_BANDS && !(lo > 0.0 && hi > lo && std::isfinite(hi) && ctx)) {
         sh_set_error(-1, "[sh_rope_steps] turns %g .. %g of a context of %u", lo, hi, ctx);
         return -1;
