@@ -371,7 +371,7 @@ __global__ __launch_bounds__(NT) void k_kv_append(AppendArgs a) {
 // workgroups. A thread's eight columns of a key are four pairs of each of its four tokens, and it keeps their cosines and sines (fp64, about 180
 // cycles a wave each) for `kh` heads, the next head's halves on their way while one is stored: of 17 thousand rows of 32 + 8 heads of 128, 78.6 us (4.1 TB/s) with
 // four heads, 82.2 with two, 126 with one. Three waves a SIMD hold too little in flight for more: queries spread among the workgroups that append, so that both
-// run at once, made it slower (88.5). 64 single rows 5.6 us, one launch: slots and positions, then rows and scales, then codes.
+// run at once, made it slower (88.5). 64 single rows 5.3 us, one launch: slots and positions, then rows and scales, then codes.
 struct AppendRopeArgs {
     AppendArgs a;
     RopeArgs q;                            // rows turned for themselves

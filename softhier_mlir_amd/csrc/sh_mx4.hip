@@ -224,7 +224,9 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
         sh_u4v x[MT][SU];
         int sx[MT];
         const uint32_t keep = load(u);
-        if constexpr (F16)                                                     // (loads and work of their own, while the codes are on their way)
+        // Halves are issued behind the codes' DMAs, and loads are counted off in order: the first wait for a half is one for all of the unit's codes, and
+        // the conversion stands behind them. With few rows the lanes n repeat a row, and its conversion.
+        if constexpr (F16)
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const uint16_t *row = a.x + min(m0 + 16 * i + n, a.M - 1) * a.ldx;
@@ -278,10 +280,11 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_rows(MxArgs a) {
 // slices (16 bytes of a row) into a ring of three. A slice is two steps of 64 k; a step's operands are read while the last step multiplies, and the barrier that frees
 // a stage lies between the two, so that no wave meets it without products to issue. Chunk c of a row lies at c ^ ((row / 2 ^ row / 8 % 2) % 4) of its 64 bytes, so
 // that neither eight nor sixteen lanes in a row meet in a bank (row / 2 % 4 alone: twice the conflicts). Behind the last block the codes are those of the last one again and both scales 2^-127: their product is 0 in fp32.
-// Bound by what L2 gives the CUs (12 TB/s at most was seen here, in lines or halves of them alike: 256 columns a slice in two stages, or a line of 128 bytes a row in four,
-// were no faster) and, in large problems, by power: 8192^3, 298 us, 3.7 PFLOP/s at 1.78 GHz, matrix pipe busy 47 %; the pipe alone, fed from registers, gives 6.3 PFLOP/s
-// of random codes and 9.7 of zeros. Eight waves share a 256 x 256 tile (four, with twice the registers each: 302 us); of the 73 us that a round of tiles takes
-// there, 10 are its start and its end.
+// Large problems are bound by power and by what the two waves of a SIMD wait: 8192^3, 290 to 300 us, 3.7 PFLOP/s at 1.78 GHz, matrix pipe busy 47 %; the pipe alone, fed
+// from registers, gives 6.3 PFLOP/s of random codes and 9.7 of zeros. Eight waves share a 256 x 256 tile (four, with twice the registers each: 302 us); of the 73 us
+// that a round of tiles takes there, 10 are its start and its end. One round of small tiles is bound by its start, its end and one workgroup of four waves a CU: 700 x 5000
+// x 2880, 15.7 us, pipe busy 11 %. L2 bounds neither: a kernel of these DMAs alone gets 22 TB/s of whole lines, 17 to 19 of half lines and 14 of rows of 1440 bytes, every
+// second half of which lies over two lines; the two take 7.6 (of 17) and 6.0 (of 14). 256 columns a slice in two stages, or a line of 128 bytes a row in four, were no faster.
 template <int BM, int BN, int WGM, int WGN>
 struct Tile {
     static constexpr int NW = WGM * WGN, TM = BM / WGM / 32, TN = BN / WGN / 32, NST = 4, ROWS = BM + BN;
@@ -664,7 +667,8 @@ int sh_gemm_mx4(uint64_t xc, uint64_t xs, uint64_t wc, uint64_t ws, uint64_t z, 
     a.xc = (const uint8_t *)xc; a.xs = (const uint8_t *)xs;
     a.ldxc = ldxc; a.ldxs = ldxs;
     const hipStream_t st = sh_stream();
-    // Tiles by the rounds of workgroups that they take on 256 CUs. Times (us, K = 4096, epilogue without residual) of the first round and of a further one: small
+    // Tiles by the rounds of workgroups that they take on 256 CUs, whatever K: a workgroup has all of it, so few tiles of a long K leave CUs idle (128 x 1024, 32 tiles:
+    // K = 4096 6.8 us, 16384 24.4). Times (us, K = 4096, epilogue without residual) of the first round and of a further one: small
     // tiles' workgroups share a CU. 2048 x 4096: 47 / 40 / 30 / 27.5 / 31.5; 1000 x 2048: 14.4 / 13.6 / 15.0 / 21 / 29; 300 x 4096: 12.0 / 11.8 / 13.7 / 20 / 27;
     // 100 x 4096: 8.0 / 10.3 / 12.0 / 17 / 24; 700 x 5000 (K = 2880): 22 / 18.5 / 15.3 / 19.7 / 26; 4096 x 4096: 87 / 70 / 55 / 51 / 41.
     struct Shape { uint32_t bm, bn; double first, more; };
@@ -679,7 +683,8 @@ int sh_gemm_mx4(uint64_t xc, uint64_t xs, uint64_t wc, uint64_t ws, uint64_t z, 
     const bool near = ldxc <= (1u << 24) && ldwc <= (1u << 24) && ldxs <= (1u << 24) && ldws <= (1u << 24);       // a tile's rows within 32-bit offsets
     bool ok = true;
     // Up to 64 rows the chain is shared by a workgroup's waves; more than 32 of many columns fill the GPU as tiles (64 rows of 4096 x 6144: 9.4 us, 10.7 so; 48 of
-    // 2880 x 5000 7.1 and 8.6; but 64 of 4096 x 4096 9.1 and 5.9, of 8192 x 2048 13.8 and 7.9).
+    // 2880 x 5000 7.1 and 8.6; but 64 of 4096 x 4096 9.1 and 5.9, of 8192 x 2048 13.8 and 7.9). Rows too far apart for a tile's offsets take the kernel for few rows
+    // however many there are (700 x 1024 x 2880 7.1 us, 12.4 so).
     if (M <= 16) ok = launch_rows<1, false>(a, st);
     else if (M <= 32) ok = launch_rows<2, false>(a, st);
     else if ((M <= 64 && N <= 4096) || !near) ok = launch_rows<4, false>(a, st);

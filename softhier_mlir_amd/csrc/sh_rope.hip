@@ -37,7 +37,8 @@ __global__ void k_rope_steps(StepArgs a) {
     a.step[i] = (uint64_t)rint((turns - floor(turns)) * 0x1p64);
 }
 
-// Bound by HBM where rows are many (16 thousand rows, 328 MB: 66 us, 5.0 TB/s; all columns turned 63), else by the launch (64 rows 3.8 us).
+// Bound by HBM where rows are many (16 thousand rows, 328 MB: 66 us, 5.0 TB/s; all columns turned 63), else by the launch (64 rows 3.3 to 3.9 us). Turned columns that are no
+// multiple of 8 go pair by pair, two bytes a lane (16 thousand rows of 40 heads of 80, 205 MB: 20 turned 76 us, 16 turned 56).
 template <int P>
 __global__ __launch_bounds__(256) void k_rope_pos(RopeArgs a) { rope_rows<P>(a, blockIdx.x * 256u + threadIdx.x); }
 
