@@ -101,8 +101,8 @@ def _run(lib, x, w, K, wide, bias=None, bias32=False, act=0, residual=None, cpad
 
 
 def _check(got, x, w, bias=None, gelu=False, residual=None):
-    """Rounding to fp16 (half a step, 2^-11, twice with a residual). Sums of exact products in fp32: up to 64 terms within an instruction, a chain of
-    an instruction's sums (K / 64) and eight more operations, each at most 2^-23 of sum |x w| (the matrix pipe may cut instead of rounding);
+    """Rounding to fp16 (half a step, 2^-11, twice with a residual). Sums of exact products in fp32: within an instruction up to 128 terms (few rows; 64
+    in tiles), a chain of an instruction's sums (K / 64 at most), eight waves' (few rows) and eight more operations, each at most 2^-23 of sum |x w| (the matrix pipe may cut instead of rounding);
     GELU's slope is below 1.13, and its hardware exp2 and reciprocal add 2^-19 of the result and 2^-22."""
     import torch
     xv, wv = _value(*x), _value(*w)
@@ -110,7 +110,7 @@ def _check(got, x, w, bias=None, gelu=False, residual=None):
     if bias is not None:
         b = torch.from_numpy(bias).cuda().double()
         z, s = z + b, s + b.abs()
-    d = (64 + xv.shape[1] / 64 + 8) * 2.0 ** -23 * s
+    d = (128 + xv.shape[1] / 64 + 16) * 2.0 ** -23 * s
     if gelu:
         z = 0.5 * z * (1 + torch.tanh(np.sqrt(2 / np.pi) * (z + 0.044715 * z ** 3)))
         d = 1.13 * d + 2.0 ** -19 * z.abs() + 2.0 ** -22
